@@ -18,6 +18,7 @@ at::ScalarType toTorchDType(DType dtype) {
     case DType::BFloat16: return at::kBFloat16;
     case DType::Float16: return at::kHalf;
     case DType::Int32: return at::kInt;
+    case DType::UInt8: return at::kByte;
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -29,6 +30,7 @@ DType fromTorchDType(at::ScalarType dtype) {
     case at::kBFloat16: return DType::BFloat16;
     case at::kHalf: return DType::Float16;
     case at::kInt: return DType::Int32;
+    case at::kByte: return DType::UInt8;
     default: break;
   }
   throw std::invalid_argument(std::string("unsupported torch tensor dtype: ") +
@@ -64,6 +66,8 @@ DType dtypeOf<std::int64_t>() { return DType::Int64; }
 template <>
 DType dtypeOf<std::int32_t>() { return DType::Int32; }
 template <>
+DType dtypeOf<std::uint8_t>() { return DType::UInt8; }
+template <>
 DType dtypeOf<at::BFloat16>() { return DType::BFloat16; }
 template <>
 DType dtypeOf<at::Half>() { return DType::Float16; }
@@ -91,6 +95,7 @@ std::string toString(DType dtype) {
     case DType::BFloat16: return "bfloat16";
     case DType::Float16: return "float16";
     case DType::Int32: return "int32";
+    case DType::UInt8: return "uint8";
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -101,6 +106,7 @@ DType dtypeFromString(const std::string& dtype) {
   if (dtype == "bfloat16" || dtype == "bf16") return DType::BFloat16;
   if (dtype == "float16" || dtype == "f16") return DType::Float16;
   if (dtype == "int32" || dtype == "i32") return DType::Int32;
+  if (dtype == "uint8" || dtype == "u8") return DType::UInt8;
   throw std::invalid_argument("unsupported dtype: " + dtype);
 }
 
@@ -111,6 +117,7 @@ std::size_t byteSize(DType dtype) {
     case DType::BFloat16: return 2;
     case DType::Float16: return 2;
     case DType::Int32: return 4;
+    case DType::UInt8: return 1;
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -237,6 +244,8 @@ template std::int64_t* Tensor::data<std::int64_t>();
 template const std::int64_t* Tensor::data<std::int64_t>() const;
 template std::int32_t* Tensor::data<std::int32_t>();
 template const std::int32_t* Tensor::data<std::int32_t>() const;
+template std::uint8_t* Tensor::data<std::uint8_t>();
+template const std::uint8_t* Tensor::data<std::uint8_t>() const;
 template at::BFloat16* Tensor::data<at::BFloat16>();
 template const at::BFloat16* Tensor::data<at::BFloat16>() const;
 template at::Half* Tensor::data<at::Half>();

@@ -1,0 +1,163 @@
+// Entry points of the microscaled operators (declared in include/dli_hip.h): argument checks,
+// launch geometry and the launch of the matching gfx950 kernel.
+#include <string>
+
+#include "runtime.h"
+
+namespace dli::hip {
+namespace {
+
+int badArg(const char* op, const std::string& what) {
+  return fail(DLI_HIP_EINVAL, std::string(op) + ": " + what);
+}
+
+bool aligned(const void* p, uintptr_t bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+int dtypeIndex(int dtype) {
+  return dtype == DLI_F32 ? 0 : dtype == DLI_BF16 ? 1 : dtype == DLI_F16 ? 2 : -1;
+}
+
+// The kernels <base>_<fp8|fp4>_<f32|bf16|f16> and, for data of any alignment, <...>_any.
+struct MxKernels {
+  DeviceKernel k[2][2][3];  // [any][format][dtype]
+#define DLI_MX_NAMES(base, any)                                                          \
+  {                                                                                      \
+    {{"mx_quantize", base "_fp8_f32" any}, {"mx_quantize", base "_fp8_bf16" any},        \
+     {"mx_quantize", base "_fp8_f16" any}},                                              \
+        {{"mx_quantize", base "_fp4_f32" any}, {"mx_quantize", base "_fp4_bf16" any},    \
+         {"mx_quantize", base "_fp4_f16" any}}                                           \
+  }
+};
+
+MxKernels k_quantize{{DLI_MX_NAMES("mx_quantize", ""), DLI_MX_NAMES("mx_quantize", "_any")}};
+MxKernels k_dequantize{{DLI_MX_NAMES("mx_dequantize", ""), DLI_MX_NAMES("mx_dequantize", "_any")}};
+MxKernels k_rms_norm{{DLI_MX_NAMES("rms_norm_mx", ""), DLI_MX_NAMES("rms_norm_mx", "_any")}};
+MxKernels k_silu_mul{{DLI_MX_NAMES("silu_mul_mx", ""), DLI_MX_NAMES("silu_mul_mx", "_any")}};
+DeviceKernel k_linear_tile[2][3] = {{{"mx_linear", "mx_linear_tile_fp8_f32"},
+                                     {"mx_linear", "mx_linear_tile_fp8_bf16"},
+                                     {"mx_linear", "mx_linear_tile_fp8_f16"}},
+                                    {{"mx_linear", "mx_linear_tile_fp4_f32"},
+                                     {"mx_linear", "mx_linear_tile_fp4_bf16"},
+                                     {"mx_linear", "mx_linear_tile_fp4_f16"}}};
+
+// 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
+int checkTensor(const char* op, int dtype, int format, int64_t rows, int64_t k, const char* name) {
+  if (dtypeIndex(dtype) < 0)
+    return badArg(op, "unsupported dtype code " + std::to_string(dtype));
+  if (format != DLI_MX_FP8 && format != DLI_MX_FP4)
+    return badArg(op, "unsupported format " + std::to_string(format));
+  if (rows < 0 || k < 0) return badArg(op, "negative size");
+  if (k % 32 != 0) return badArg(op, std::string(name) + " must be a multiple of 32");
+  // element counts, offsets in bytes and chunk counts stay far inside 63 bits
+  if (k > 0 && rows > (int64_t{1} << 56) / k) return badArg(op, "tensor is too large");
+  return 0;
+}
+
+// Grid-stride launches of one chunk (8 values) per thread: enough blocks to fill 256 CUs.
+unsigned chunkBlocks(int64_t chunks) {
+  const int64_t blocks = (chunks + 255) / 256;
+  return static_cast<unsigned>(blocks < 8192 ? blocks : 8192);
+}
+
+}  // namespace
+}  // namespace dli::hip
+
+using namespace dli::hip;
+
+extern "C" {
+
+int dli_hip_mx_quantize(int dtype, int format, const void* x, void* codes, void* scales,
+                        int64_t rows, int64_t k, void* stream) {
+  const char* op = "mx_quantize";
+  if (int rc = checkTensor(op, dtype, format, rows, k, "k")) return rc;
+  if (rows == 0 || k == 0) return 0;
+  if (x == nullptr || codes == nullptr || scales == nullptr) return badArg(op, "NULL pointer");
+  const int any = aligned(x, 16) && aligned(codes, 8) ? 0 : 1;
+  const int64_t chunks = rows * (k / 8);
+  return launch(k_quantize.k[any][format][dtypeIndex(dtype)], {chunkBlocks(chunks)}, {256}, 0,
+                stream, x, codes, scales, chunks);
+}
+
+int dli_hip_mx_dequantize(int dtype, int format, const void* codes, const void* scales, void* out,
+                          int64_t rows, int64_t k, void* stream) {
+  const char* op = "mx_dequantize";
+  if (int rc = checkTensor(op, dtype, format, rows, k, "k")) return rc;
+  if (rows == 0 || k == 0) return 0;
+  if (out == nullptr || codes == nullptr || scales == nullptr) return badArg(op, "NULL pointer");
+  const int any = aligned(out, 16) && aligned(codes, 8) ? 0 : 1;
+  const int64_t chunks = rows * (k / 8);
+  return launch(k_dequantize.k[any][format][dtypeIndex(dtype)], {chunkBlocks(chunks)}, {256}, 0,
+                stream, codes, scales, out, chunks);
+}
+
+int dli_hip_rms_norm_mx(int dtype, int format, const void* x, const void* residual,
+                        const void* weight, void* hidden_out, void* codes, void* scales,
+                        int64_t rows, int64_t hidden, float eps, void* stream) {
+  const char* op = "rms_norm_mx";
+  if (int rc = checkTensor(op, dtype, format, rows, hidden, "hidden")) return rc;
+  if (hidden == 0) return badArg(op, "hidden must be positive");
+  if (rows == 0) return 0;
+  if (x == nullptr || weight == nullptr || codes == nullptr || scales == nullptr)
+    return badArg(op, "NULL pointer");
+  const int any = aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) &&
+                          aligned(hidden_out, 16) && aligned(codes, 8)
+                      ? 0
+                      : 1;
+  const unsigned blocks = static_cast<unsigned>(rows < 65535 ? rows : 65535);
+  return launch(k_rms_norm.k[any][format][dtypeIndex(dtype)], {blocks}, {256}, 0, stream, x,
+                residual, weight, hidden_out, codes, scales, rows, hidden, eps);
+}
+
+int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up, int64_t stride,
+                        void* codes, void* scales, int64_t rows, int64_t ffn, void* stream) {
+  const char* op = "silu_mul_mx";
+  if (int rc = checkTensor(op, dtype, format, rows, ffn, "ffn")) return rc;
+  if (stride < ffn) return badArg(op, "stride must be at least ffn");
+  if (stride > 0 && rows > (int64_t{1} << 56) / stride) return badArg(op, "tensor is too large");
+  if (rows == 0 || ffn == 0) return 0;
+  if (gate == nullptr || up == nullptr || codes == nullptr || scales == nullptr)
+    return badArg(op, "NULL pointer");
+  const int any = aligned(gate, 16) && aligned(up, 16) && aligned(codes, 8) &&
+                          (dtype == DLI_F32 ? stride % 4 : stride % 8) == 0
+                      ? 0
+                      : 1;
+  const int64_t row_chunks = ffn / 8;
+  return launch(k_silu_mul.k[any][format][dtypeIndex(dtype)], {chunkBlocks(rows * row_chunks)},
+                {256}, 0, stream, gate, up, stride, codes, scales, rows, row_chunks);
+}
+
+size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k) {
+  (void)x_format;
+  (void)m;
+  (void)n;
+  (void)k;
+  return 0;
+}
+
+int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
+                      const void* w_codes, const void* w_scales, const void* bias,
+                      const void* residual, void* out, int64_t m, int64_t n, int64_t k,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "mx_linear";
+  (void)workspace;
+  (void)workspace_bytes;
+  if (int rc = checkTensor(op, out_dtype, x_format, m, k, "k")) return rc;
+  if (int rc = checkTensor(op, out_dtype, x_format, n, k, "k")) return rc;
+  if (k == 0) return badArg(op, "k must be positive");
+  if (n > 0 && m > (int64_t{1} << 56) / n) return badArg(op, "output is too large");
+  if (m == 0 || n == 0) return 0;
+  if (m > 65535 * int64_t{16} || n > (int64_t{1} << 31) - 64)
+    return badArg(op, "m must be at most 1048560, n below 2^31 - 64");
+  if (x_codes == nullptr || x_scales == nullptr || w_codes == nullptr || w_scales == nullptr ||
+      out == nullptr)
+    return badArg(op, "NULL pointer");
+  if (!aligned(x_codes, 16) || !aligned(w_codes, 16))
+    return badArg(op, "codes must be 16-byte aligned");
+  return launch(k_linear_tile[x_format][dtypeIndex(out_dtype)],
+                {blocksFor(n, 64), blocksFor(m, 16)}, {256}, 0, stream, x_codes, x_scales, w_codes,
+                w_scales, bias, residual, out, m, n, k);
+}
+
+}  // extern "C"

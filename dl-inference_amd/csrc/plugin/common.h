@@ -23,6 +23,7 @@ inline int hipDtype(DType dtype) {
     case DType::BFloat16: return DLI_BF16;
     case DType::Float16: return DLI_F16;
     case DType::Int32: return DLI_I32;
+    case DType::UInt8: return DLI_U8;
   }
   throw std::invalid_argument("unknown dtype");
 }
@@ -127,5 +128,6 @@ void add(OperatorRegistry* registry) {
 // Registration hooks of the plugin's source files.
 void registerReferenceOps(OperatorRegistry* registry);
 void registerFusedOps(OperatorRegistry* registry);
+void registerMxOps(OperatorRegistry* registry);
 
 }  // namespace dli::plugin

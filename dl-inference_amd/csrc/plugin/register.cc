@@ -9,6 +9,7 @@ extern "C" __attribute__((visibility("default"))) bool dli_register_operators(
   try {
     dli::plugin::registerReferenceOps(registry);
     dli::plugin::registerFusedOps(registry);
+    dli::plugin::registerMxOps(registry);
     return true;
   } catch (...) {
     return false;

@@ -1,6 +1,6 @@
 // ATen CPU reference plugin (lib/libdli_aten_ops.so): the reference plugin's 16 operator names
-// (python/dli_ops/aot/*/template.cc), plus the decode graph's argmax, implemented with ATen on
-// host tensors. It runs the same dli.graph.v1 graphs as the gfx950 plugin through the same
+// (python/dli_ops/aot/*/template.cc), plus the decode graph's argmax and the
+// microscaled operators, implemented with ATen on host tensors. It runs the same dli.graph.v1 graphs as the gfx950 plugin through the same
 // Engine, so the CPU time of a graph is measured on the reference's own runtime path (Engine ->
 // registry -> operator), with ATen's CPU kernels in place of the device kernels.
 //
@@ -9,6 +9,7 @@
 // and rounds its output to the input dtype once, the rounding points of the device path. The
 // paged KV cache keeps host entries (include/dli/kv_cache.h: one block per sequence).
 #include <ATen/ATen.h>
+#include <ATen/TensorIndexing.h>
 
 #include <cmath>
 #include <memory>
@@ -435,6 +436,187 @@ class ArgmaxOp final : public Operator {
   }
 };
 
+// Microscaled tensors (include/dli_hip.h, section 4) on the host: the same values as the gfx950
+// operators, from elementary ATen operations.
+constexpr std::int64_t kMxBlock = 32;
+
+bool mxIsFp8(const Attributes& attrs, const std::string& op) {
+  const std::string format = attrs.value_or<std::string>("format", "fp8");
+  if (format != "fp8" && format != "fp4")
+    throw std::invalid_argument(op + " format must be fp8 or fp4, not " + format);
+  return format == "fp8";
+}
+
+// Quantises y [.., K] in fp32 into codes and scales.
+void mxQuantize(const at::Tensor& y, bool fp8, const std::string& op, Tensor& codes_out,
+                Tensor& scales_out) {
+  const std::int64_t k = y.size(-1);
+  if (k <= 0 || k % kMxBlock != 0)
+    throw std::invalid_argument(op + ": the last dimension must be a positive multiple of 32");
+  std::vector<std::int64_t> shape(y.sizes().begin(), y.sizes().end());
+  const at::Tensor blocks = y.reshape({-1, kMxBlock}).contiguous();
+  const at::Tensor bits = blocks.view(at::kInt).bitwise_and(0x7FFFFFFF).amax(-1);
+  const at::Tensor exponent = bits.bitwise_right_shift(23);
+  const at::Tensor bad = exponent.eq(255);
+  const at::Tensor code = at::where(bad, 255, (exponent - (fp8 ? 8 : 2)).clamp_min(0));
+  const at::Tensor inverse = (254 - code).clamp_min(1).bitwise_left_shift(23).view(at::kFloat);
+  const double largest = fp8 ? 448.0 : 6.0;
+  const at::Tensor v = (blocks * inverse.unsqueeze(-1))
+                           .clamp(-largest, largest)
+                           .masked_fill(bad.unsqueeze(-1), 0.0);
+  at::Tensor codes;
+  if (fp8) {
+    codes = v.to(at::kFloat8_e4m3fn).view(at::kByte).reshape(shape);
+  } else {
+    const at::Tensor a = v.abs();
+    // below 2 elements lie 1/2 apart, below 4 1, then 2; at::round takes ties to even
+    const at::Tensor e = at::where(
+        a.lt(2), at::round(a * 2), at::where(a.lt(4), at::round(a) + 2, at::round(a / 2) + 4));
+    const at::Tensor nibbles =
+        (e.clamp_max(7) + 8 * at::signbit(v).to(at::kFloat)).to(at::kByte).reshape({-1, 2});
+    shape.back() = k / 2;
+    codes = (nibbles.select(1, 0) + nibbles.select(1, 1) * 16).reshape(shape);
+  }
+  shape.back() = k / kMxBlock;
+  codes_out = Tensor(codes.contiguous());
+  scales_out = Tensor(code.to(at::kByte).reshape(shape).contiguous());
+}
+
+// The values [.., K] of codes and scales in fp32; *fp4 tells the format.
+at::Tensor mxValues(const Tensor& codes, const Tensor& scales, const std::string& op, bool* fp4) {
+  if (codes.dtype() != DType::UInt8 || scales.dtype() != DType::UInt8)
+    throw std::invalid_argument(op + " codes and scales must be uint8");
+  const std::int64_t s = scales.shape().back(), c = codes.shape().back();
+  bool same = codes.rank() == scales.rank() && s > 0 && (c == s * 32 || c == s * 16);
+  for (std::size_t i = 0; same && i + 1 < codes.rank(); ++i) same = codes.dim(i) == scales.dim(i);
+  if (!same)
+    throw std::invalid_argument(op + ": codes " + formatShape(codes.shape()) + " and scales " +
+                                formatShape(scales.shape()) + " are not a microscaled tensor");
+  *fp4 = c == s * 16;
+  at::Tensor e;
+  if (*fp4) {
+    const at::Tensor b = codes.torchTensor().to(at::kLong).reshape({-1, 1});
+    const at::Tensor table = at::tensor({0.f, .5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f, -0.f, -.5f, -1.f,
+                                         -1.5f, -2.f, -3.f, -4.f, -6.f});
+    e = table.index({at::cat({b.bitwise_and(15), b.bitwise_right_shift(4)}, 1)});
+  } else {
+    e = codes.torchTensor().view(at::kFloat8_e4m3fn).to(at::kFloat);
+  }
+  const at::Tensor code = scales.torchTensor().reshape({-1, 1});
+  const at::Tensor scale = at::exp2(code.to(at::kDouble) - 127.0)
+                               .to(at::kFloat)
+                               .masked_fill(code.eq(255), std::nanf(""));
+  std::vector<std::int64_t> shape(codes.shape());
+  shape.back() = s * kMxBlock;
+  return (e.reshape({-1, kMxBlock}) * scale).reshape(shape);
+}
+
+class MxQuantizeOp final : public Operator {
+ public:
+  std::string type() const override { return "mx_quantize"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext&) const override {
+    requireArity(in, out, 1, 1, 2, type());
+    requireFloating(*in[0], type());
+    mxQuantize(f32(*in[0]), mxIsFp8(attrs, type()), type(), *out[0], *out[1]);
+  }
+};
+
+class MxDequantizeOp final : public Operator {
+ public:
+  std::string type() const override { return "mx_dequantize"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext&) const override {
+    requireArity(in, out, 2, 2, 1, type());
+    const DType dtype = dtypeFromString(attrs.value_or<std::string>("dtype", "bfloat16"));
+    if (!isFloating(dtype)) throw std::invalid_argument(type() + " dtype must be a floating type");
+    bool fp4 = false;
+    *out[0] = result(mxValues(*in[0], *in[1], type(), &fp4), dtype);
+  }
+};
+
+class RmsNormMxOp final : public Operator {
+ public:
+  std::string type() const override { return "rms_norm_mx"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext&) const override {
+    requireArity(in, out, 2, 3, in.size() == 3 ? 3 : 2, type());
+    requireFloating(*in[0], type());
+    requireSameDType(*in[0], *in[1], type());
+    if (static_cast<std::int64_t>(in[1]->numel()) != in[0]->shape().back())
+      throw std::invalid_argument("rms_norm_mx weight size must match the last input dim");
+    const auto eps = static_cast<float>(attrDouble(attrs, "eps", 1e-6));
+    at::Tensor h = f32(*in[0]);
+    if (in.size() == 3) {
+      requireSameDType(*in[0], *in[2], type());
+      if (!sameShape(*in[0], *in[2]))
+        throw std::invalid_argument("rms_norm_mx residual must have the shape of x");
+      *out[2] = result(h + f32(*in[2]), in[0]->dtype());
+      h = f32(*out[2]);
+    }
+    const at::Tensor mean = h.to(at::kDouble).square().mean(-1, true);
+    const at::Tensor inv = at::reciprocal(at::sqrt(mean + static_cast<double>(eps))).to(at::kFloat);
+    mxQuantize(h * inv * f32(*in[1]).reshape({-1}), mxIsFp8(attrs, type()), type(), *out[0],
+               *out[1]);
+  }
+};
+
+class SiluMulMxOp final : public Operator {
+ public:
+  std::string type() const override { return "silu_mul_mx"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext&) const override {
+    requireArity(in, out, 1, 2, 2, type());
+    requireFloating(*in[0], type());
+    at::Tensor gate = f32(*in[0]), up;
+    if (in.size() == 2) {
+      requireSameDType(*in[0], *in[1], type());
+      if (!sameShape(*in[0], *in[1]))
+        throw std::invalid_argument("silu_mul_mx gate and up must have one shape");
+      up = f32(*in[1]);
+    } else {
+      if (gate.size(-1) % 2 != 0)
+        throw std::invalid_argument("silu_mul_mx: a joined gate and up has an even last dimension");
+      const std::vector<at::Tensor> halves = gate.chunk(2, -1);
+      gate = halves[0];
+      up = halves[1];
+    }
+    mxQuantize(gate / (1 + at::exp(-gate)) * up, mxIsFp8(attrs, type()), type(), *out[0], *out[1]);
+  }
+};
+
+class MxLinearOp final : public Operator {
+ public:
+  std::string type() const override { return "mx_linear"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext&) const override {
+    const bool has_residual = attrs.value_or<bool>("residual", false);
+    requireArity(in, out, has_residual ? 5 : 4, has_residual ? 6 : 5, 1, type());
+    bool x4 = false, w4 = false;
+    const at::Tensor x = mxValues(*in[0], *in[1], type(), &x4);
+    if (in[2]->rank() != 2) throw std::invalid_argument("mx_linear weight must be 2-D");
+    const at::Tensor w = mxValues(*in[2], *in[3], type(), &w4);
+    if (!w4) throw std::invalid_argument("mx_linear weight must be fp4");
+    if (x.size(-1) != w.size(1))
+      throw std::invalid_argument("mx_linear weight shape " + formatShape(in[2]->shape()) +
+                                  " does not match input " + formatShape(in[0]->shape()));
+    const DType dtype = dtypeFromString(attrs.value_or<std::string>("out_dtype", "bfloat16"));
+    if (!isFloating(dtype)) throw std::invalid_argument("mx_linear out_dtype must be a floating type");
+    at::Tensor y = at::matmul(x, w.t());
+    if (in.size() == (has_residual ? 6u : 5u)) {
+      if (in[4]->dtype() != dtype || static_cast<std::int64_t>(in[4]->numel()) != w.size(0))
+        throw std::invalid_argument("mx_linear bias must have the output features and out_dtype");
+      y = y + f32(*in[4]).reshape({-1});
+    }
+    if (has_residual) {
+      if (in.back()->dtype() != dtype || in.back()->torchTensor().sizes() != y.sizes())
+        throw std::invalid_argument("mx_linear residual must have the output's shape and out_dtype");
+      y = y + f32(*in.back());
+    }
+    *out[0] = result(y, dtype);
+  }
+};
+
 template <typename Op>
 void add(OperatorRegistry* registry) {
   registry->registerFactory(Op().type(), [] { return std::make_unique<Op>(); });
@@ -466,6 +648,11 @@ extern "C" __attribute__((visibility("default"))) bool dli_register_operators(
     add<MaxPool2dOp>(registry);
     add<BatchNorm2dOp>(registry);
     add<ArgmaxOp>(registry);
+    add<MxQuantizeOp>(registry);
+    add<MxDequantizeOp>(registry);
+    add<RmsNormMxOp>(registry);
+    add<SiluMulMxOp>(registry);
+    add<MxLinearOp>(registry);
     return true;
   } catch (...) {
     return false;

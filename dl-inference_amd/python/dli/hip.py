@@ -13,9 +13,10 @@ import torch
 
 from . import hip_library_path
 
-F32, I64, BF16, F16, I32 = 0, 1, 2, 3, 4
+F32, I64, BF16, F16, I32, U8 = 0, 1, 2, 3, 4, 5
+MX_FP8, MX_FP4 = 0, 1
 _TORCH_CODES = {torch.float32: F32, torch.int64: I64, torch.bfloat16: BF16, torch.float16: F16,
-                torch.int32: I32}
+                torch.int32: I32, torch.uint8: U8}
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -116,6 +117,15 @@ _SIGNATURES = {
                               _c_void_p] + [_i64] * 9 + [_float, _int, _c_void_p, _size,
                                                          _c_void_p, _c_void_p, _c_void_p],
     "dli_hip_decoder_stack_status": [_c_void_p, ctypes.POINTER(_int), _c_void_p],
+    "dli_hip_mx_quantize": [_int, _int, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _c_void_p],
+    "dli_hip_mx_dequantize": [_int, _int, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                              _c_void_p],
+    "dli_hip_rms_norm_mx": [_int, _int] + [_c_void_p] * 6 + [_i64, _i64, _float, _c_void_p],
+    "dli_hip_silu_mul_mx": [_int, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64,
+                            _i64, _c_void_p],
+    "dli_hip_mx_linear_workspace": [_int, _i64, _i64, _i64],
+    "dli_hip_mx_linear": [_int, _int] + [_c_void_p] * 7 + [_i64] * 3 + [_c_void_p, _size,
+                                                                        _c_void_p],
     "dli_hip_stream_is_capturing": [_c_void_p, ctypes.POINTER(_int)],
 }
 _RESTYPES = {
@@ -124,6 +134,7 @@ _RESTYPES = {
     "dli_hip_target_arch": ctypes.c_char_p,
     "dli_hip_linear_workspace": _size,
     "dli_hip_conv2d_workspace": _size,
+    "dli_hip_mx_linear_workspace": _size,
     "dli_hip_paged_attention_workspace": _size,
     "dli_hip_chunk_attention_workspace": _size,
     "dli_hip_splitk_workspace": _size,

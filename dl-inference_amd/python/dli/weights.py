@@ -2,7 +2,7 @@
 python/dli_export/weights.py:18-62). One JSON manifest {format, data, tensors{name: {dtype,
 shape, offset, nbytes}}} next to one binary blob; the names follow the reference's
 <stem>.dli.weights.json / <stem>.dli.weights.bin. Besides the reference's float32 and int64,
-bfloat16, float16 and int32 tensors are written as they are (no widening to float32), and every
+bfloat16, float16, int32 and uint8 tensors are written as they are (no widening to float32), and every
 tensor starts at a 64-byte aligned offset."""
 from __future__ import annotations
 
@@ -12,7 +12,7 @@ from pathlib import Path
 import torch
 
 _DTYPES = {torch.float32: "float32", torch.int64: "int64", torch.bfloat16: "bfloat16",
-           torch.float16: "float16", torch.int32: "int32"}
+           torch.float16: "float16", torch.int32: "int32", torch.uint8: "uint8"}
 _ALIGN = 64
 
 

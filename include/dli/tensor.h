@@ -18,7 +18,7 @@
 namespace dli {
 
 enum class DeviceType { Cpu, Cuda };
-enum class DType { Float32, Int64, BFloat16, Float16, Int32 };
+enum class DType { Float32, Int64, BFloat16, Float16, Int32, UInt8 };
 
 std::string toString(DeviceType device);
 DeviceType deviceFromString(const std::string& device);

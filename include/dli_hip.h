@@ -23,8 +23,8 @@
  *  - stream: a hipStream_t passed as void*; NULL is the null stream. Every kernel entry point
  *    is asynchronous on that stream, allocates nothing and never synchronizes, so a sequence
  *    of them can be captured into a HIP graph.
- *  - dtype codes follow dli::DType: DLI_F32=0, DLI_I64=1, DLI_BF16=2, DLI_F16=3, DLI_I32=4.
- *    Floating kernels compute in fp32 and round the result to the output dtype once.
+ *  - dtype codes follow dli::DType: DLI_F32=0, DLI_I64=1, DLI_BF16=2, DLI_F16=3, DLI_I32=4,
+ *    DLI_U8=5. Floating kernels compute in fp32 and round the result to the output dtype once.
  *  - Sizes are element counts unless named *_bytes. Zero-sized work is a successful no-op.
  */
 #ifndef DLI_HIP_H_
@@ -43,6 +43,7 @@ enum {
   DLI_BF16 = 2,
   DLI_F16 = 3,
   DLI_I32 = 4,
+  DLI_U8 = 5,
 };
 
 enum {
@@ -55,6 +56,12 @@ enum {
 enum {
   DLI_ACT_NONE = 0,
   DLI_ACT_RELU = 1,
+};
+
+/* Elements of a microscaled tensor (dli_hip_mx_quantize). */
+enum {
+  DLI_MX_FP8 = 0, /* e4m3, one byte each */
+  DLI_MX_FP4 = 1, /* e2m1, two to a byte */
 };
 
 /* memcpy kinds, numbered as cudaMemcpyKind in include/dli/cuda_runtime.h:8-12. */
@@ -526,6 +533,52 @@ int dli_hip_decoder_stack(const DliDecoderLayer* layers, int num_layers, const v
  * for another workgroup (its outputs are invalid; this can only happen when the workgroups
  * were not all resident at once), else 0. Clears the flag. */
 int dli_hip_decoder_stack_status(void* workspace, int* aborted, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * 4. Microscaled (MX) tensors: linears on 4-bit weights. No counterpart in the reference, whose
+ *    tensors are fp32.
+ *
+ *    A microscaled tensor [rows, k] (k a multiple of 32) holds each row in blocks of 32 values
+ *    with one scale per block, a power of two:
+ *      scales  uint8 [rows, k / 32], 2^(code - 127); 255 makes the block NaN
+ *      codes   DLI_MX_FP8: uint8 [rows, k], e4m3; DLI_MX_FP4: uint8 [rows, k / 2], e2m1, element
+ *              2j in the low half of byte j and 2j + 1 in the high half
+ *    A block is quantised with scale code max(E - 8, 0) (e4m3) or max(E - 2, 0) (e2m1), E the
+ *    biased exponent of its largest magnitude, and elements value / scale rounded to nearest
+ *    even, at most 448 or 6 in magnitude. A block that holds a NaN or an infinity gets scale code
+ *    255 and zero elements.
+ * ------------------------------------------------------------------------------------- */
+
+/* codes, scales = x [rows, k] (fp32, bf16 or f16) quantised to `format` (DLI_MX_*). */
+int dli_hip_mx_quantize(int dtype, int format, const void* x, void* codes, void* scales,
+                        int64_t rows, int64_t k, void* stream);
+/* out [rows, k] (fp32, bf16 or f16) = what codes and scales stand for, rounded to dtype. */
+int dli_hip_mx_dequantize(int dtype, int format, const void* codes, const void* scales, void* out,
+                          int64_t rows, int64_t k, void* stream);
+/* h = x + residual rounded to dtype (residual NULL: h = x), y = h * inv * weight with
+ * inv = 1 / sqrt(mean(h^2) + eps); codes, scales = y quantised, without a rounding in between.
+ * x, residual, weight and hidden_out share dtype; hidden_out [rows, hidden] receives h (may be
+ * NULL; may be x or residual itself). mean, root and quotient are computed in 64 bits, inv rounded to
+ * 32, so that a scale does not depend on the order of a sum. */
+int dli_hip_rms_norm_mx(int dtype, int format, const void* x, const void* residual,
+                        const void* weight, void* hidden_out, void* codes, void* scales,
+                        int64_t rows, int64_t hidden, float eps, void* stream);
+/* codes, scales = gate / (1 + exp(-gate)) * up quantised. gate and up: [rows, ffn] with rows
+ * `stride` elements apart (ffn for tensors of their own; 2 * ffn, up = gate + ffn, for the two
+ * halves of one projection's rows). */
+int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up, int64_t stride,
+                        void* codes, void* scales, int64_t rows, int64_t ffn, void* stream);
+/* out[m, n] = sum_k x[m, k] * w[n, k] (+ bias[n]) (+ residual[m, n]), rounded once to out_dtype
+ * (fp32, bf16 or f16). x: microscaled [m, k] in x_format; w: microscaled [n, k] in DLI_MX_FP4.
+ * bias and residual (out_dtype) may be NULL; residual may be out itself. Scaled MFMA, fp32 sums.
+ * A workspace of dli_hip_mx_linear_workspace bytes (of any content; 0 for most shapes) lets shapes
+ * with few output tiles and a long k split k over more workgroups, summed in a fixed order; with
+ * NULL or a smaller one they do not. codes must be 16-byte aligned. */
+size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k);
+int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
+                      const void* w_codes, const void* w_scales, const void* bias,
+                      const void* residual, void* out, int64_t m, int64_t n, int64_t k,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
