@@ -35,12 +35,38 @@ MxKernels k_quantize{{DLI_MX_NAMES("mx_quantize", ""), DLI_MX_NAMES("mx_quantize
 MxKernels k_dequantize{{DLI_MX_NAMES("mx_dequantize", ""), DLI_MX_NAMES("mx_dequantize", "_any")}};
 MxKernels k_rms_norm{{DLI_MX_NAMES("rms_norm_mx", ""), DLI_MX_NAMES("rms_norm_mx", "_any")}};
 MxKernels k_silu_mul{{DLI_MX_NAMES("silu_mul_mx", ""), DLI_MX_NAMES("silu_mul_mx", "_any")}};
-DeviceKernel k_linear_tile[2][3] = {{{"mx_linear", "mx_linear_tile_fp8_f32"},
-                                     {"mx_linear", "mx_linear_tile_fp8_bf16"},
-                                     {"mx_linear", "mx_linear_tile_fp8_f16"}},
-                                    {{"mx_linear", "mx_linear_tile_fp4_f32"},
-                                     {"mx_linear", "mx_linear_tile_fp4_bf16"},
-                                     {"mx_linear", "mx_linear_tile_fp4_f16"}}};
+#define DLI_MX_LINEAR(form, odd)                                                                 \
+  {                                                                                              \
+    {{"mx_linear", form "_fp8_f32" odd}, {"mx_linear", form "_fp8_bf16" odd},                    \
+     {"mx_linear", form "_fp8_f16" odd}},                                                        \
+        {{"mx_linear", form "_fp4_f32" odd}, {"mx_linear", form "_fp4_bf16" odd},                \
+         {"mx_linear", form "_fp4_f16" odd}}                                                     \
+  }
+#define DLI_MX_STREAM(rows, odd)                                                            \
+  {                                                                                         \
+    DLI_MX_LINEAR("mx_stream_r" rows "_k1", odd), DLI_MX_LINEAR("mx_stream_r" rows "_k2", odd), \
+        DLI_MX_LINEAR("mx_stream_r" rows "_k4", odd),                                       \
+        DLI_MX_LINEAR("mx_stream_r" rows "_k8", odd)                                        \
+  }
+// [rows of scales that are not whole words][activation rows: 1, 4, 16][log2 of the waves that
+// split K][format][dtype]
+DeviceKernel k_stream[2][3][4][2][3] = {
+    {DLI_MX_STREAM("1", ""), DLI_MX_STREAM("4", ""), DLI_MX_STREAM("16", "")},
+    {DLI_MX_STREAM("1", "_odd"), DLI_MX_STREAM("4", "_odd"), DLI_MX_STREAM("16", "_odd")}};
+
+DeviceKernel k_big[2][3] = DLI_MX_LINEAR("mx_big", "");
+DeviceKernel k_scale_words("mx_linear", "mx_scale_words");
+
+// Words of 4 scales per row as the tiles read them: whole stages of 256 columns.
+int64_t scaleWords(int64_t k) { return (k + 255) / 256 * 2; }
+
+int64_t padded256(int64_t rows) { return (rows + 255) / 256 * 256; }
+
+// Whether 256 x 256 tiles take a product: from 129 rows on if there are some tiles (700 x 4608 x
+// 3584: 46 us, the stream 118; 333 x 1152 x 896: 18 and 8). Row offsets within a tile are 32-bit.
+bool bigTiles(int64_t m, int64_t n, int64_t k) {
+  return m > 128 && m * n >= int64_t{1} << 20 && k <= (int64_t{1} << 23);
+}
 
 // 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
 int checkTensor(const char* op, int dtype, int format, int64_t rows, int64_t k, const char* name) {
@@ -129,11 +155,11 @@ int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up,
 }
 
 size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k) {
-  (void)x_format;
-  (void)m;
-  (void)n;
-  (void)k;
-  return 0;
+  if (checkTensor("mx_linear", DLI_F32, x_format, m, k, "k") != 0 ||
+      checkTensor("mx_linear", DLI_F32, x_format, n, k, "k") != 0 || m == 0 || n == 0 || k == 0)
+    return 0;
+  if (!bigTiles(m, n, k)) return 0;
+  return static_cast<size_t>(scaleWords(k) * 4 * (padded256(m) + padded256(n)));
 }
 
 int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
@@ -141,8 +167,6 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
                       const void* residual, void* out, int64_t m, int64_t n, int64_t k,
                       void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "mx_linear";
-  (void)workspace;
-  (void)workspace_bytes;
   if (int rc = checkTensor(op, out_dtype, x_format, m, k, "k")) return rc;
   if (int rc = checkTensor(op, out_dtype, x_format, n, k, "k")) return rc;
   if (k == 0) return badArg(op, "k must be positive");
@@ -150,13 +174,36 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
   if (m == 0 || n == 0) return 0;
   if (m > 65535 * int64_t{16} || n > (int64_t{1} << 31) - 64)
     return badArg(op, "m must be at most 1048560, n below 2^31 - 64");
+  if (k > int64_t{1} << 28) return badArg(op, "k must be at most 2^28");
   if (x_codes == nullptr || x_scales == nullptr || w_codes == nullptr || w_scales == nullptr ||
       out == nullptr)
     return badArg(op, "NULL pointer");
   if (!aligned(x_codes, 16) || !aligned(w_codes, 16))
     return badArg(op, "codes must be 16-byte aligned");
-  return launch(k_linear_tile[x_format][dtypeIndex(out_dtype)],
-                {blocksFor(n, 64), blocksFor(m, 16)}, {256}, 0, stream, x_codes, x_scales, w_codes,
+  const size_t needed = dli_hip_mx_linear_workspace(x_format, m, n, k);
+  if (needed > 0 && workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16)) {
+    const int64_t m_pad = padded256(m), n_pad = padded256(n), words = scaleWords(k);
+    auto* xw = static_cast<uint32_t*>(workspace);
+    uint32_t* ww = xw + words * m_pad;
+    if (int rc = launch(k_scale_words, {static_cast<unsigned>((m_pad + n_pad) / 64), blocksFor(words, 16)},
+                        {256}, 0, stream, x_scales, w_scales, xw, ww, m, n,
+                        static_cast<int>(k / 32), m_pad, n_pad))
+      return rc;
+    return launch(k_big[x_format][dtypeIndex(out_dtype)],
+                  {static_cast<unsigned>(n_pad / 256), static_cast<unsigned>(m_pad / 256)}, {x_format == DLI_MX_FP8 ? 512u : 256u}, 0,
+                  stream, x_codes, xw, w_codes, ww, bias, residual, out, m, n, k, m_pad, n_pad);
+  }
+  const int odd = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4) ? 0 : 1;
+  const int form = m == 1 ? 0 : m <= 4 ? 1 : 2, rows = form == 0 ? 1 : form == 1 ? 4 : 16;
+  // the waves that share K: about 2048 waves in all, each with at least one unit of 256 columns, two
+  // where 8 share (4608 x 3584, one row: 7.8 us on 8, 5.4 on 4; 3584 x 18944: 9.4 and 10.1)
+  const int64_t tiles = (n + 15) / 16;
+  int split = 0;
+  while (split < 3 && (tiles << split) < 2048 && k >= (split < 2 ? 256 << split : 4096)) ++split;
+  const int waves = split < 3 ? 4 : 8;
+  return launch(k_stream[odd][form][split][x_format][dtypeIndex(out_dtype)],
+                {blocksFor(n, 16 * (waves >> split)), blocksFor(m, rows)},
+                {static_cast<unsigned>(64 * waves)}, 0, stream, x_codes, x_scales, w_codes,
                 w_scales, bias, residual, out, m, n, k);
 }
 
