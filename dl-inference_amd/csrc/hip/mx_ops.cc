@@ -54,7 +54,12 @@ DeviceKernel k_stream[2][3][4][2][3] = {
     {DLI_MX_STREAM("1", ""), DLI_MX_STREAM("4", ""), DLI_MX_STREAM("16", "")},
     {DLI_MX_STREAM("1", "_odd"), DLI_MX_STREAM("4", "_odd"), DLI_MX_STREAM("16", "_odd")}};
 
-DeviceKernel k_big[2][3] = DLI_MX_LINEAR("mx_big", "");
+// [tile: 256 x 256, 128 x 128, 64 x 128][format][dtype]
+DeviceKernel k_tile[3][2][3] = {DLI_MX_LINEAR("mx_tile_256", ""), DLI_MX_LINEAR("mx_tile_128", ""),
+                                DLI_MX_LINEAR("mx_tile_64", "")};
+DeviceKernel k_sum_parts[3] = {{"mx_linear", "mx_sum_parts_f32"},
+                               {"mx_linear", "mx_sum_parts_bf16"},
+                               {"mx_linear", "mx_sum_parts_f16"}};
 DeviceKernel k_scale_words("mx_linear", "mx_scale_words");
 
 // Words of 4 scales per row as the tiles read them: whole stages of 256 columns.
@@ -62,10 +67,30 @@ int64_t scaleWords(int64_t k) { return (k + 255) / 256 * 2; }
 
 int64_t padded256(int64_t rows) { return (rows + 255) / 256 * 256; }
 
-// Whether 256 x 256 tiles take a product: from 129 rows on if there are some tiles (700 x 4608 x
-// 3584: 46 us, the stream 118; 333 x 1152 x 896: 18 and 8). Row offsets within a tile are 32-bit.
-bool bigTiles(int64_t m, int64_t n, int64_t k) {
-  return m > 128 && m * n >= int64_t{1} << 20 && k <= (int64_t{1} << 23);
+// How a product runs: the tile (index of k_tile; -1: the weight stream) and the parts of K.
+struct Plan {
+  int tile, parts;
+};
+constexpr int kTileRows[3] = {256, 128, 64}, kTileColumns[3] = {256, 128, 128};
+
+int64_t tilesOf(int tile, int64_t m, int64_t n) {
+  return (m + kTileRows[tile] - 1) / kTileRows[tile] *
+         ((n + kTileColumns[tile] - 1) / kTileColumns[tile]);
+}
+
+Plan planFor(int64_t m, int64_t n, int64_t k) {
+  // Row offsets within a tile are 32-bit.
+  if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1};
+  // Large tiles once they fill most of the 256 CUs (1500 x 9728 x 896, 228 tiles: 23.5 us, in tiles of
+  // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
+  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1};
+  // Parts of K until the small tiles are about two to a CU (one of 64 rows), each part at least 2048
+  // columns (1024): 484 x 3584 x 18944 in 1, 2, 4 and 8 parts 85.6, 58.2, 53.6 and 62.4 us; 64 rows
+  // 60.0, 37.4, 26.1, 22.7 and, in 16, 26.6; 700 x 4608 x 3584 24.3 whole and 30.1 in 2.
+  const int tile = m > 64 ? 1 : 2;
+  const int64_t most = (tile == 1 ? 512 : 256) / tilesOf(tile, m, n);
+  const int64_t deep = k / (tile == 1 ? 2048 : 1024), parts = most < deep ? most : deep;
+  return {tile, static_cast<int>(parts < 1 ? 1 : parts)};
 }
 
 // 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
@@ -158,8 +183,10 @@ size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k
   if (checkTensor("mx_linear", DLI_F32, x_format, m, k, "k") != 0 ||
       checkTensor("mx_linear", DLI_F32, x_format, n, k, "k") != 0 || m == 0 || n == 0 || k == 0)
     return 0;
-  if (!bigTiles(m, n, k)) return 0;
-  return static_cast<size_t>(scaleWords(k) * 4 * (padded256(m) + padded256(n)));
+  const Plan plan = planFor(m, n, k);
+  if (plan.tile < 0) return 0;
+  return static_cast<size_t>(scaleWords(k) * 4 * (padded256(m) + padded256(n)) +
+                             (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
 }
 
 int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
@@ -182,16 +209,26 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
     return badArg(op, "codes must be 16-byte aligned");
   const size_t needed = dli_hip_mx_linear_workspace(x_format, m, n, k);
   if (needed > 0 && workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16)) {
+    const Plan plan = planFor(m, n, k);
     const int64_t m_pad = padded256(m), n_pad = padded256(n), words = scaleWords(k);
     auto* xw = static_cast<uint32_t*>(workspace);
     uint32_t* ww = xw + words * m_pad;
-    if (int rc = launch(k_scale_words, {static_cast<unsigned>((m_pad + n_pad) / 64), blocksFor(words, 16)},
-                        {256}, 0, stream, x_scales, w_scales, xw, ww, m, n,
-                        static_cast<int>(k / 32), m_pad, n_pad))
+    float* parts = plan.parts > 1 ? reinterpret_cast<float*>(ww + words * n_pad) : nullptr;
+    if (int rc = launch(k_scale_words,
+                        {static_cast<unsigned>((m_pad + n_pad) / 64), blocksFor(words, 16)}, {256},
+                        0, stream, x_scales, w_scales, xw, ww, m, n, static_cast<int>(k / 32),
+                        m_pad, n_pad))
       return rc;
-    return launch(k_big[x_format][dtypeIndex(out_dtype)],
-                  {static_cast<unsigned>(n_pad / 256), static_cast<unsigned>(m_pad / 256)}, {x_format == DLI_MX_FP8 ? 512u : 256u}, 0,
-                  stream, x_codes, xw, w_codes, ww, bias, residual, out, m, n, k, m_pad, n_pad);
+    const unsigned threads = plan.tile == 0 && x_format == DLI_MX_FP8 ? 512 : 256;
+    if (int rc = launch(k_tile[plan.tile][x_format][dtypeIndex(out_dtype)],
+                        {blocksFor(n, kTileColumns[plan.tile]), blocksFor(m, kTileRows[plan.tile]),
+                         static_cast<unsigned>(plan.parts)},
+                        {threads}, 0, stream, x_codes, xw, w_codes, ww, bias, residual, out, parts,
+                        m, n, k, m_pad, n_pad))
+      return rc;
+    if (parts == nullptr) return 0;
+    return launch(k_sum_parts[dtypeIndex(out_dtype)], {chunkBlocks((m * n + 7) / 8)}, {256}, 0,
+                  stream, parts, plan.parts, bias, residual, out, m, n);
   }
   const int odd = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4) ? 0 : 1;
   const int form = m == 1 ? 0 : m <= 4 ? 1 : 2, rows = form == 0 ? 1 : form == 1 ? 4 : 16;

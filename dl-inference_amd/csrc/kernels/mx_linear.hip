@@ -380,11 +380,11 @@ struct Big {
   static constexpr int kSBytes = kScales % (1024 * kWaves) == 0 ? 16 : 4;  // a lane's load of scales
   static constexpr int kSRows = 16 * kSBytes;                   // rows of a load of scales
   static constexpr int kXLoads = kX / (1024 * kWaves), kWLoads = kW / (1024 * kWaves);
-  static constexpr int kSLoads = kScales / (64 * kSBytes * kWaves);
+  static constexpr int kSAll = kScales / (64 * kSBytes);  // loads of scales
+  static constexpr int kSLoads = (kSAll + kWaves - 1) / kWaves;
   static constexpr int kLoads = kXLoads + kWLoads + kSLoads;  // of a wave, per stage
   static_assert(kX % (1024 * kWaves) == 0 && kW % (1024 * kWaves) == 0 &&
-                    kScales % (64 * kSBytes * kWaves) == 0 &&
-                    BM % kSRows == 0 && BN % kSRows == 0,
+                    kScales % (64 * kSBytes) == 0 && BM % kSRows == 0 && BN % kSRows == 0,
                 "whole loads");
 };
 
@@ -406,8 +406,8 @@ template <class F, class T, int BM, int BN, int WM, int WN, int KS, int ST>
 __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* xw,
                                               const uint8_t* w, const uint32_t* ww,
                                               const void* bias, const void* residual, void* out,
-                                              int64_t M, int64_t N, int64_t K, int64_t mPad,
-                                              int64_t nPad) {
+                                              float* parts, int64_t M, int64_t N, int64_t K,
+                                              int64_t mPad, int64_t nPad) {
   constexpr int kWaves = WM * WN, kM = BM / WM, kN = BN / WN;  // a wave's part of the tile
   using B = Big<F, BM, BN, KS, kWaves>;
   constexpr bool kSplit = sizeof(T) == 4;
@@ -423,13 +423,16 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   int64_t m0, n0;
   groupedTile(BM, BN, m0, n0);
   const int blocks = static_cast<int>(K / kMxBlock);
-  const int stages = static_cast<int>((K + KS - 1) / KS);
-  const int live = blocks - (stages - 1) * (KS / kMxBlock);  // blocks of the last stage
+  // the stages of this part of K (blockIdx.z of gridDim.z), and the blocks of its last one
+  const int all = static_cast<int>((K + KS - 1) / KS);
+  const int from = static_cast<int>(static_cast<int64_t>(all) * blockIdx.z / gridDim.z);
+  const int stages = static_cast<int>(static_cast<int64_t>(all) * (blockIdx.z + 1) / gridDim.z) - from;
+  const int live = from + stages == all ? blocks - (all - 1) * (KS / kMxBlock) : KS / kMxBlock;
   const uint32_t ldsAt = __builtin_amdgcn_readfirstlane(ldsAddress(smem));
   const uint32_t xStride = static_cast<uint32_t>(K * F::kWords / 2);
   const uint32_t wStride = static_cast<uint32_t>(K / 2);
-  const uint8_t* const xTile = uniform(x + m0 * (K * F::kWords / 2));
-  const uint8_t* const wTile = uniform(w + n0 * (K / 2));
+  const uint8_t* const xTile = uniform(x + m0 * (K * F::kWords / 2) + static_cast<int64_t>(from) * B::kXRow);
+  const uint8_t* const wTile = uniform(w + n0 * (K / 2) + static_cast<int64_t>(from) * B::kWRow);
   const int mLast = static_cast<int>(M - 1 - m0 < BM ? M - 1 - m0 : BM - 1);
   const int nLast = static_cast<int>(N - 1 - n0 < BN ? N - 1 - n0 : BN - 1);
 
@@ -475,9 +478,11 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
                          at + B::kX + (j * kWaves + wave) * 1024);
     } else {
       // scales: [word][x rows | w rows]
-      const int q = (i - B::kXLoads - B::kWLoads) * kWaves + wave;
+      // (with fewer loads than waves to make them, some are made twice)
+      int q = (i - B::kXLoads - B::kWLoads) * kWaves + wave;
+      if constexpr (B::kSAll % kWaves != 0) q = q < B::kSAll ? q : B::kSAll - 1;
       constexpr int kPerWord = (BM + BN) / B::kSRows;
-      const int64_t word = static_cast<int64_t>(s) * B::kWordsK + q / kPerWord;
+      const int64_t word = static_cast<int64_t>(from + s) * B::kWordsK + q / kPerWord;
       const int row = q % kPerWord * B::kSRows;
       const uint32_t* p = row < BM ? xw + word * mPad + m0 + row : ww + word * nPad + n0 + row - BM;
       loadLds<B::kSBytes, false>(uniform(reinterpret_cast<const uint8_t*>(p)), lane * B::kSBytes,
@@ -641,6 +646,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   // ---- epilogue: through LDS, so that rows of out are written whole ----
   __builtin_amdgcn_s_barrier();
   float* const slab = reinterpret_cast<float*>(smem) + wave * 32 * kPitch;
+  float* const part = parts == nullptr ? nullptr : parts + blockIdx.z * M * N;
   const bool vec = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(bias) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(residual) & 15) == 0;
@@ -656,7 +662,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
     constexpr int kRuns = kN / 8, kRows = kWave / kRuns;  // 8 columns per lane
     const int64_t n = n0 + wn * kN + (lane % kRuns) * 8;
     float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (bias != nullptr && n < N) {
+    if (bias != nullptr && part == nullptr && n < N) {
       if (vec) mxLoad8<T, true>(static_cast<const T*>(bias) + n, b);
       else
 #pragma unroll
@@ -677,7 +683,15 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
       }
       if (m >= M || n >= N) continue;
       const int64_t at = m * N + n;
-      if (vec) {
+      if (part != nullptr) {
+        if (N % 8 == 0) {
+          mxStore8<float, true>(part + at, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < N) part[at + e] = v[e];
+        }
+      } else if (vec) {
         if (residual != nullptr) {
           float s[8];
           mxLoad8<T, true>(static_cast<const T*>(residual) + at, s);
@@ -693,6 +707,49 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
             st(static_cast<T*>(out) + at + e, v[e]);
           }
       }
+    }
+  }
+}
+
+// out = the sum of `count` parts [M, N] (+ bias) (+ residual), in order.
+template <class T>
+__device__ __forceinline__ void mx_sum_parts(const float* parts, int count, const void* bias,
+                                             const void* residual, void* out, int64_t M, int64_t N) {
+  const int64_t total = M * N, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const bool vec = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(bias) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(residual) & 15) == 0;
+  T* const po = static_cast<T*>(out);
+  const T *const pb = static_cast<const T*>(bias), *const pr = static_cast<const T*>(residual);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (vec) {
+    for (int64_t i = first; i < total / 8; i += step) {
+      float v[8], a[8];
+      mxLoad8<float, true>(parts + i * 8, v);
+      for (int q = 1; q < count; ++q) {
+        mxLoad8<float, true>(parts + q * total + i * 8, a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += a[e];
+      }
+      if (bias != nullptr) {
+        mxLoad8<T, true>(pb + i * 8 % N, a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += a[e];
+      }
+      if (residual != nullptr) {
+        mxLoad8<T, true>(pr + i * 8, a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += a[e];
+      }
+      mxStore8<T, true>(po + i * 8, v);
+    }
+  } else {
+    for (int64_t i = first; i < total; i += step) {
+      float v = parts[i];
+      for (int q = 1; q < count; ++q) v += parts[q * total + i];
+      if (bias != nullptr) v += ld(pb + i % N);
+      if (residual != nullptr) v += ld(pr + i);
+      st(po + i, v);
     }
   }
 }
@@ -768,24 +825,39 @@ MX_STREAM_ROWS(1, 4)
 MX_STREAM_ROWS(4, 4)
 MX_STREAM_ROWS(16, 2)
 
-#define MX_BIG(name, F, T, BM, BN, WM, WN, KS, ST)                                               \
+#define MX_BIG(name, F, T, BM, BN, WM, WN, KS, ST, PER)                                          \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                     \
-      __attribute__((amdgpu_waves_per_eu(WM * WN / 4, WM * WN / 4)))                             \
+      __attribute__((amdgpu_waves_per_eu(PER, PER)))                                             \
       name(const uint8_t* x, const uint32_t* xw, const uint8_t* w, const uint32_t* ww,           \
-           const void* bias, const void* residual, void* out, int64_t M, int64_t N, int64_t K,   \
-           int64_t mPad, int64_t nPad) {                                                         \
-    mx_linear_big<F, T, BM, BN, WM, WN, KS, ST>(x, xw, w, ww, bias, residual, out, M, N, K,      \
-                                                mPad, nPad);                                     \
+           const void* bias, const void* residual, void* out, float* parts, int64_t M,           \
+           int64_t N, int64_t K, int64_t mPad, int64_t nPad) {                                   \
+    mx_linear_big<F, T, BM, BN, WM, WN, KS, ST>(x, xw, w, ww, bias, residual, out, parts, M, N,  \
+                                                K, mPad, nPad);                                  \
   }
-// e2m1 rows: 4 waves, stages of 256 columns (two fill LDS). e4m3 rows: 8 waves of 128 x 64, whose
-// MFMAs leave time for their fragments twice over, stages of 128 columns (8192 rows x 8192 x 8192:
-// 441 us, 488 with 4 waves; e2m1 on 8 waves ran out of registers).
-MX_BIG(mx_big_fp8_f32, MxFp8, float, 256, 256, 4, 2, 128, 3)
-MX_BIG(mx_big_fp8_bf16, MxFp8, bf16, 256, 256, 4, 2, 128, 3)
-MX_BIG(mx_big_fp8_f16, MxFp8, f16, 256, 256, 4, 2, 128, 3)
-MX_BIG(mx_big_fp4_f32, MxFp4, float, 256, 256, 2, 2, 256, 2)
-MX_BIG(mx_big_fp4_bf16, MxFp4, bf16, 256, 256, 2, 2, 256, 2)
-MX_BIG(mx_big_fp4_f16, MxFp4, f16, 256, 256, 2, 2, 256, 2)
+#define MX_BIG_FORMS(name, F, BM, BN, WM, WN, KS, ST, PER)         \
+  MX_BIG(name##_f32, F, float, BM, BN, WM, WN, KS, ST, PER)        \
+  MX_BIG(name##_bf16, F, bf16, BM, BN, WM, WN, KS, ST, PER)        \
+  MX_BIG(name##_f16, F, f16, BM, BN, WM, WN, KS, ST, PER)
+// 256 x 256. e2m1 rows: 4 waves, stages of 256 columns (two fill LDS). e4m3 rows: 8 waves of 128 x 64,
+// whose MFMAs leave time for their fragments twice over, stages of 128 columns (8192 rows x 8192 x
+// 8192: 441 us, 488 with 4 waves; e2m1 on 8 waves ran out of registers).
+MX_BIG_FORMS(mx_tile_256_fp8, MxFp8, 256, 256, 4, 2, 128, 3, 2)
+MX_BIG_FORMS(mx_tile_256_fp4, MxFp4, 256, 256, 2, 2, 256, 2, 1)
+// smaller tiles, two workgroups to a CU
+MX_BIG_FORMS(mx_tile_128_fp8, MxFp8, 128, 128, 2, 2, 128, 3, 2)
+MX_BIG_FORMS(mx_tile_128_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2)
+MX_BIG_FORMS(mx_tile_64_fp8, MxFp8, 64, 128, 2, 2, 128, 4, 2)
+MX_BIG_FORMS(mx_tile_64_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2)
+
+#define MX_SUM_PARTS(name, T)                                                                 \
+  extern "C" __global__ void __launch_bounds__(256)                                           \
+      name(const float* parts, int count, const void* bias, const void* residual, void* out,  \
+           int64_t M, int64_t N) {                                                            \
+    mx_sum_parts<T>(parts, count, bias, residual, out, M, N);                                 \
+  }
+MX_SUM_PARTS(mx_sum_parts_f32, float)
+MX_SUM_PARTS(mx_sum_parts_bf16, bf16)
+MX_SUM_PARTS(mx_sum_parts_f16, f16)
 
 extern "C" __global__ void __launch_bounds__(256)
     mx_scale_words(const uint8_t* xs, const uint8_t* ws, uint32_t* xw, uint32_t* ww, int64_t M,
