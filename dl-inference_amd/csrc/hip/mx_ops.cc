@@ -54,9 +54,10 @@ DeviceKernel k_stream[2][3][4][2][3] = {
     {DLI_MX_STREAM("1", ""), DLI_MX_STREAM("4", ""), DLI_MX_STREAM("16", "")},
     {DLI_MX_STREAM("1", "_odd"), DLI_MX_STREAM("4", "_odd"), DLI_MX_STREAM("16", "_odd")}};
 
-// [tile: 256 x 256, 128 x 128, 64 x 128][format][dtype]
-DeviceKernel k_tile[3][2][3] = {DLI_MX_LINEAR("mx_tile_256", ""), DLI_MX_LINEAR("mx_tile_128", ""),
-                                DLI_MX_LINEAR("mx_tile_64", "")};
+// [tile: 256 x 256, 128 x 128, 64 x 128, then the last two on scales as they are][format][dtype]
+DeviceKernel k_tile[5][2][3] = {DLI_MX_LINEAR("mx_tile_256", ""), DLI_MX_LINEAR("mx_tile_128", ""),
+                                DLI_MX_LINEAR("mx_tile_64", ""), DLI_MX_LINEAR("mx_tile_128r", ""),
+                                DLI_MX_LINEAR("mx_tile_64r", "")};
 DeviceKernel k_sum_parts[3] = {{"mx_linear", "mx_sum_parts_f32"},
                                {"mx_linear", "mx_sum_parts_bf16"},
                                {"mx_linear", "mx_sum_parts_f16"}};
@@ -67,9 +68,16 @@ int64_t scaleWords(int64_t k) { return (k + 255) / 256 * 2; }
 
 int64_t padded256(int64_t rows) { return (rows + 255) / 256 * 256; }
 
-// How a product runs: the tile (index of k_tile; -1: the weight stream) and the parts of K.
+// Scales laid out for the tiles (mx_scale_words).
+int64_t scaleWordBytes(int64_t m, int64_t n, int64_t k) {
+  return scaleWords(k) * 4 * (padded256(m) + padded256(n));
+}
+
+// How a product runs: the tile (0 to 2; -1: the weight stream), the parts of K, and whether the tile
+// kernel reads the scales as they are.
 struct Plan {
   int tile, parts;
+  bool rows;
 };
 constexpr int kTileRows[3] = {256, 128, 64}, kTileColumns[3] = {256, 128, 128};
 
@@ -78,19 +86,27 @@ int64_t tilesOf(int tile, int64_t m, int64_t n) {
          ((n + kTileColumns[tile] - 1) / kTileColumns[tile]);
 }
 
-Plan planFor(int64_t m, int64_t n, int64_t k) {
+// words: the scales are rows of aligned words (K % 128 == 0).
+Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // Row offsets within a tile are 32-bit.
-  if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1};
+  if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1, false};
+  // The stream takes about 3 us and one for 1000 of its units; where the tiles need their scales laid
+  // out first, it does small products sooner (333 x 1003 x 928 in fp4, a call: 8.0 us, 21.6 in tiles).
+  if (!words && (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256) < 10000) return {-1, 1, false};
   // Large tiles once they fill most of the 256 CUs (1500 x 9728 x 896, 228 tiles: 23.5 us, in tiles of
   // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
-  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1};
+  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false};
   // Parts of K until the small tiles are about two to a CU (one of 64 rows), each part at least 2048
   // columns (1024): 484 x 3584 x 18944 in 1, 2, 4 and 8 parts 85.6, 58.2, 53.6 and 62.4 us; 64 rows
   // 60.0, 37.4, 26.1, 22.7 and, in 16, 26.6; 700 x 4608 x 3584 24.3 whole and 30.1 in 2.
   const int tile = m > 64 ? 1 : 2;
   const int64_t most = (tile == 1 ? 512 : 256) / tilesOf(tile, m, n);
-  const int64_t deep = k / (tile == 1 ? 2048 : 1024), parts = most < deep ? most : deep;
-  return {tile, static_cast<int>(parts < 1 ? 1 : parts)};
+  const int64_t deep = k / (tile == 1 ? 2048 : 1024), fit = most < deep ? most : deep;
+  const int64_t parts = fit < 1 ? 1 : fit;
+  // Reading scales as they are takes a cache line for every 8 bytes, over a long K more than the launch
+  // that lays them out (64 x 9728 x 896: 6.5 us as they are, 9.7 laid out; 700 x 4608 x 3584: 21.1 and
+  // 24.7; 484 x 3584 x 18944 in 4 parts 60.2 and 52.8; 2000 x 3584 x 18944 180 and 139).
+  return {tile, static_cast<int>(parts), words && k / parts <= 4096};
 }
 
 // 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
@@ -183,9 +199,9 @@ size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k
   if (checkTensor("mx_linear", DLI_F32, x_format, m, k, "k") != 0 ||
       checkTensor("mx_linear", DLI_F32, x_format, n, k, "k") != 0 || m == 0 || n == 0 || k == 0)
     return 0;
-  const Plan plan = planFor(m, n, k);
+  const Plan plan = planFor(m, n, k, k % 128 == 0);
   if (plan.tile < 0) return 0;
-  return static_cast<size_t>(scaleWords(k) * 4 * (padded256(m) + padded256(n)) +
+  return static_cast<size_t>((plan.rows ? 0 : scaleWordBytes(m, n, k)) +
                              (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
 }
 
@@ -207,20 +223,30 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
     return badArg(op, "NULL pointer");
   if (!aligned(x_codes, 16) || !aligned(w_codes, 16))
     return badArg(op, "codes must be 16-byte aligned");
-  const size_t needed = dli_hip_mx_linear_workspace(x_format, m, n, k);
-  if (needed > 0 && workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16)) {
-    const Plan plan = planFor(m, n, k);
-    const int64_t m_pad = padded256(m), n_pad = padded256(n), words = scaleWords(k);
-    auto* xw = static_cast<uint32_t*>(workspace);
-    uint32_t* ww = xw + words * m_pad;
-    float* parts = plan.parts > 1 ? reinterpret_cast<float*>(ww + words * n_pad) : nullptr;
-    if (int rc = launch(k_scale_words,
-                        {static_cast<unsigned>((m_pad + n_pad) / 64), blocksFor(words, 16)}, {256},
-                        0, stream, x_scales, w_scales, xw, ww, m, n, static_cast<int>(k / 32),
-                        m_pad, n_pad))
-      return rc;
+  const bool words = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4);
+  Plan plan = planFor(m, n, k, words);
+  if (workspace == nullptr && plan.rows) plan.parts = 1;  // no room for parts
+  const int64_t scale_bytes = plan.rows ? 0 : scaleWordBytes(m, n, k);
+  const int64_t part_bytes = plan.parts > 1 ? plan.parts * m * n * 4 : 0;
+  const auto needed = static_cast<size_t>(scale_bytes + part_bytes);
+  if (plan.tile >= 0 &&
+      (needed == 0 ||
+       (workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16)))) {
+    const int64_t m_pad = padded256(m), n_pad = padded256(n), row_words = scaleWords(k);
+    auto* const parts = plan.parts > 1 ? static_cast<char*>(workspace) + scale_bytes : nullptr;
+    const void *xw = x_scales, *ww = w_scales;
+    if (!plan.rows) {
+      auto* const to = static_cast<uint32_t*>(workspace);
+      xw = to;
+      ww = to + row_words * m_pad;
+      if (int rc = launch(k_scale_words,
+                          {static_cast<unsigned>((m_pad + n_pad) / 64), blocksFor(row_words, 16)},
+                          {256}, 0, stream, x_scales, w_scales, xw, ww, m, n,
+                          static_cast<int>(k / 32), m_pad, n_pad))
+        return rc;
+    }
     const unsigned threads = plan.tile == 0 && x_format == DLI_MX_FP8 ? 512 : 256;
-    if (int rc = launch(k_tile[plan.tile][x_format][dtypeIndex(out_dtype)],
+    if (int rc = launch(k_tile[plan.tile + (plan.rows ? 2 : 0)][x_format][dtypeIndex(out_dtype)],
                         {blocksFor(n, kTileColumns[plan.tile]), blocksFor(m, kTileRows[plan.tile]),
                          static_cast<unsigned>(plan.parts)},
                         {threads}, 0, stream, x_codes, xw, w_codes, ww, bias, residual, out, parts,
@@ -230,7 +256,7 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
     return launch(k_sum_parts[dtypeIndex(out_dtype)], {chunkBlocks((m * n + 7) / 8)}, {256}, 0,
                   stream, parts, plan.parts, bias, residual, out, m, n);
   }
-  const int odd = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4) ? 0 : 1;
+  const int odd = words ? 0 : 1;
   const int form = m == 1 ? 0 : m <= 4 ? 1 : 2, rows = form == 0 ? 1 : form == 1 ? 4 : 16;
   // the waves that share K: about 2048 waves in all, each with at least one unit of 256 columns, two
   // where 8 share (4608 x 3584, one row: 7.8 us on 8, 5.4 on 4; 3584 x 18944: 9.4 and 10.1)

@@ -371,14 +371,14 @@ __device__ __forceinline__ f32x16 mma32(const Frag<MxFp4>& w, uint32_t sw, const
   }
 }
 
-template <class F, int BM, int BN, int KS, int kWaves>
+template <class F, int BM, int BN, int KS, int kWaves, bool kRowScales>
 struct Big {
   static constexpr int kXRow = KS * F::kWords / 2, kWRow = KS / 2;  // bytes of a row's stage
   static constexpr int kX = BM * kXRow, kW = BN * kWRow, kWordsK = KS / 128;
   static constexpr int kScales = kWordsK * (BM + BN) * 4;
   static constexpr int kStage = kX + kW + kScales;
-  static constexpr int kSBytes = kScales % (1024 * kWaves) == 0 ? 16 : 4;  // a lane's load of scales
-  static constexpr int kSRows = 16 * kSBytes;                   // rows of a load of scales
+  static constexpr int kSBytes = !kRowScales && kScales % (1024 * kWaves) == 0 ? 16 : 4;  // of a lane
+  static constexpr int kSRows = kRowScales ? 64 / kWordsK : 16 * kSBytes;  // rows of a load of scales
   static constexpr int kXLoads = kX / (1024 * kWaves), kWLoads = kW / (1024 * kWaves);
   static constexpr int kSAll = kScales / (64 * kSBytes);  // loads of scales
   static constexpr int kSLoads = (kSAll + kWaves - 1) / kWaves;
@@ -399,20 +399,20 @@ __device__ __forceinline__ uint32_t ldsRead4(uint32_t at) {
 // once then fall on different banks.
 template <int kRow>
 __device__ __forceinline__ int chunkSwizzle(int row) {
-  return kRow == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+  return kRow == 256 ? row & 15 : kRow == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-template <class F, class T, int BM, int BN, int WM, int WN, int KS, int ST>
+template <class F, class T, int BM, int BN, int WM, int WN, int KS, int ST, bool kRowScales>
 __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* xw,
                                               const uint8_t* w, const uint32_t* ww,
                                               const void* bias, const void* residual, void* out,
                                               float* parts, int64_t M, int64_t N, int64_t K,
                                               int64_t mPad, int64_t nPad) {
   constexpr int kWaves = WM * WN, kM = BM / WM, kN = BN / WN;  // a wave's part of the tile
-  using B = Big<F, BM, BN, KS, kWaves>;
+  using B = Big<F, BM, BN, KS, kWaves, kRowScales>;
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr int TM = kM / 32, TN = kN / 32, NK = KS / 64;
-  static_assert(NK % 2 == 0 && ST >= 2 && ST <= 4, "stages");
+  static_assert(NK % 2 == 0 && ST >= 2 && ST <= 4 && kN % 64 == 0, "stages, and the epilogue's runs");
   constexpr int kPitch = kN + 4;  // floats of a row of the epilogue's slab (32 rows per wave)
   constexpr int kEpilogue = kWaves * 32 * kPitch * 4;
   constexpr int kBytes = ST * B::kStage > kEpilogue ? ST * B::kStage : kEpilogue;
@@ -433,6 +433,9 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   const uint32_t wStride = static_cast<uint32_t>(K / 2);
   const uint8_t* const xTile = uniform(x + m0 * (K * F::kWords / 2) + static_cast<int64_t>(from) * B::kXRow);
   const uint8_t* const wTile = uniform(w + n0 * (K / 2) + static_cast<int64_t>(from) * B::kWRow);
+  // the rows' scales as they are, of x and w (kRowScales)
+  const uint8_t* const xsTile = uniform(reinterpret_cast<const uint8_t*>(xw) + (kRowScales ? m0 * blocks : 0));
+  const uint8_t* const wsTile = uniform(reinterpret_cast<const uint8_t*>(ww) + (kRowScales ? n0 * blocks : 0));
   const int mLast = static_cast<int>(M - 1 - m0 < BM ? M - 1 - m0 : BM - 1);
   const int nLast = static_cast<int>(N - 1 - n0 < BN ? N - 1 - n0 : BN - 1);
 
@@ -477,16 +480,28 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
       loadLds<16, false>(wTile + static_cast<int64_t>(s) * B::kWRow, wOff[j],
                          at + B::kX + (j * kWaves + wave) * 1024);
     } else {
-      // scales: [word][x rows | w rows]
       // (with fewer loads than waves to make them, some are made twice)
       int q = (i - B::kXLoads - B::kWLoads) * kWaves + wave;
       if constexpr (B::kSAll % kWaves != 0) q = q < B::kSAll ? q : B::kSAll - 1;
-      constexpr int kPerWord = (BM + BN) / B::kSRows;
-      const int64_t word = static_cast<int64_t>(from + s) * B::kWordsK + q / kPerWord;
-      const int row = q % kPerWord * B::kSRows;
-      const uint32_t* p = row < BM ? xw + word * mPad + m0 + row : ww + word * nPad + n0 + row - BM;
-      loadLds<B::kSBytes, false>(uniform(reinterpret_cast<const uint8_t*>(p)), lane * B::kSBytes,
-                                 at + B::kX + B::kW + q * B::kSRows * 4);
+      const uint32_t to = at + B::kX + B::kW + q * 256 * (B::kSBytes / 4);
+      if constexpr (kRowScales) {
+        // [x rows | w rows][word] from the scales as they are: rows of whole words (K % 128 == 0),
+        // words past the last one stand for it
+        const int row = q * B::kSRows + lane / B::kWordsK, here = row < BM ? row : row - BM;
+        const int most = row < BM ? mLast : nLast;
+        int word = (from + s) * B::kWordsK + lane % B::kWordsK;
+        word = word < blocks / 4 ? word : blocks / 4 - 1;
+        const bool isX = q * B::kSRows < BM;
+        loadLds<4, false>(isX ? xsTile : wsTile,
+                          static_cast<uint32_t>(here < most ? here : most) * blocks + word * 4, to);
+      } else {
+        // [word][x rows | w rows]
+        constexpr int kPerWord = (BM + BN) / B::kSRows;
+        const int64_t word = static_cast<int64_t>(from + s) * B::kWordsK + q / kPerWord;
+        const int row = q % kPerWord * B::kSRows;
+        const uint32_t* p = row < BM ? xw + word * mPad + m0 + row : ww + word * nPad + n0 + row - BM;
+        loadLds<B::kSBytes, false>(uniform(reinterpret_cast<const uint8_t*>(p)), lane * B::kSBytes, to);
+      }
     }
   };
 
@@ -504,7 +519,9 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   const int xr = wm * kM + r, wr = wn * kN + r;
   const uint32_t xBase = ldsAt + xr * B::kXRow + ((g ^ chunkSwizzle<B::kXRow>(xr)) * 16);
   const uint32_t wBase = ldsAt + B::kX + wr * B::kWRow + ((g ^ chunkSwizzle<B::kWRow>(wr)) * 16);
-  const uint32_t sBase = ldsAt + B::kX + B::kW + xr * 4;
+  constexpr int kSRow = kRowScales ? 4 * B::kWordsK : 4;         // bytes from row to row
+  constexpr int kSWord = kRowScales ? 4 : (BM + BN) * 4;  // and from word to word
+  const uint32_t sBase = ldsAt + B::kX + B::kW + xr * kSRow;
   struct At {
     uint32_t x, w, s;
   };
@@ -525,11 +542,11 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
       f.x[q].q[h] = ldsRead16((at.x ^ (kStep * 32 * F::kWords + h * 32)) + q * 32 * B::kXRow);
     }
   };
-  const int wFromX = (BM + wr - xr) * 4;
+  const int wFromX = (BM + wr - xr) * kSRow;
   auto readScale = [&](const At& at, int word, int i, Scales& s) {
-    const uint32_t p = at.s + word * (BM + BN) * 4;
-    if (i < TN) s.w[i] = ldsRead4(p + wFromX + i * 128);
-    else s.x[i - TN] = ldsRead4(p + (i - TN) * 128);
+    const uint32_t p = at.s + word * kSWord;
+    if (i < TN) s.w[i] = ldsRead4(p + wFromX + i * 32 * kSRow);
+    else s.x[i - TN] = ldsRead4(p + (i - TN) * 32 * kSRow);
   };
   auto shiftScales = [&](Scales& s) {  // the lane's blocks to bytes 0 and 2
 #pragma unroll
@@ -659,39 +676,31 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
         *reinterpret_cast<f32x4*>(&slab[r * kPitch + i * 32 + v * 8 + g * 4]) =
             f32x4{acc[i][q][4 * v], acc[i][q][4 * v + 1], acc[i][q][4 * v + 2],
                   acc[i][q][4 * v + 3]};
-    constexpr int kRuns = kN / 8, kRows = kWave / kRuns;  // 8 columns per lane
-    const int64_t n = n0 + wn * kN + (lane % kRuns) * 8;
-    float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (bias != nullptr && part == nullptr && n < N) {
-      if (vec) mxLoad8<T, true>(static_cast<const T*>(bias) + n, b);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < N) b[e] = ld(static_cast<const T*>(bias) + n + e);
-    }
+    const int64_t mq = m0 + wm * kM + q * 32;
+    if (vec) {
+      constexpr int kRuns = kN / 8, kRows = kWave / kRuns;  // 8 columns per lane
+      const int c = (lane % kRuns) * 8;
+      const int64_t n = n0 + wn * kN + c;
+      float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (bias != nullptr && part == nullptr && n < N)
+        mxLoad8<T, true>(static_cast<const T*>(bias) + n, b);
 #pragma unroll 4
-    for (int p = 0; p < 32; p += kRows) {
-      const int row = p + lane / kRuns;
-      const int64_t m = m0 + wm * kM + q * 32 + row;
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(&slab[row * kPitch + (lane % kRuns) * 8]);
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(&slab[row * kPitch + (lane % kRuns) * 8 + 4]);
-      float v[8];
+      for (int p = 0; p < 32; p += kRows) {
+        const int row = p + lane / kRuns;
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(&slab[row * kPitch + c]);
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(&slab[row * kPitch + c + 4]);
+        float v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = lo[e] + b[e];
-        v[4 + e] = hi[e] + b[4 + e];
-      }
-      if (m >= M || n >= N) continue;
-      const int64_t at = m * N + n;
-      if (part != nullptr) {
-        if (N % 8 == 0) {
-          mxStore8<float, true>(part + at, v);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < N) part[at + e] = v[e];
+        for (int e = 0; e < 4; ++e) {
+          v[e] = lo[e] + b[e];
+          v[4 + e] = hi[e] + b[4 + e];
         }
-      } else if (vec) {
+        if (mq + row >= M || n >= N) continue;
+        const int64_t at = (mq + row) * N + n;
+        if (part != nullptr) {
+          mxStore8<float, true>(part + at, v);
+          continue;
+        }
         if (residual != nullptr) {
           float s[8];
           mxLoad8<T, true>(static_cast<const T*>(residual) + at, s);
@@ -699,13 +708,32 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
           for (int e = 0; e < 8; ++e) v[e] += s[e];
         }
         mxStore8<T, true>(static_cast<T*>(out) + at, v);
-      } else {
+      }
+    } else {
+      // a lane takes one column of a run of 64, 8 rows at a time: their loads are in flight together
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (n + e < N) {
-            if (residual != nullptr) v[e] += ld(static_cast<const T*>(residual) + at + e);
-            st(static_cast<T*>(out) + at + e, v[e]);
+      for (int run = 0; run < kN / 64; ++run) {
+        const int c = run * 64 + lane;
+        const int64_t n = n0 + wn * kN + c;
+        if (n >= N) continue;
+        const float b = bias != nullptr && part == nullptr ? ld(static_cast<const T*>(bias) + n) : 0.f;
+        const T* const pr = part == nullptr ? static_cast<const T*>(residual) : nullptr;
+        for (int p = 0; p < 32; p += 8) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int64_t m = mq + p + e < M ? mq + p + e : M - 1;
+            v[e] = pr != nullptr ? ld(pr + m * N + n) : 0.f;
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int64_t m = mq + p + e;
+            if (m >= M) break;
+            const float sum = slab[(p + e) * kPitch + c] + b + v[e];
+            if (part != nullptr) part[m * N + n] = sum;
+            else st(static_cast<T*>(out) + m * N + n, sum);
+          }
+        }
       }
     }
   }
@@ -825,29 +853,33 @@ MX_STREAM_ROWS(1, 4)
 MX_STREAM_ROWS(4, 4)
 MX_STREAM_ROWS(16, 2)
 
-#define MX_BIG(name, F, T, BM, BN, WM, WN, KS, ST, PER)                                          \
+#define MX_BIG(name, F, T, BM, BN, WM, WN, KS, ST, PER, RS)                                          \
   extern "C" __global__ void __launch_bounds__(64 * WM * WN)                                     \
       __attribute__((amdgpu_waves_per_eu(PER, PER)))                                             \
       name(const uint8_t* x, const uint32_t* xw, const uint8_t* w, const uint32_t* ww,           \
            const void* bias, const void* residual, void* out, float* parts, int64_t M,           \
            int64_t N, int64_t K, int64_t mPad, int64_t nPad) {                                   \
-    mx_linear_big<F, T, BM, BN, WM, WN, KS, ST>(x, xw, w, ww, bias, residual, out, parts, M, N,  \
-                                                K, mPad, nPad);                                  \
+    mx_linear_big<F, T, BM, BN, WM, WN, KS, ST, RS>(x, xw, w, ww, bias, residual, out, parts, M, \
+                                                    N, K, mPad, nPad);                           \
   }
-#define MX_BIG_FORMS(name, F, BM, BN, WM, WN, KS, ST, PER)         \
-  MX_BIG(name##_f32, F, float, BM, BN, WM, WN, KS, ST, PER)        \
-  MX_BIG(name##_bf16, F, bf16, BM, BN, WM, WN, KS, ST, PER)        \
-  MX_BIG(name##_f16, F, f16, BM, BN, WM, WN, KS, ST, PER)
+#define MX_BIG_FORMS(name, F, BM, BN, WM, WN, KS, ST, PER, RS)         \
+  MX_BIG(name##_f32, F, float, BM, BN, WM, WN, KS, ST, PER, RS)        \
+  MX_BIG(name##_bf16, F, bf16, BM, BN, WM, WN, KS, ST, PER, RS)        \
+  MX_BIG(name##_f16, F, f16, BM, BN, WM, WN, KS, ST, PER, RS)
 // 256 x 256. e2m1 rows: 4 waves, stages of 256 columns (two fill LDS). e4m3 rows: 8 waves of 128 x 64,
 // whose MFMAs leave time for their fragments twice over, stages of 128 columns (8192 rows x 8192 x
 // 8192: 441 us, 488 with 4 waves; e2m1 on 8 waves ran out of registers).
-MX_BIG_FORMS(mx_tile_256_fp8, MxFp8, 256, 256, 4, 2, 128, 3, 2)
-MX_BIG_FORMS(mx_tile_256_fp4, MxFp4, 256, 256, 2, 2, 256, 2, 1)
+MX_BIG_FORMS(mx_tile_256_fp8, MxFp8, 256, 256, 4, 2, 128, 3, 2, false)
+MX_BIG_FORMS(mx_tile_256_fp4, MxFp4, 256, 256, 2, 2, 256, 2, 1, false)
 // smaller tiles, two workgroups to a CU
-MX_BIG_FORMS(mx_tile_128_fp8, MxFp8, 128, 128, 2, 2, 128, 3, 2)
-MX_BIG_FORMS(mx_tile_128_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2)
-MX_BIG_FORMS(mx_tile_64_fp8, MxFp8, 64, 128, 2, 2, 128, 4, 2)
-MX_BIG_FORMS(mx_tile_64_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2)
+MX_BIG_FORMS(mx_tile_128_fp8, MxFp8, 128, 128, 2, 2, 128, 3, 2, false)
+MX_BIG_FORMS(mx_tile_128_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2, false)
+MX_BIG_FORMS(mx_tile_64_fp8, MxFp8, 64, 128, 2, 2, 256, 2, 2, false)
+MX_BIG_FORMS(mx_tile_64_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2, false)
+MX_BIG_FORMS(mx_tile_128r_fp8, MxFp8, 128, 128, 2, 2, 128, 3, 2, true)
+MX_BIG_FORMS(mx_tile_128r_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2, true)
+MX_BIG_FORMS(mx_tile_64r_fp8, MxFp8, 64, 128, 2, 2, 256, 2, 2, true)
+MX_BIG_FORMS(mx_tile_64r_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2, true)
 
 #define MX_SUM_PARTS(name, T)                                                                 \
   extern "C" __global__ void __launch_bounds__(256)                                           \
