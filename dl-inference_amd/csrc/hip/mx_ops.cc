@@ -173,8 +173,12 @@ int dli_hip_rms_norm_mx(int dtype, int format, const void* x, const void* residu
                       ? 0
                       : 1;
   const unsigned blocks = static_cast<unsigned>(rows < 65535 ? rows : 65535);
-  return launch(k_rms_norm.k[any][format][dtypeIndex(dtype)], {blocks}, {256}, 0, stream, x,
-                residual, weight, hidden_out, codes, scales, rows, hidden, eps);
+  // A chunk of 8 values per thread, up to 4 waves. 8192 rows of 896: 21.6 us with 4 waves, 17.1 with
+  // 2 or 1; 333 of 4864: 16.8 with 1, 10.7 with 2, 7.2 with 4.
+  const unsigned threads = hidden <= 512 ? 64 : hidden <= 1024 ? 128 : 256;
+  return launch(k_rms_norm.k[any][format][dtypeIndex(dtype)], {blocks}, {threads}, 0, stream, x,
+                residual, weight, hidden_out, codes, scales, rows, hidden,
+                1.0 / static_cast<double>(hidden), eps);
 }
 
 int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up, int64_t stride,

@@ -122,35 +122,70 @@ __device__ __forceinline__ uint32_t mxQuantize8(const float (&y)[8], uint32_t (&
   return code;
 }
 
+// 8 values of T as they lie in memory, for values that stay in registers: half the registers of
+// floats where T has 16 bits.
+template <class T>
+struct MxRaw8 {
+  uint32_t w[2 * sizeof(T)];
+};
+
+template <class T>
+__device__ __forceinline__ void mxUnpack8(const MxRaw8<T>& raw, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(raw.w[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (__is_same(T, bf16)) {
+        v[2 * i] = __uint_as_float(raw.w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(raw.w[i] & 0xFFFF0000u);
+      } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 h = __builtin_bit_cast(h2, raw.w[i]);
+        v[2 * i] = static_cast<float>(h[0]);
+        v[2 * i + 1] = static_cast<float>(h[1]);
+      }
+    }
+  }
+}
+
+template <class T>
+__device__ __forceinline__ MxRaw8<T> mxPack8(const float (&v)[8]) {
+  MxRaw8<T> raw;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw.w[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (__is_same(T, bf16)) {
+        raw.w[i] = packBf16x2(v[2 * i], v[2 * i + 1]);
+      } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 h = {static_cast<_Float16>(v[2 * i]), static_cast<_Float16>(v[2 * i + 1])};
+        raw.w[i] = __builtin_bit_cast(uint32_t, h);
+      }
+    }
+  }
+  return raw;
+}
+
 // 8 consecutive values as floats. kVec: p is 16-byte aligned.
 template <class T, bool kVec>
 __device__ __forceinline__ void mxLoad8(const T* p, float (&v)[8]) {
   if constexpr (!kVec) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = ld(p + i);
-  } else if constexpr (sizeof(T) == 4) {
-    const U32x4 a = gp(reinterpret_cast<const U32x4*>(p))[0];
-    const U32x4 b = gp(reinterpret_cast<const U32x4*>(p))[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = __uint_as_float(a[i]);
-      v[4 + i] = __uint_as_float(b[i]);
-    }
   } else {
-    const U32x4 a = *gp(reinterpret_cast<const U32x4*>(p));
+    MxRaw8<T> raw;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (__is_same(T, bf16)) {
-        v[2 * i] = __uint_as_float(a[i] << 16);
-        v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
-      } else {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const uint32_t bits = a[i];  // (a bit cast of the vector element itself reads element 0)
-        const h2 h = __builtin_bit_cast(h2, bits);
-        v[2 * i] = static_cast<float>(h[0]);
-        v[2 * i + 1] = static_cast<float>(h[1]);
-      }
+    for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j) {
+      const U32x4 a = gp(reinterpret_cast<const U32x4*>(p))[j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw.w[4 * j + i] = a[i];
     }
+    mxUnpack8<T>(raw, v);
   }
 }
 
@@ -159,28 +194,15 @@ __device__ __forceinline__ void mxStore8(T* p, const float (&v)[8]) {
   if constexpr (!kVec) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) st(p + i, v[i]);
-  } else if constexpr (sizeof(T) == 4) {
-    U32x4 a, b;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = __float_as_uint(v[i]);
-      b[i] = __float_as_uint(v[4 + i]);
-    }
-    gp(reinterpret_cast<U32x4*>(p))[0] = a;
-    gp(reinterpret_cast<U32x4*>(p))[1] = b;
   } else {
-    U32x4 a;
+    const MxRaw8<T> raw = mxPack8<T>(v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (__is_same(T, bf16)) {
-        a[i] = packBf16x2(v[2 * i], v[2 * i + 1]);
-      } else {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const h2 h = {static_cast<_Float16>(v[2 * i]), static_cast<_Float16>(v[2 * i + 1])};
-        a[i] = __builtin_bit_cast(uint32_t, h);
-      }
+    for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j) {
+      U32x4 a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = raw.w[4 * j + i];
+      gp(reinterpret_cast<U32x4*>(p))[j] = a;
     }
-    *gp(reinterpret_cast<U32x4*>(p)) = a;
   }
 }
 
