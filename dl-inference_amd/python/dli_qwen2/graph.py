@@ -17,6 +17,10 @@ the embedding table itself), bit-identical to the fused graph. It
 has a third output, `status` (int32 [1], the launch status the decoder_stack node accumulates:
 non-zero when a wait in the persistent launch gave up and the step's outputs are invalid), which
 the decode drivers check where they synchronize anyway.
+
+microscaled graph (mx="fp8" or "fp4"): the layers' linears on 4-bit weights (mx_linear), their
+inputs quantised to `mx` by the nodes before them (rms_norm_mx, mx_quantize, silu_mul_mx).
+pack_mx_weights makes its weights. Both plugins run it; prompts have a form of it too.
 """
 from __future__ import annotations
 
@@ -175,6 +179,95 @@ def _large_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, fused:
     _node(nodes, "greedy", "argmax", ["logits"], ["next_ids"])
 
 
+def _mx_linear(nodes: list, name: str, x: str, out: str, bias: bool = False,
+               residual: str | None = None, dtype: str = "bfloat16"):
+    inputs = [f"{x}.codes", f"{x}.scales", f"{name}.weight.codes", f"{name}.weight.scales"]
+    attrs = {"out_dtype": dtype}
+    if bias:
+        inputs.append(f"{name}.bias")
+    if residual is not None:
+        inputs.append(residual)
+        attrs["residual"] = True
+    _node(nodes, name, "mx_linear", inputs, [out], attrs)
+
+
+def _mx_layer_nodes(cfg: Qwen2Config, batch: int, seq: int | None, i: int, h: str, nodes: list,
+                    mx: str, dtype: str, bshd: bool) -> str:
+    """One decoder layer on microscaled linears. seq None: a decode step (positions input);
+    else a prompt of seq tokens. bshd: attention writes [B, S, H, D] itself (GPU plugin).
+    Returns the layer's output name."""
+    p, t = f"model.layers.{i}", f"layers_{i}"
+    lead = [batch] if seq is None else [batch, seq]
+
+    def coded(x):
+        return [f"{x}.codes", f"{x}.scales"]
+
+    _node(nodes, f"{p}.input_layernorm", "rms_norm_mx", [h, f"{p}.input_layernorm.weight"],
+          coded(f"{t}_input_norm"), {"eps": cfg.eps, "format": mx})
+    for proj, heads in (("q", cfg.heads), ("k", cfg.kv_heads), ("v", cfg.kv_heads)):
+        _mx_linear(nodes, f"{p}.self_attn.{proj}_proj", f"{t}_input_norm", f"{t}_{proj}",
+                   bias=True, dtype=dtype)
+        shape = [batch, heads, 1, cfg.head_dim] if seq is None else [batch, seq, heads, cfg.head_dim]
+        out = f"{t}_{proj}_heads" if seq is None else f"{t}_{proj}_bshd"
+        _node(nodes, f"{p}.self_attn.{proj}_reshape", "reshape", [f"{t}_{proj}"], [out],
+              {"shape": shape})
+        if seq is not None:
+            _node(nodes, f"{p}.self_attn.{proj}_transpose", "transpose", [out],
+                  [f"{t}_{proj}_heads"], {"perm": [0, 2, 1, 3]})
+    rotary = [f"{t}_q_heads", f"{t}_k_heads", "rotary_cos", "rotary_sin"]
+    attention = [f"{t}_q_rotary", f"{t}_k_rotary", f"{t}_v_heads"]
+    cache = {"causal": True, "kv_cache": f"layer_{i}"}
+    if seq is None:
+        _node(nodes, f"{p}.self_attn.rotary_embedding", "rotary_embedding",
+              rotary + ["positions"], attention[:2])
+        _node(nodes, f"{p}.self_attn.attention", "attention", attention + ["positions"],
+              [f"{t}_attention"], cache)
+    else:
+        _node(nodes, f"{p}.self_attn.rotary_embedding", "rotary_embedding", rotary,
+              attention[:2], {"start_pos": 0})
+        if bshd:
+            _node(nodes, f"{p}.self_attn.attention", "attention", attention, [f"{t}_attention"],
+                  {**cache, "output_layout": "bshd"})
+        else:
+            _node(nodes, f"{p}.self_attn.attention", "attention", attention,
+                  [f"{t}_attention_bhsd"], cache)
+            _node(nodes, f"{p}.self_attn.attention_transpose", "transpose",
+                  [f"{t}_attention_bhsd"], [f"{t}_attention"], {"perm": [0, 2, 1, 3]})
+    _node(nodes, f"{p}.self_attn.merge", "reshape", [f"{t}_attention"],
+          [f"{t}_attention_merged"], {"shape": lead + [cfg.heads * cfg.head_dim]})
+    _node(nodes, f"{p}.self_attn.attention_codes", "mx_quantize", [f"{t}_attention_merged"],
+          coded(f"{t}_attention_merged"), {"format": mx})
+    _mx_linear(nodes, f"{p}.self_attn.o_proj", f"{t}_attention_merged", f"{t}_after_attention",
+               residual=h, dtype=dtype)
+    _node(nodes, f"{p}.post_attention_layernorm", "rms_norm_mx",
+          [f"{t}_after_attention", f"{p}.post_attention_layernorm.weight"],
+          coded(f"{t}_post_attention_norm"), {"eps": cfg.eps, "format": mx})
+    _mx_linear(nodes, f"{p}.mlp.gate_up_proj", f"{t}_post_attention_norm", f"{t}_gate_up",
+               dtype=dtype)
+    _node(nodes, f"{p}.mlp.act_fn", "silu_mul_mx", [f"{t}_gate_up"], coded(f"{t}_gated"),
+          {"format": mx})
+    _mx_linear(nodes, f"{p}.mlp.down_proj", f"{t}_gated", f"{t}_output",
+               residual=f"{t}_after_attention", dtype=dtype)
+    return f"{t}_output"
+
+
+def _check_mx(cfg: Qwen2Config, mx: str):
+    if mx not in ("fp8", "fp4"):
+        raise ValueError(f"mx must be fp8 or fp4, not {mx!r}")
+    for what, k in (("hidden", cfg.hidden), ("heads * head_dim", cfg.heads * cfg.head_dim),
+                    ("ffn", cfg.ffn)):
+        if k % 32:
+            raise ValueError(f"microscaled linears need {what} ({k}) to be a multiple of 32")
+
+
+def _plain_head_nodes(cfg: Qwen2Config, nodes: list, h: str):
+    _node(nodes, "model.norm", "rms_norm", [h, "model.norm.weight"], ["norm_hidden"],
+          {"eps": cfg.eps})
+    _node(nodes, "lm_head", "linear", ["norm_hidden", "lm_head.weight"], ["logits"],
+          {"out_dtype": "float32"})
+    _node(nodes, "greedy", "argmax", ["logits"], ["next_ids"])
+
+
 def _fused_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, logits_dtype: str):
     h = "hidden_states"
     for i in range(cfg.layers):
@@ -263,8 +356,11 @@ def uses_large_graph(cfg: Qwen2Config, fused: bool) -> bool:
 def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
                        splits: dict | None = None, logits_dtype: str = "float32",
                        stack: bool = False, check_status: bool = False,
-                       large_fused: bool = False, stack_trace: bool = False) -> "dli.Graph":
-    """fused=False: the reference's node sequence; fused=True: five launches per layer;
+                       large_fused: bool = False, stack_trace: bool = False,
+                       mx: str | None = None, dtype: str = "bfloat16") -> "dli.Graph":
+    """mx: the layers on microscaled linears with activations in that format ("fp8", "fp4") and
+    hidden states in `dtype` (_mx_layer_nodes), whatever the forms below; fused then only says
+    that the head may be one lm_head_argmax node. Else fused=False: the reference's node sequence; fused=True: five launches per layer;
     stack=True (with fused): all layers in one decoder_stack node (check_status: the node waits
     for its launch and fails if a workgroup gave up waiting; for tests, not for capture). With
     fused=True and a hidden size above 1024 (the Qwen2-7B shape) the step is the large-hidden
@@ -273,9 +369,21 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
     choice}; stack_trace: the decoder_stack node records its stage timeline into graph input
     "stack_trace" (int64, layers x CUs x 24)."""
     nodes: list = []
-    if not (fused and stack) or uses_large_graph(cfg, fused):  # the stack gathers it itself
+    if mx is not None or not (fused and stack) or uses_large_graph(cfg, fused):  # the stack gathers it itself
         _node(nodes, "model.embed_tokens", "embedding", ["input_ids", "model.embed_tokens.weight"],
               ["hidden_states"])
+    if mx is not None:
+        _check_mx(cfg, mx)
+        h = "hidden_states"
+        for i in range(cfg.layers):
+            h = _mx_layer_nodes(cfg, batch, None, i, h, nodes, mx, dtype, False)
+        if fused and not uses_large_graph(cfg, fused):
+            _head_nodes(cfg, nodes, h, logits_dtype)
+        else:
+            _plain_head_nodes(cfg, nodes, h)
+        graph = {"format": "dli.graph.v1", "model_type": "qwen2_decode_mx",
+                 "inputs": INPUTS, "outputs": OUTPUTS, "nodes": nodes}
+        return dli.Graph.from_json(json.dumps(graph))
     if uses_large_graph(cfg, fused):
         _large_nodes(cfg, batch, nodes, splits or large_splits(batch), large_fused)
         graph = {"format": "dli.graph.v1", "model_type": "qwen2_decode_large",
@@ -377,7 +485,8 @@ def _prefill_layer_nodes(cfg: Qwen2Config, batch: int, seq: int, i: int, h: str,
 
 def build_prefill_graph(cfg: Qwen2Config, batch: int, seq: int, layers: int | None = None,
                         from_hidden: bool = False, fused_head: bool = True,
-                        fused: bool = False) -> "dli.Graph":
+                        fused: bool = False, mx: str | None = None,
+                        dtype: str = "bfloat16") -> "dli.Graph":
     """Prefill of a `seq`-token prompt per sequence (every sequence starts at position 0 of an
     empty KV cache; the cache entries layer_0.. are filled with the prompt's keys and values, so
     decode-step graphs continue at position `seq`).
@@ -388,7 +497,11 @@ def build_prefill_graph(cfg: Qwen2Config, batch: int, seq: int, layers: int | No
     outputs logits [B, V] and next_ids [B] (the first generated token).
     from_hidden=True: hidden_states [B, S, H] -> the decoder layers (the first `layers`) ->
     output hidden [B, S, H] (one decoder layer of prefill, the config-3 workload).
-    fused: the layers' fused form (_prefill_layer_nodes), which reads mlp.gate_up_proj.weight."""
+    fused: the layers' fused form (_prefill_layer_nodes), which reads mlp.gate_up_proj.weight.
+    mx: the layers on microscaled linears (_mx_layer_nodes; fused then only chooses attention's
+    output layout)."""
+    if mx is not None:
+        _check_mx(cfg, mx)
     n_layers = cfg.layers if layers is None else layers
     nodes: list = []
     h = "hidden_states"
@@ -396,7 +509,8 @@ def build_prefill_graph(cfg: Qwen2Config, batch: int, seq: int, layers: int | No
         _node(nodes, "model.embed_tokens", "embedding",
               ["input_ids", "model.embed_tokens.weight"], [h])
     for i in range(n_layers):
-        h = _prefill_layer_nodes(cfg, batch, seq, i, h, nodes, fused)
+        h = (_prefill_layer_nodes(cfg, batch, seq, i, h, nodes, fused) if mx is None else
+             _mx_layer_nodes(cfg, batch, seq, i, h, nodes, mx, dtype, fused))
     if from_hidden:
         _node(nodes, "output", "reshape", [h], ["output"], {"shape": [batch, seq, cfg.hidden]})
         graph = {"format": "dli.graph.v1", "model_type": "qwen2_prefill_layers",
@@ -408,11 +522,7 @@ def build_prefill_graph(cfg: Qwen2Config, batch: int, seq: int, layers: int | No
     if fused_head:
         _head_nodes(cfg, nodes, "last_hidden", "float32")
     else:
-        _node(nodes, "model.norm", "rms_norm", ["last_hidden", "model.norm.weight"],
-              ["norm_hidden"], {"eps": cfg.eps})
-        _node(nodes, "lm_head", "linear", ["norm_hidden", "lm_head.weight"], ["logits"],
-              {"out_dtype": "float32"})
-        _node(nodes, "greedy", "argmax", ["logits"], ["next_ids"])
+        _plain_head_nodes(cfg, nodes, "last_hidden")
     graph = {"format": "dli.graph.v1", "model_type": "qwen2_prefill",
              "inputs": ["input_ids"], "outputs": OUTPUTS, "nodes": nodes}
     return dli.Graph.from_json(json.dumps(graph))
@@ -461,4 +571,30 @@ def pack_fused_weights(cfg: Qwen2Config, weights: dict, drop_unfused: bool = Fal
                 out.pop(f"{a}.{x}_proj.bias")
             out.pop(f"{p}.mlp.gate_proj.weight")
             out.pop(f"{p}.mlp.up_proj.weight")
+    return out
+
+
+def pack_mx_weights(cfg: Qwen2Config, weights: dict, engine: "dli.Engine") -> dict:
+    """The microscaled graphs' tensors: every layer's linear weight as 4-bit codes and scales
+    ({name}.codes, {name}.scales), quantised by `engine` where the weight lies, gate_proj above
+    up_proj in mlp.gate_up_proj. Embedding, norms, biases and lm_head keep their type."""
+    _check_mx(cfg, "fp4")
+    quantize = dli.Graph.from_json(json.dumps(
+        {"format": "dli.graph.v1", "model_type": "mx_quantize", "inputs": ["x"],
+         "outputs": ["codes", "scales"],
+         "nodes": [{"name": "quantize", "op": "mx_quantize", "inputs": ["x"],
+                    "outputs": ["codes", "scales"], "attrs": {"format": "fp4"}}]}))
+    out = dict(weights)
+
+    def pack(name, weight):
+        coded = engine.run(quantize, {"x": weight.contiguous()})
+        out[f"{name}.codes"], out[f"{name}.scales"] = coded["codes"], coded["scales"]
+
+    for i in range(cfg.layers):
+        p = f"model.layers.{i}"
+        for name in ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj",
+                     "self_attn.o_proj", "mlp.down_proj"):
+            pack(f"{p}.{name}.weight", out.pop(f"{p}.{name}.weight"))
+        pack(f"{p}.mlp.gate_up_proj.weight", torch.cat(
+            [out.pop(f"{p}.mlp.gate_proj.weight"), out.pop(f"{p}.mlp.up_proj.weight")]))
     return out

@@ -13,7 +13,7 @@ import dli
 
 from .config import Qwen2Config
 from .graph import (build_decode_graph, build_prefill_graph, pack_fused_weights,
-                    pack_large_weights, uses_large_graph)
+                    pack_large_weights, pack_mx_weights, uses_large_graph)
 
 
 class DecodeSession:
@@ -21,11 +21,18 @@ class DecodeSession:
                  fused: bool = True, engine: "dli.Engine | None" = None, splits: dict | None = None,
                  block_size: int = 64, logits_dtype: str = "float32", device: str = "cuda",
                  stack: bool = False, check_status: bool = False, prefill: bool = False,
-                 stack_trace: "torch.Tensor | None" = None):
+                 stack_trace: "torch.Tensor | None" = None, mx: str | None = None):
+        """mx ("fp8" or "fp4"): the layers' linears run on 4-bit weights, quantised here, with
+        activations in that format; decode steps and prompts alike. It has no stack form."""
+        if mx is not None and stack:
+            raise ValueError("the microscaled graph has no decoder stack form")
         self.cfg = cfg
         self.batch = batch
         self.fused = fused
         self.stack = fused and stack and not uses_large_graph(cfg, fused)
+        # mx: hidden states stay in the weights' type
+        self._mx = {} if mx is None else {
+            "mx": mx, "dtype": str(weights["model.norm.weight"].dtype).removeprefix("torch.")}
         self.engine = engine or dli.Engine().load_plugin()
         self.engine.configure_kv_cache(block_size=block_size, max_seq_len=max_seq_len)
         # the large-hidden graph's GPU form (fused q|k|v, residual + RMSNorm and MLP nodes of
@@ -38,12 +45,14 @@ class DecodeSession:
         self.graph = build_decode_graph(cfg, batch, fused=fused, splits=splits,
                                         logits_dtype=logits_dtype, stack=stack,
                                         check_status=check_status, large_fused=large_fused,
-                                        stack_trace=stack_trace is not None)
+                                        stack_trace=stack_trace is not None, **self._mx)
         # prefill=True: generate() runs the prompt through one prefill graph (the layers over
         # [B, S] tokens at once), which reads the unpacked q/k/v and gate/up weights
         self.prefill = prefill
         self._prefill_graphs: dict = {}
-        if fused and not uses_large_graph(cfg, fused):
+        if mx is not None:
+            tensors = pack_mx_weights(cfg, weights, self.engine)
+        elif fused and not uses_large_graph(cfg, fused):
             tensors = pack_fused_weights(cfg, weights, drop_unfused=not prefill)
         elif large_fused:
             tensors = pack_large_weights(cfg, weights)
@@ -153,11 +162,14 @@ class DecodeSession:
             raise ValueError("prompt exceeds the KV cache capacity")
         graph = self._prefill_graphs.get(s)
         if graph is None:
-            on_gpu = prompt.is_cuda and self.fused and not uses_large_graph(self.cfg, self.fused)
+            # (attention writes [B, S, H, D] itself in the fused and the microscaled form)
+            on_gpu = prompt.is_cuda and (bool(self._mx) or (
+                self.fused and not uses_large_graph(self.cfg, self.fused)))
             # lm_head_argmax holds a tile's rows in registers (hidden <= 1024): larger hiddens
             # take rms_norm + linear + argmax
             fused_head = prompt.is_cuda and not uses_large_graph(self.cfg, True)
-            graph = build_prefill_graph(self.cfg, b, s, fused_head=fused_head, fused=on_gpu)
+            graph = build_prefill_graph(self.cfg, b, s, fused_head=fused_head, fused=on_gpu,
+                                        **self._mx)
             self._prefill_graphs[s] = graph
         self.engine.set_kv_cache_length(0)  # the prompt starts every sequence at position 0
         inputs = dict(self.inputs)
