@@ -377,7 +377,7 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
         h = "hidden_states"
         for i in range(cfg.layers):
             h = _mx_layer_nodes(cfg, batch, None, i, h, nodes, mx, dtype, False)
-        if fused and not uses_large_graph(cfg, fused):
+        if fused and not uses_large_graph(cfg, fused) and dtype == "bfloat16":
             _head_nodes(cfg, nodes, h, logits_dtype)
         else:
             _plain_head_nodes(cfg, nodes, h)

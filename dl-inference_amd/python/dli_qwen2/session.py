@@ -162,12 +162,14 @@ class DecodeSession:
             raise ValueError("prompt exceeds the KV cache capacity")
         graph = self._prefill_graphs.get(s)
         if graph is None:
-            # (attention writes [B, S, H, D] itself in the fused and the microscaled form)
-            on_gpu = prompt.is_cuda and (bool(self._mx) or (
-                self.fused and not uses_large_graph(self.cfg, self.fused)))
+            on_gpu = prompt.is_cuda and self.fused and not uses_large_graph(self.cfg, self.fused)
+            if self._mx:  # attention's [B, S, H, D] output, a form of bf16 and head_dim 64
+                on_gpu = (prompt.is_cuda and self.cfg.head_dim == 64
+                          and self._mx["dtype"] == "bfloat16")
             # lm_head_argmax holds a tile's rows in registers (hidden <= 1024): larger hiddens
-            # take rms_norm + linear + argmax
-            fused_head = prompt.is_cuda and not uses_large_graph(self.cfg, True)
+            # take rms_norm + linear + argmax (as do microscaled graphs of other types)
+            fused_head = (prompt.is_cuda and not uses_large_graph(self.cfg, True)
+                          and self._mx.get("dtype", "bfloat16") == "bfloat16")
             graph = build_prefill_graph(self.cfg, b, s, fused_head=fused_head, fused=on_gpu,
                                         **self._mx)
             self._prefill_graphs[s] = graph

@@ -44,6 +44,22 @@ def test_prompt_node_by_node(form, seq):
     check_step(s, ids, torch.full((2,), seq, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float16])
+@pytest.mark.parametrize("head_dim,hidden", [(64, 896), (128, 1280)])
+def test_prompt_then_steps(dtype, head_dim, hidden):
+    """Every type and head size that a prompt may have, then decode steps from its cache."""
+    cfg = replace(tiny_config(ffn=1216), hidden=hidden, head_dim=head_dim, heads=8,
+                  tied_embeddings=False)
+    w = on_gpu(random_weights(cfg, seed=9, dtype=dtype))
+    prompt = torch.randint(0, cfg.vocab, (2, 5), generator=torch.Generator().manual_seed(3)).cuda()
+    s = DecodeSession(cfg, w, 2, max_seq_len=32, mx="fp8", prefill=True)
+    logits, ids = s.run_prefill(prompt)
+    assert torch.equal(logits.argmax(-1), ids)
+    out = check_step(s, ids, torch.full((2,), 5, device="cuda"))
+    assert out["layers_0_output"].dtype == dtype
+    assert s.generate(prompt, 3).shape == (2, 3)
+
+
 @pytest.mark.parametrize("form", ["fp8", "fp4"])
 def test_captured_steps_repeat_eager_ones(form):
     cfg = tiny_config(ffn=1216)
