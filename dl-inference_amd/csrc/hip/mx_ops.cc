@@ -54,10 +54,11 @@ DeviceKernel k_stream[2][3][4][2][3] = {
     {DLI_MX_STREAM("1", ""), DLI_MX_STREAM("4", ""), DLI_MX_STREAM("16", "")},
     {DLI_MX_STREAM("1", "_odd"), DLI_MX_STREAM("4", "_odd"), DLI_MX_STREAM("16", "_odd")}};
 
-// [tile: 256 x 256, 128 x 128, 64 x 128, then the last two on scales as they are][format][dtype]
-DeviceKernel k_tile[5][2][3] = {DLI_MX_LINEAR("mx_tile_256", ""), DLI_MX_LINEAR("mx_tile_128", ""),
+// [tile: 256 x 256, 128 x 128, 64 x 128, then the last two and 64 x up to 256 on scales as they are]
+// [format][dtype]
+DeviceKernel k_tile[6][2][3] = {DLI_MX_LINEAR("mx_tile_256", ""), DLI_MX_LINEAR("mx_tile_128", ""),
                                 DLI_MX_LINEAR("mx_tile_64", ""), DLI_MX_LINEAR("mx_tile_128r", ""),
-                                DLI_MX_LINEAR("mx_tile_64r", "")};
+                                DLI_MX_LINEAR("mx_tile_64r", ""), DLI_MX_LINEAR("mx_tile_64w", "")};
 DeviceKernel k_sum_parts[3] = {{"mx_linear", "mx_sum_parts_f32"},
                                {"mx_linear", "mx_sum_parts_bf16"},
                                {"mx_linear", "mx_sum_parts_f16"}};
@@ -73,13 +74,14 @@ int64_t scaleWordBytes(int64_t m, int64_t n, int64_t k) {
   return scaleWords(k) * 4 * (padded256(m) + padded256(n));
 }
 
-// How a product runs: the tile (0 to 2; -1: the weight stream), the parts of K, and whether the tile
-// kernel reads the scales as they are.
+// How a product runs: the tile (-1: the weight stream), the parts of K, and whether the tile kernel
+// reads the scales as they are.
 struct Plan {
   int tile, parts;
   bool rows;
+  int64_t width;  // columns of a tile
 };
-constexpr int kTileRows[3] = {256, 128, 64}, kTileColumns[3] = {256, 128, 128};
+constexpr int kTileRows[4] = {256, 128, 64, 64}, kTileColumns[3] = {256, 128, 128};
 
 int64_t tilesOf(int tile, int64_t m, int64_t n) {
   return (m + kTileRows[tile] - 1) / kTileRows[tile] *
@@ -89,13 +91,21 @@ int64_t tilesOf(int tile, int64_t m, int64_t n) {
 // words: the scales are rows of aligned words (K % 128 == 0).
 Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // Row offsets within a tile are 32-bit.
-  if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1, false};
+  if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1, false, 0};
   // The stream takes about 3 us and one for 1000 of its units; where the tiles need their scales laid
   // out first, it does small products sooner (333 x 1003 x 928 in fp4, a call: 8.0 us, 21.6 in tiles).
-  if (!words && (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256) < 10000) return {-1, 1, false};
+  if (!words && (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256) < 10000) return {-1, 1, false, 0};
   // Large tiles once they fill most of the 256 CUs (1500 x 9728 x 896, 228 tiles: 23.5 us, in tiles of
   // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
-  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false};
+  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false, 256};
+  // Up to 64 rows are bound by what one CU can load. Where tiles of 128 columns would fall on some CUs
+  // twice and on others once, every CU takes an equal run of columns instead (64 x 37888 x 3584: 24.0
+  // us, 31.1 in 296 tiles; 64 x 60000 x 3584 32.7 and 35.4). Past two tiles to a CU both take as long
+  // (70000 columns: 46.4 and 45.8), and over a short K the tiles' smaller stages start sooner (64 x
+  // 37888 x 1024: 12.2 and 11.3).
+  const int64_t tiles64 = tilesOf(2, m, n);
+  if (m <= 64 && words && tiles64 > 256 && tiles64 <= 512 && k >= 2048 && k <= 4096)
+    return {3, 1, true, ((n + 255) / 256 + 7) / 8 * 8};
   // Parts of K until the small tiles are about two to a CU (one of 64 rows), each part at least 2048
   // columns (1024): 484 x 3584 x 18944 in 1, 2, 4 and 8 parts 85.6, 58.2, 53.6 and 62.4 us; 64 rows
   // 60.0, 37.4, 26.1, 22.7 and, in 16, 26.6; 700 x 4608 x 3584 24.3 whole and 30.1 in 2.
@@ -106,7 +116,7 @@ Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // Reading scales as they are takes a cache line for every 8 bytes, over a long K more than the launch
   // that lays them out (64 x 9728 x 896: 6.5 us as they are, 9.7 laid out; 700 x 4608 x 3584: 21.1 and
   // 24.7; 484 x 3584 x 18944 in 4 parts 60.2 and 52.8; 2000 x 3584 x 18944 180 and 139).
-  return {tile, static_cast<int>(parts), words && k / parts <= 4096};
+  return {tile, static_cast<int>(parts), words && k / parts <= 4096, 128};
 }
 
 // 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
@@ -229,13 +239,11 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
     return badArg(op, "codes must be 16-byte aligned");
   const bool words = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4);
   Plan plan = planFor(m, n, k, words);
-  if (workspace == nullptr && plan.rows) plan.parts = 1;  // no room for parts
   const int64_t scale_bytes = plan.rows ? 0 : scaleWordBytes(m, n, k);
-  const int64_t part_bytes = plan.parts > 1 ? plan.parts * m * n * 4 : 0;
-  const auto needed = static_cast<size_t>(scale_bytes + part_bytes);
-  if (plan.tile >= 0 &&
-      (needed == 0 ||
-       (workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16)))) {
+  const auto needed = static_cast<size_t>(scale_bytes + (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
+  const bool room = workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16);
+  if (!room && plan.rows) plan.parts = 1;
+  if (plan.tile >= 0 && (room || plan.rows)) {
     const int64_t m_pad = padded256(m), n_pad = padded256(n), row_words = scaleWords(k);
     auto* const parts = plan.parts > 1 ? static_cast<char*>(workspace) + scale_bytes : nullptr;
     const void *xw = x_scales, *ww = w_scales;
@@ -249,12 +257,12 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
                           static_cast<int>(k / 32), m_pad, n_pad))
         return rc;
     }
-    const unsigned threads = plan.tile == 0 && x_format == DLI_MX_FP8 ? 512 : 256;
+    const unsigned threads = plan.tile == 3 || (plan.tile == 0 && x_format == DLI_MX_FP8) ? 512 : 256;
     if (int rc = launch(k_tile[plan.tile + (plan.rows ? 2 : 0)][x_format][dtypeIndex(out_dtype)],
-                        {blocksFor(n, kTileColumns[plan.tile]), blocksFor(m, kTileRows[plan.tile]),
+                        {blocksFor(n, plan.width), blocksFor(m, kTileRows[plan.tile]),
                          static_cast<unsigned>(plan.parts)},
                         {threads}, 0, stream, x_codes, xw, w_codes, ww, bias, residual, out, parts,
-                        m, n, k, m_pad, n_pad))
+                        m, n, k, m_pad, n_pad, static_cast<int>(plan.width)))
       return rc;
     if (parts == nullptr) return 0;
     return launch(k_sum_parts[dtypeIndex(out_dtype)], {chunkBlocks((m * n + 7) / 8)}, {256}, 0,

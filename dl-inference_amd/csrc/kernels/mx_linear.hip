@@ -407,7 +407,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
                                               const uint8_t* w, const uint32_t* ww,
                                               const void* bias, const void* residual, void* out,
                                               float* parts, int64_t M, int64_t N, int64_t K,
-                                              int64_t mPad, int64_t nPad) {
+                                              int64_t mPad, int64_t nPad, int width) {
   constexpr int kWaves = WM * WN, kM = BM / WM, kN = BN / WN;  // a wave's part of the tile
   using B = Big<F, BM, BN, KS, kWaves, kRowScales>;
   constexpr bool kSplit = sizeof(T) == 4;
@@ -421,7 +421,8 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int wm = wave / WN, wn = wave % WN;
   int64_t m0, n0;
-  groupedTile(BM, BN, m0, n0);
+  const int bn = kRowScales && BM == 64 ? width : BN;  // the tile's columns, a multiple of 8
+  groupedTile(BM, bn, m0, n0);
   const int blocks = static_cast<int>(K / kMxBlock);
   // the stages of this part of K (blockIdx.z of gridDim.z), and the blocks of its last one
   const int all = static_cast<int>((K + KS - 1) / KS);
@@ -437,7 +438,8 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   const uint8_t* const xsTile = uniform(reinterpret_cast<const uint8_t*>(xw) + (kRowScales ? m0 * blocks : 0));
   const uint8_t* const wsTile = uniform(reinterpret_cast<const uint8_t*>(ww) + (kRowScales ? n0 * blocks : 0));
   const int mLast = static_cast<int>(M - 1 - m0 < BM ? M - 1 - m0 : BM - 1);
-  const int nLast = static_cast<int>(N - 1 - n0 < BN ? N - 1 - n0 : BN - 1);
+  const int nLast = static_cast<int>(N - 1 - n0 < bn ? N - 1 - n0 : bn - 1);
+  const int64_t nEnd = n0 + nLast + 1;
 
   // ---- loads ----
   constexpr int kXPer = B::kXRow / 16, kWPer = B::kWRow / 16;  // chunks per row
@@ -682,7 +684,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
       const int c = (lane % kRuns) * 8;
       const int64_t n = n0 + wn * kN + c;
       float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (bias != nullptr && part == nullptr && n < N)
+      if (bias != nullptr && part == nullptr && n < nEnd)
         mxLoad8<T, true>(static_cast<const T*>(bias) + n, b);
 #pragma unroll 4
       for (int p = 0; p < 32; p += kRows) {
@@ -695,7 +697,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
           v[e] = lo[e] + b[e];
           v[4 + e] = hi[e] + b[4 + e];
         }
-        if (mq + row >= M || n >= N) continue;
+        if (mq + row >= M || n >= nEnd) continue;
         const int64_t at = (mq + row) * N + n;
         if (part != nullptr) {
           mxStore8<float, true>(part + at, v);
@@ -715,7 +717,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
       for (int run = 0; run < kN / 64; ++run) {
         const int c = run * 64 + lane;
         const int64_t n = n0 + wn * kN + c;
-        if (n >= N) continue;
+        if (n >= nEnd) continue;
         const float b = bias != nullptr && part == nullptr ? ld(static_cast<const T*>(bias) + n) : 0.f;
         const T* const pr = part == nullptr ? static_cast<const T*>(residual) : nullptr;
         for (int p = 0; p < 32; p += 8) {
@@ -858,9 +860,9 @@ MX_STREAM_ROWS(16, 2)
       __attribute__((amdgpu_waves_per_eu(PER, PER)))                                             \
       name(const uint8_t* x, const uint32_t* xw, const uint8_t* w, const uint32_t* ww,           \
            const void* bias, const void* residual, void* out, float* parts, int64_t M,           \
-           int64_t N, int64_t K, int64_t mPad, int64_t nPad) {                                   \
+           int64_t N, int64_t K, int64_t mPad, int64_t nPad, int width) {                        \
     mx_linear_big<F, T, BM, BN, WM, WN, KS, ST, RS>(x, xw, w, ww, bias, residual, out, parts, M, \
-                                                    N, K, mPad, nPad);                           \
+                                                    N, K, mPad, nPad, width);                    \
   }
 #define MX_BIG_FORMS(name, F, BM, BN, WM, WN, KS, ST, PER, RS)         \
   MX_BIG(name##_f32, F, float, BM, BN, WM, WN, KS, ST, PER, RS)        \
@@ -880,6 +882,10 @@ MX_BIG_FORMS(mx_tile_128r_fp8, MxFp8, 128, 128, 2, 2, 128, 3, 2, true)
 MX_BIG_FORMS(mx_tile_128r_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2, true)
 MX_BIG_FORMS(mx_tile_64r_fp8, MxFp8, 64, 128, 2, 2, 256, 2, 2, true)
 MX_BIG_FORMS(mx_tile_64r_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2, true)
+
+// one workgroup to a CU, of as many columns as the launch says: three stages of 48 KB
+MX_BIG_FORMS(mx_tile_64w_fp8, MxFp8, 64, 256, 2, 4, 256, 3, 2, true)
+MX_BIG_FORMS(mx_tile_64w_fp4, MxFp4, 64, 256, 2, 4, 256, 3, 2, true)
 
 #define MX_SUM_PARTS(name, T)                                                                 \
   extern "C" __global__ void __launch_bounds__(256)                                           \

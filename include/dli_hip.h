@@ -95,7 +95,8 @@ int dli_hip_set_device(int device);
  * any grid dimension 0 returns 0 without touching the runtime (cuda_driver.cc:123). */
 int dli_hip_module_load(const void* image, size_t image_bytes, void** module);
 /* Image of the library's embedded gfx950 code object `name` ("attention", "conv", "decode",
- * "elementwise", "flash_attention", "gemm", "mfma_gemm", "norm", "stack"), for
+ * "elementwise", "flash_attention", "gemm", "mfma_gemm", "mx_linear", "mx_quantize", "norm",
+ * "stack"), for
  * dli_hip_module_load. The reference's counterpart is the cubin file its plugin reads next to
  * itself (CudaAotKernel::load, cuda_driver.cc:107-117); here the images live inside the library.
  * The image stays valid while the library is loaded. */
@@ -571,9 +572,11 @@ int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up,
 /* out[m, n] = sum_k x[m, k] * w[n, k] (+ bias[n]) (+ residual[m, n]), rounded once to out_dtype
  * (fp32, bf16 or f16). x: microscaled [m, k] in x_format; w: microscaled [n, k] in DLI_MX_FP4.
  * bias and residual (out_dtype) may be NULL; residual may be out itself. Scaled MFMA, fp32 sums.
- * A workspace of dli_hip_mx_linear_workspace bytes (of any content; 0 for most shapes) lets shapes
- * with few output tiles and a long k split k over more workgroups, summed in a fixed order; with
- * NULL or a smaller one they do not. codes must be 16-byte aligned. */
+ * A workspace of dli_hip_mx_linear_workspace bytes, 16-byte aligned and of any content, holds the
+ * scales in the order that the tile kernels read them and the partial sums of products with few
+ * output tiles and a long k, added in a fixed order. It is 0 for up to 16 rows and for many other
+ * shapes; with NULL or a smaller one the product runs in a form that needs none, at most of the
+ * shapes slower. Two calls that may run at once need one each. codes must be 16-byte aligned. */
 size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k);
 int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
                       const void* w_codes, const void* w_scales, const void* bias,

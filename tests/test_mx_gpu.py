@@ -6,6 +6,7 @@ import torch
 
 import dli
 import mx_oracle as mx
+from dli import hip
 from support import one_node_graph, plugin_engine, run_op
 from test_mx_cpu import DTYPES, some, special_rows
 
@@ -401,3 +402,76 @@ def test_offsets_past_32_bits():
     assert y.numel() > 2 ** 31
     ref = (mx.values(host(q[0][-3:]), host(q[1][-3:])) @ mx.values(host(w[0]), host(w[1])).T)
     assert np.linalg.norm(host(y[-3:].double()) - ref) <= 2.5e-3 * np.linalg.norm(ref)
+
+
+@pytest.mark.parametrize("form,out_dtype", [("fp8", "bfloat16"), ("fp4", "float16"),
+                                            ("fp8", "float32"), ("fp4", "float32")])
+@pytest.mark.parametrize("m,n,k", [
+    (3001, 4104, 416), (1537, 8193, 288),   # tiles of 256 x 256, partly past every end
+    (64, 33000, 2176), (17, 32803, 2048),   # one run of columns per CU
+    (2047, 1300, 2336), (90, 520, 8256), (40, 200, 6272)])  # parts of K
+def test_linear_of_many_tiles(form, out_dtype, m, n, k):
+    check_linear(form, out_dtype, m, n, k)
+
+
+def c_linear(form, t, m, n, k, workspace=None, ws_bytes=0, out=None):
+    """The C entry point on the tensors of check_linear's inputs."""
+    out = torch.empty_like(t["r"]) if out is None else out
+    hip.call("dli_hip_mx_linear", hip.MX_FP8 if form == "fp8" else hip.MX_FP4, hip.dtype_code(out),
+             hip.ptr(t["x"]), hip.ptr(t["xs"]), hip.ptr(t["w"]), hip.ptr(t["ws"]), hip.ptr(t["b"]),
+             hip.ptr(t["r"]), hip.ptr(out), m, n, k, workspace, ws_bytes, hip.current_stream())
+    return out
+
+
+@pytest.mark.parametrize("form", ["fp8", "fp4"])
+@pytest.mark.parametrize("m,n,k", [(40, 200, 6272), (90, 520, 8256), (300, 1003, 1056),
+                                   (700, 1300, 640)])
+def test_linear_with_any_workspace(form, m, n, k):
+    """Without a workspace, with one that is too small or not aligned, and with one of any content
+    inside a larger buffer whose ends stay as they were."""
+    inputs, _, out = check_linear(form, "float32", m, n, k)
+    size = hip.lib().dli_hip_mx_linear_workspace(hip.MX_FP8 if form == "fp8" else hip.MX_FP4, m, n, k)
+    # two orders of the same fp32 sums, each within the bound of check_linear
+    x, w = (np.abs(mx.values(host(inputs[a]), host(inputs[b]))) for a, b in (("x", "xs"), ("w", "ws")))
+    terms = torch.from_numpy(x @ w.T).cuda() + inputs["b"].abs() + inputs["r"].abs()
+    bound = (k // 8 + 4) * 2.0 ** -22 * terms
+
+    def close(got):
+        assert ((got.double() - out.double()).abs() <= bound).all()
+
+    close(c_linear(form, inputs, m, n, k))
+    buffer = torch.full((size + 512,), 255, dtype=torch.uint8, device="cuda")
+    for offset, count in ((256, size), (256, size - 1), (260, size)):
+        if count <= 0:
+            continue
+        buffer.fill_(255)
+        got = c_linear(form, inputs, m, n, k, buffer.data_ptr() + offset, count)
+        close(got)
+        assert (buffer[:256] == 255).all() and (buffer[256 + size:] == 255).all()
+    # the residual's own memory as the output
+    alias = inputs["r"].clone()
+    got = c_linear(form, {**inputs, "r": alias}, m, n, k, buffer.data_ptr() + 256, size, out=alias)
+    close(got)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("rows,hidden", [(3, 96), (5, 896), (4, 3584), (2, 8192), (3, 9000 // 32 * 32),
+                                         (70000, 32)])
+def test_norm_in_place(dtype, rows, hidden):
+    """hidden_out as x or as the residual, at every width of the kernel and past 65535 rows."""
+    t = DTYPES[dtype]
+    x, r, w = (some(s, t, i).cuda() for i, s in enumerate([(rows, hidden), (rows, hidden),
+                                                           (hidden,)]))
+    want = run_op("rms_norm_mx", {"x": x, "w": w, "r": r}, ("c", "s", "h"), {"format": "fp8"})
+    assert torch.equal(want["h"], (x.float() + r.float()).to(t))
+    for which in ("x", "r", None):
+        a, b = x.clone(), r.clone()
+        to = {"x": a, "r": b, None: None}[which]
+        c = torch.empty(rows, hidden, dtype=torch.uint8, device="cuda")
+        s = torch.empty(rows, hidden // 32, dtype=torch.uint8, device="cuda")
+        hip.call("dli_hip_rms_norm_mx", hip.dtype_code(x), hip.MX_FP8, hip.ptr(a), hip.ptr(b),
+                 hip.ptr(w), hip.ptr(to), hip.ptr(c), hip.ptr(s), rows, hidden, 1e-6,
+                 hip.current_stream())
+        assert torch.equal(c, want["c"]) and torch.equal(s, want["s"])
+        if to is not None:
+            assert torch.equal(to, want["h"])
