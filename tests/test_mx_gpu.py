@@ -408,6 +408,7 @@ def test_offsets_past_32_bits():
                                             ("fp8", "float32"), ("fp4", "float32")])
 @pytest.mark.parametrize("m,n,k", [
     (3001, 4104, 416), (1537, 8193, 288),   # tiles of 256 x 256, partly past every end
+    (4100, 8200, 416), (4200, 8193, 96), (4100, 4104, 768),  # more than one to a CU
     (64, 33000, 2176), (17, 32803, 2048),   # one run of columns per CU
     (2047, 1300, 2336), (90, 520, 8256), (40, 200, 6272)])  # parts of K
 def test_linear_of_many_tiles(form, out_dtype, m, n, k):
