@@ -92,9 +92,13 @@ int64_t tilesOf(int tile, int64_t m, int64_t n) {
 Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // Row offsets within a tile are 32-bit.
   if (m <= 16 || k > (int64_t{1} << 23)) return {-1, 1, false, 0};
-  // The stream takes about 3 us and one for 1000 of its units; where the tiles need their scales laid
-  // out first, it does small products sooner (333 x 1003 x 928 in fp4, a call: 8.0 us, 21.6 in tiles).
-  if (!words && (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256) < 10000) return {-1, 1, false, 0};
+  // Small products stay on the stream, which takes about 3 us and one for 1000 of its units (16 x 16
+  // outputs, 256 columns): 64 x 512 x 3584 5.3 us, 9.0 in tiles and their parts; 32 x 3584 x 3584 7.1
+  // and 9.9 (64 rows 11.7 and 10.8); 64 x 896 x 4864 5.9 and 10.5; 200 x 896 x 896 5.7 and 6.8; 20 x 9728
+  // x 896 8.7 and 6.2. The tiles' time grows with the columns that one walks, and by a launch where
+  // their scales have to be laid out (333 x 1003 x 928 in fp4, a call: 8.0 and 21.6).
+  const int64_t units = (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256);
+  if (units < (words ? 3000 + (k < 5000 ? k : 5000) : 10000)) return {-1, 1, false, 0};
   // Large tiles once they fill most of the 256 CUs (1500 x 9728 x 896, 228 tiles: 23.5 us, in tiles of
   // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
   if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false, 256};

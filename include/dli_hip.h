@@ -96,9 +96,9 @@ int dli_hip_set_device(int device);
 int dli_hip_module_load(const void* image, size_t image_bytes, void** module);
 /* Image of the library's embedded gfx950 code object `name` ("attention", "conv", "decode",
  * "elementwise", "flash_attention", "gemm", "mfma_gemm", "mx_linear", "mx_quantize", "norm",
- * "stack"), for
- * dli_hip_module_load. The reference's counterpart is the cubin file its plugin reads next to
- * itself (CudaAotKernel::load, cuda_driver.cc:107-117); here the images live inside the library.
+ * "stack"), for dli_hip_module_load. The reference's counterpart is the cubin file its plugin reads
+ * next to itself (CudaAotKernel::load, cuda_driver.cc:107-117); here the images live inside the
+ * library.
  * The image stays valid while the library is loaded. */
 int dli_hip_code_object(const char* name, const void** image, size_t* image_bytes);
 int dli_hip_module_get_function(void* module, const char* name, void** function);

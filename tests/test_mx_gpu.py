@@ -410,7 +410,9 @@ def test_offsets_past_32_bits():
     (3001, 4104, 416), (1537, 8193, 288),   # tiles of 256 x 256, partly past every end
     (4100, 8200, 416), (4200, 8193, 96), (4100, 4104, 768),  # more than one to a CU
     (64, 33000, 2176), (17, 32803, 2048),   # one run of columns per CU
-    (2047, 1300, 2336), (90, 520, 8256), (40, 200, 6272)])  # parts of K
+    (50, 9001, 896), (60, 9001, 1056),      # tiles of 64 rows, on scales as they are and laid out
+    (60, 4700, 3712), (50, 1300, 8224), (300, 1003, 8288),  # and parts of K
+    (2047, 1300, 2336), (90, 520, 8256), (40, 200, 6272)])
 def test_linear_of_many_tiles(form, out_dtype, m, n, k):
     check_linear(form, out_dtype, m, n, k)
 
@@ -425,8 +427,8 @@ def c_linear(form, t, m, n, k, workspace=None, ws_bytes=0, out=None):
 
 
 @pytest.mark.parametrize("form", ["fp8", "fp4"])
-@pytest.mark.parametrize("m,n,k", [(40, 200, 6272), (90, 520, 8256), (300, 1003, 1056),
-                                   (700, 1300, 640)])
+@pytest.mark.parametrize("m,n,k", [(40, 200, 6272), (60, 4700, 3712), (50, 1300, 8224),
+                                   (300, 1003, 8288), (700, 1300, 640)])
 def test_linear_with_any_workspace(form, m, n, k):
     """Without a workspace, with one that is too small or not aligned, and with one of any content
     inside a larger buffer whose ends stay as they were."""
