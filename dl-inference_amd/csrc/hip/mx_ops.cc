@@ -233,8 +233,9 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
   if (k == 0) return badArg(op, "k must be positive");
   if (n > 0 && m > (int64_t{1} << 56) / n) return badArg(op, "output is too large");
   if (m == 0 || n == 0) return 0;
-  if (m > 65535 * int64_t{16} || n > (int64_t{1} << 31) - 64)
-    return badArg(op, "m must be at most 1048560, n below 2^31 - 64");
+  // (a launch has fewer than 2^32 threads along x: 4 per output column at most)
+  if (m > 65535 * int64_t{16} || n > int64_t{1} << 29)
+    return badArg(op, "m must be at most 1048560, n at most 2^29");
   if (k > int64_t{1} << 28) return badArg(op, "k must be at most 2^28");
   if (x_codes == nullptr || x_scales == nullptr || w_codes == nullptr || w_scales == nullptr ||
       out == nullptr)

@@ -159,7 +159,6 @@ __device__ __forceinline__ void rms_norm_mx_impl(const void* x, const void* resi
                                                  const void* weight, void* hidden_out,
                                                  uint8_t* codes, uint8_t* scales, int64_t rows,
                                                  int64_t hidden, double share, float eps) {
-  FP_EXACT
   __shared__ double scratch[4];
   const T* pw = static_cast<const T*>(weight);
   const int64_t chunks = hidden / 8, held = (chunks + blockDim.x - 1) / blockDim.x;

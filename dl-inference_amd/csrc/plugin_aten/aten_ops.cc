@@ -450,7 +450,7 @@ bool mxIsFp8(const Attributes& attrs, const std::string& op) {
 // Quantises y [.., K] in fp32 into codes and scales.
 void mxQuantize(const at::Tensor& y, bool fp8, const std::string& op, Tensor& codes_out,
                 Tensor& scales_out) {
-  const std::int64_t k = y.size(-1);
+  const std::int64_t k = y.dim() == 0 ? 1 : y.size(-1);
   if (k <= 0 || k % kMxBlock != 0)
     throw std::invalid_argument(op + ": the last dimension must be a positive multiple of 32");
   std::vector<std::int64_t> shape(y.sizes().begin(), y.sizes().end());
@@ -575,7 +575,7 @@ class SiluMulMxOp final : public Operator {
         throw std::invalid_argument("silu_mul_mx gate and up must have one shape");
       up = f32(*in[1]);
     } else {
-      if (gate.size(-1) % 2 != 0)
+      if (gate.dim() == 0 || gate.size(-1) % 2 != 0)
         throw std::invalid_argument("silu_mul_mx: a joined gate and up has an even last dimension");
       const std::vector<at::Tensor> halves = gate.chunk(2, -1);
       gate = halves[0];

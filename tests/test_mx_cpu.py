@@ -139,6 +139,20 @@ def test_operators_refuse_what_is_not_microscaled():
             aten(op, inputs, outputs, attrs)
 
 
+def test_operators_refuse_scalars():
+    one, byte = torch.tensor(1.0), torch.tensor(1, dtype=torch.uint8)
+    c, s = (torch.from_numpy(a) for a in mx.quantize(np.ones((2, 64)), "fp4"))
+    for op, inputs, n, text in (
+            ("mx_quantize", {"x": one}, 2, "multiple of 32"),
+            ("mx_dequantize", {"c": byte, "s": byte}, 1, "not a microscaled"),
+            ("rms_norm_mx", {"x": one, "w": one}, 2, "multiple of 32"),
+            ("silu_mul_mx", {"g": one}, 2, "even"),
+            ("silu_mul_mx", {"g": one, "u": one}, 2, "multiple of 32"),
+            ("mx_linear", {"x": byte, "xs": byte, "w": c, "ws": s}, 1, "not a microscaled")):
+        with pytest.raises(ValueError, match=text):
+            aten(op, inputs, tuple(f"o{i}" for i in range(n)))
+
+
 def test_gpu_operators_refuse_host_tensors():
     x = torch.randn(2, 64)
     for op, inputs, n in (("mx_quantize", {"x": x}, 2), ("rms_norm_mx", {"x": x, "w": x[0]}, 2),
@@ -189,6 +203,9 @@ def test_entry_points_check_their_arguments():
     says(linear(x=ctypes.c_void_p(264)), b"16-byte aligned")
     says(linear(w=None), b"NULL")
     says(linear(m_=1 << 40, n=1 << 40), b"too large")
+    says(linear(n=(1 << 29) + 1), b"n at most 2^29")
+    says(linear(m_=(1 << 20) - 15), b"m must be at most 1048560")
+    says(linear(k=(1 << 28) + 32), b"k must be at most 2^28")
     assert lib.dli_hip_mx_linear_workspace(0, 0, 8, 64) == 0
     assert lib.dli_hip_mx_linear_workspace(0, 4, 8, 33) == 0
 
