@@ -297,7 +297,7 @@ __device__ __forceinline__ void mx_linear_stream(const uint8_t* x, const uint8_t
     int slot = 0, u = 0;
     for (; u + kDepth <= n; ++u) {  // kDepth - 1 units in flight behind this one
       waitLoads<(kDepth - 1) * S::kLoads>();
-      multiply(u, slot, kDepth == 1 && done + u == partial ? last : 8);
+      multiply(u, slot);
       waitLdsReads();
       if (u + kDepth < n) issue(done + u + kDepth, slot);
       slot = slot + 1 == kDepth ? 0 : slot + 1;
@@ -312,7 +312,7 @@ __device__ __forceinline__ void mx_linear_stream(const uint8_t* x, const uint8_t
         slot = slot + 1 == kDepth ? 0 : slot + 1;
       }
     };
-    static_assert(kDepth <= 4, "units in flight");
+    static_assert(kDepth >= 2 && kDepth <= 4, "units in flight (the partial one is drained)");
     drain(Int<2>{});
     drain(Int<1>{});
     drain(Int<0>{});
@@ -424,7 +424,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   using B = Big<F, BM, BN, KS, kWaves, kRowScales>;
   constexpr bool kSplit = sizeof(T) == 4;
   constexpr int TM = kM / 32, TN = kN / 32, NK = KS / 64;
-  static_assert(NK % 2 == 0 && ST >= 2 && ST <= 4 && kN % 64 == 0, "stages, and the epilogue's runs");
+  static_assert(NK % 2 == 0 && ST >= 2 && ST <= 3 && kN % 64 == 0, "stages, and the epilogue's runs");
   constexpr int kPitch = kN + 4;  // floats of a row of the epilogue's slab (32 rows per wave)
   constexpr int kEpilogue = kWaves * 32 * kPitch * 4;
   constexpr int kBytes = ST * B::kStage > kEpilogue ? ST * B::kStage : kEpilogue;
@@ -586,8 +586,7 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   for (int s = 0; s < ST; ++s)
     if (s < stages) issueAll(s, s);
   auto waitStage = [&](int after) {  // `after`: stages issued behind the awaited one
-    if (ST > 3 && after >= 3) waitLoads<ST < 4 ? 0 : 3 * B::kLoads>();
-    else if (ST > 2 && after >= 2) waitLoads<ST < 3 ? 0 : 2 * B::kLoads>();
+    if (ST > 2 && after >= 2) waitLoads<ST < 3 ? 0 : 2 * B::kLoads>();
     else if (after >= 1) waitLoads<B::kLoads>();
     else waitLoads<0>();
   };
