@@ -165,7 +165,10 @@ class LinearOp final : public Operator {
     if (act == "relu") y = at::relu(y);
     else if (act != "none") throw std::invalid_argument("linear: unsupported activation " + act);
     const std::string requested = attrs.value_or<std::string>("out_dtype", "");
-    *out[0] = result(y, requested.empty() ? in[0]->dtype() : dtypeFromString(requested));
+    const DType dtype = requested.empty() ? in[0]->dtype() : dtypeFromString(requested);
+    if (dtype == DType::UInt8)  // codes and scales: a negative sum has no uint8 value
+      throw std::invalid_argument("linear: unsupported out_dtype uint8");
+    *out[0] = result(y, dtype);
   }
 };
 
