@@ -136,6 +136,20 @@ int checkTensor(const char* op, int dtype, int format, int64_t rows, int64_t k, 
   return 0;
 }
 
+// 0 when mx_linear takes a product of these sizes (planFor's arithmetic stays inside 63 bits then).
+int checkProduct(const char* op, int out_dtype, int x_format, int64_t m, int64_t n, int64_t k) {
+  if (int rc = checkTensor(op, out_dtype, x_format, m, k, "k")) return rc;
+  if (int rc = checkTensor(op, out_dtype, x_format, n, k, "k")) return rc;
+  if (k == 0) return badArg(op, "k must be positive");
+  if (m == 0 || n == 0) return 0;
+  if (m > (int64_t{1} << 56) / n) return badArg(op, "output is too large");
+  // (a launch has fewer than 2^32 threads along x: 4 per output column at most)
+  if (m > 65535 * int64_t{16} || n > int64_t{1} << 29)
+    return badArg(op, "m must be at most 1048560, n at most 2^29");
+  if (k > int64_t{1} << 28) return badArg(op, "k must be at most 2^28");
+  return 0;
+}
+
 // Grid-stride launches of one chunk (8 values) per thread: enough blocks to fill 256 CUs.
 unsigned chunkBlocks(int64_t chunks) {
   const int64_t blocks = (chunks + 255) / 256;
@@ -214,9 +228,7 @@ int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up,
 }
 
 size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k) {
-  if (checkTensor("mx_linear", DLI_F32, x_format, m, k, "k") != 0 ||
-      checkTensor("mx_linear", DLI_F32, x_format, n, k, "k") != 0 || m == 0 || n == 0 || k == 0)
-    return 0;
+  if (checkProduct("mx_linear", DLI_F32, x_format, m, n, k) != 0 || m == 0 || n == 0) return 0;
   const Plan plan = planFor(m, n, k, k % 128 == 0);
   if (plan.tile < 0) return 0;
   return static_cast<size_t>((plan.rows ? 0 : scaleWordBytes(m, n, k)) +
@@ -228,15 +240,8 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
                       const void* residual, void* out, int64_t m, int64_t n, int64_t k,
                       void* workspace, size_t workspace_bytes, void* stream) {
   const char* op = "mx_linear";
-  if (int rc = checkTensor(op, out_dtype, x_format, m, k, "k")) return rc;
-  if (int rc = checkTensor(op, out_dtype, x_format, n, k, "k")) return rc;
-  if (k == 0) return badArg(op, "k must be positive");
-  if (n > 0 && m > (int64_t{1} << 56) / n) return badArg(op, "output is too large");
+  if (int rc = checkProduct(op, out_dtype, x_format, m, n, k)) return rc;
   if (m == 0 || n == 0) return 0;
-  // (a launch has fewer than 2^32 threads along x: 4 per output column at most)
-  if (m > 65535 * int64_t{16} || n > int64_t{1} << 29)
-    return badArg(op, "m must be at most 1048560, n at most 2^29");
-  if (k > int64_t{1} << 28) return badArg(op, "k must be at most 2^28");
   if (x_codes == nullptr || x_scales == nullptr || w_codes == nullptr || w_scales == nullptr ||
       out == nullptr)
     return badArg(op, "NULL pointer");
