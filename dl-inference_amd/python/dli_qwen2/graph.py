@@ -577,7 +577,8 @@ def pack_fused_weights(cfg: Qwen2Config, weights: dict, drop_unfused: bool = Fal
 def pack_mx_weights(cfg: Qwen2Config, weights: dict, engine: "dli.Engine") -> dict:
     """The microscaled graphs' tensors: every layer's linear weight as 4-bit codes and scales
     ({name}.codes, {name}.scales), quantised by `engine` where the weight lies, gate_proj above
-    up_proj in mlp.gate_up_proj. Embedding, norms, biases and lm_head keep their type."""
+    up_proj in mlp.gate_up_proj. Embedding, norms, biases and lm_head keep their type. Weights that
+    come packed (what this function returned, stored and loaded) stay as they are."""
     _check_mx(cfg, "fp4")
     quantize = dli.Graph.from_json(json.dumps(
         {"format": "dli.graph.v1", "model_type": "mx_quantize", "inputs": ["x"],
@@ -586,15 +587,27 @@ def pack_mx_weights(cfg: Qwen2Config, weights: dict, engine: "dli.Engine") -> di
                     "outputs": ["codes", "scales"], "attrs": {"format": "fp4"}}]}))
     out = dict(weights)
 
-    def pack(name, weight):
+    def pack(name, rows, k, parts):
+        """parts: the names whose weights, one above the other, are this one."""
+        if f"{name}.codes" in out:
+            for what, width in (("codes", k // 2), ("scales", k // 32)):
+                t = out.get(f"{name}.{what}")
+                if t is None or t.dtype != torch.uint8 or tuple(t.shape) != (rows, width):
+                    raise ValueError(f"packed weight {name}.{what} must be uint8 [{rows}, {width}]")
+            for part in parts:
+                out.pop(part, None)
+            return
+        weight = torch.cat([out.pop(p) for p in parts]) if len(parts) > 1 else out.pop(parts[0])
         coded = engine.run(quantize, {"x": weight.contiguous()})
         out[f"{name}.codes"], out[f"{name}.scales"] = coded["codes"], coded["scales"]
 
+    q, kv = cfg.heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim
     for i in range(cfg.layers):
         p = f"model.layers.{i}"
-        for name in ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj",
-                     "self_attn.o_proj", "mlp.down_proj"):
-            pack(f"{p}.{name}.weight", out.pop(f"{p}.{name}.weight"))
-        pack(f"{p}.mlp.gate_up_proj.weight", torch.cat(
-            [out.pop(f"{p}.mlp.gate_proj.weight"), out.pop(f"{p}.mlp.up_proj.weight")]))
+        for name, rows, k in (("self_attn.q_proj", q, cfg.hidden), ("self_attn.k_proj", kv, cfg.hidden),
+                              ("self_attn.v_proj", kv, cfg.hidden), ("self_attn.o_proj", cfg.hidden, q),
+                              ("mlp.down_proj", cfg.hidden, cfg.ffn)):
+            pack(f"{p}.{name}.weight", rows, k, [f"{p}.{name}.weight"])
+        pack(f"{p}.mlp.gate_up_proj.weight", 2 * cfg.ffn, cfg.hidden,
+             [f"{p}.mlp.gate_proj.weight", f"{p}.mlp.up_proj.weight"])
     return out

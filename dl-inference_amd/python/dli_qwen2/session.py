@@ -22,8 +22,9 @@ class DecodeSession:
                  block_size: int = 64, logits_dtype: str = "float32", device: str = "cuda",
                  stack: bool = False, check_status: bool = False, prefill: bool = False,
                  stack_trace: "torch.Tensor | None" = None, mx: str | None = None):
-        """mx ("fp8" or "fp4"): the layers' linears run on 4-bit weights, quantised here, with
-        activations in that format; decode steps and prompts alike. It has no stack form."""
+        """mx ("fp8" or "fp4"): the layers' linears run on 4-bit weights, quantised here (or taken as
+        pack_mx_weights made them), with activations in that format; decode steps and prompts alike.
+        It has no stack form."""
         if mx is not None and stack:
             raise ValueError("the microscaled graph has no decoder stack form")
         self.cfg = cfg
