@@ -353,6 +353,12 @@ def uses_large_graph(cfg: Qwen2Config, fused: bool) -> bool:
     return fused and cfg.hidden > FUSED_MAX_HIDDEN
 
 
+def fused_head_fits(cfg: Qwen2Config, batch: int, dtype: str = "bfloat16") -> bool:
+    """Whether lm_head_argmax takes the head: it holds a tile's rows in registers (hidden a multiple
+    of 64 up to 1024, at most 64 sequences, bfloat16). Else rms_norm, linear and argmax run."""
+    return dtype == "bfloat16" and cfg.hidden <= 1024 and cfg.hidden % 64 == 0 and batch <= 64
+
+
 def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
                        splits: dict | None = None, logits_dtype: str = "float32",
                        stack: bool = False, check_status: bool = False,
@@ -360,7 +366,7 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
                        mx: str | None = None, dtype: str = "bfloat16") -> "dli.Graph":
     """mx: the layers on microscaled linears with activations in that format ("fp8", "fp4") and
     hidden states in `dtype` (_mx_layer_nodes), whatever the forms below; fused then only says
-    that the head may be one lm_head_argmax node. Else fused=False: the reference's node sequence; fused=True: five launches per layer;
+    that the head may be one lm_head_argmax node, where that takes it (fused_head_fits). Else fused=False: the reference's node sequence; fused=True: five launches per layer;
     stack=True (with fused): all layers in one decoder_stack node (check_status: the node waits
     for its launch and fails if a workgroup gave up waiting; for tests, not for capture). With
     fused=True and a hidden size above 1024 (the Qwen2-7B shape) the step is the large-hidden
@@ -377,7 +383,7 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
         h = "hidden_states"
         for i in range(cfg.layers):
             h = _mx_layer_nodes(cfg, batch, None, i, h, nodes, mx, dtype, False)
-        if fused and not uses_large_graph(cfg, fused) and dtype == "bfloat16":
+        if fused and fused_head_fits(cfg, batch, dtype):
             _head_nodes(cfg, nodes, h, logits_dtype)
         else:
             _plain_head_nodes(cfg, nodes, h)

@@ -12,7 +12,7 @@ import torch
 import dli
 
 from .config import Qwen2Config
-from .graph import (build_decode_graph, build_prefill_graph, pack_fused_weights,
+from .graph import (build_decode_graph, build_prefill_graph, fused_head_fits, pack_fused_weights,
                     pack_large_weights, pack_mx_weights, uses_large_graph)
 
 
@@ -167,10 +167,8 @@ class DecodeSession:
             if self._mx:  # attention's [B, S, H, D] output, a form of bf16 and head_dim 64
                 on_gpu = (prompt.is_cuda and self.cfg.head_dim == 64
                           and self._mx["dtype"] == "bfloat16")
-            # lm_head_argmax holds a tile's rows in registers (hidden <= 1024): larger hiddens
-            # take rms_norm + linear + argmax (as do microscaled graphs of other types)
-            fused_head = (prompt.is_cuda and not uses_large_graph(self.cfg, True)
-                          and self._mx.get("dtype", "bfloat16") == "bfloat16")
+            fused_head = prompt.is_cuda and fused_head_fits(
+                self.cfg, b, self._mx.get("dtype", "bfloat16"))
             graph = build_prefill_graph(self.cfg, b, s, fused_head=fused_head, fused=on_gpu,
                                         **self._mx)
             self._prefill_graphs[s] = graph
