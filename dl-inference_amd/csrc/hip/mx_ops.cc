@@ -103,12 +103,13 @@ Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
   if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false, 256};
   // Up to 64 rows are bound by what one CU can load. Where tiles of 128 columns would fall on some CUs
-  // twice and on others once, every CU takes an equal run of columns instead (64 x 37888 x 3584: 24.0
-  // us, 31.1 in 296 tiles; 64 x 60000 x 3584 32.7 and 35.4). Past two tiles to a CU both take as long
-  // (70000 columns: 46.4 and 45.8), and over a short K the tiles' smaller stages start sooner (64 x
-  // 37888 x 1024: 12.2 and 11.3).
+  // twice and on others once, every CU takes an equal run of columns instead. In tiles and in runs, us:
+  // 64 x 37888 x 3584 31.1 and 24.0; over K = 8192, 33000 columns 59.7 and 49.7, 65536 89.6 and 79.8;
+  // K = 18944, 33000 columns 116.7 and 98.7, 65536 166.2 and 149.3. Past two tiles to a CU both take as
+  // long (70000 x 3584: 46.4 and 45.8), and over a short K the tiles' smaller stages start as soon or
+  // sooner (K = 1024: 33000 columns 11.2 and 10.4, 65536 13.2 and 13.6).
   const int64_t tiles64 = tilesOf(2, m, n);
-  if (m <= 64 && words && tiles64 > 256 && tiles64 <= 512 && k >= 2048 && k <= 4096)
+  if (m <= 64 && words && tiles64 > 256 && tiles64 <= 512 && k >= 2048)
     return {3, 1, true, ((n + 255) / 256 + 7) / 8 * 8};
   // Parts of K until the small tiles are about two to a CU (one of 64 rows), each part at least 2048
   // columns (1024): 484 x 3584 x 18944 in 1, 2, 4 and 8 parts 85.6, 58.2, 53.6 and 62.4 us; 64 rows

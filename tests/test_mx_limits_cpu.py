@@ -33,3 +33,13 @@ def test_workspace_of_the_largest_products():
         assert size(hip.MX_FP8, m, n, k) == (k + 255) // 256 * 8 * rows
     assert size(hip.MX_FP8, 1024, 1024, 1 << 28) == 0  # offsets of a tile past 32 bits: the stream
     assert size(2, 1024, 1024, 4096) == 0              # no such format
+
+
+@pytest.mark.parametrize("form", [hip.MX_FP8, hip.MX_FP4])
+@pytest.mark.parametrize("n", [32769, 49152, 65536])
+@pytest.mark.parametrize("k", [2048, 4096, 4224, 8192, 18944, 1 << 20])
+def test_runs_of_columns_over_every_long_k(form, n, k):
+    """17 to 64 rows of more tiles than CUs, fewer than two each: equal runs of columns, which read the
+    scales as they are and sum no parts, so nothing is laid out, however long K is."""
+    for m in (17, 64):
+        assert hip.load().dli_hip_mx_linear_workspace(form, m, n, k) == 0
