@@ -99,9 +99,18 @@ Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   // their scales have to be laid out (333 x 1003 x 928 in fp4, a call: 8.0 and 21.6).
   const int64_t units = (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256);
   if (units < (words ? 3000 + (k < 5000 ? k : 5000) : 10000)) return {-1, 1, false, 0};
-  // Large tiles once they fill most of the 256 CUs (1500 x 9728 x 896, 228 tiles: 23.5 us, in tiles of
-  // 128 25.2; 2000 x 3584 x 18944, 112 tiles: 205 and 138).
-  if (m > 128 && tilesOf(0, m, n) >= 192) return {0, 1, false, 256};
+  // Large tiles run one to a CU, so their time goes by whole rounds of 256, whatever part of a tile's
+  // rows is there; tiles of 128 run two to a CU and even out. Large ones pay where tiles of 128 would
+  // take at least 1.2 + 500 / k rounds to one of theirs (their scales are laid out by a launch, and first
+  // loads and the epilogue weigh more over a short K; from 1.9 rounds on they pay over any). Large tiles
+  // and tiles of 128, us, fp8: 257 x 24576 x 896 22.9 and 16.9; 2048 x 9728 x 896 37.0 and 27.0, over K =
+  // 8192 199 and 165; 512 x 37888 x 3584 97 and 90; 1025 x 9856 x 3584 50.9 and 55.5; 768 x 18944 x 3584 57
+  // and 73, x 896 22.9 and 22.6; 8192 x 37888 x 288 238 and 263. Fewer than 192 leave too many CUs empty
+  // (2000 x 3584 x 18944, 112 tiles: 205 and 138).
+  const int64_t large = tilesOf(0, m, n), rounds = (large + 255) / 256, deep_k = k < 720 ? 720 : k;
+  if (m > 128 && large >= 192 &&
+      tilesOf(1, m, n) * deep_k * 10 >= rounds * 512 * (12 * deep_k + 5000))
+    return {0, 1, false, 256};
   // Up to 64 rows are bound by what one CU can load. Where tiles of 128 columns would fall on some CUs
   // twice and on others once, every CU takes an equal run of columns instead. In tiles and in runs, us:
   // 64 x 37888 x 3584 31.1 and 24.0; over K = 8192, 33000 columns 59.7 and 49.7, 65536 89.6 and 79.8;

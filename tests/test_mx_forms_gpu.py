@@ -39,3 +39,11 @@ FORMS = [("fp8", "float32"), ("fp4", "float32"), ("fp8", "bfloat16"), ("fp4", "f
                                    (33, 32776, 18944), (64, 65537, 2176), (64, 33000, 4256)])
 def test_runs_of_columns(form, out_dtype, m, n, k):
     check(form, out_dtype, m, n, k)
+
+
+@pytest.mark.parametrize("form,out_dtype", FORMS)
+@pytest.mark.parametrize("m,n,k", [
+    (3001, 4104, 1824), (1537, 8193, 1952), (4100, 8200, 2592), (8191, 9721, 992),  # 256 x 256, past every end
+    (257, 24577, 896), (513, 16385, 1056), (2049, 9729, 640), (1025, 9857, 2560)])  # 128 x 128
+def test_large_and_smaller_tiles(form, out_dtype, m, n, k):
+    check(form, out_dtype, m, n, k)

@@ -43,3 +43,13 @@ def test_runs_of_columns_over_every_long_k(form, n, k):
     scales as they are and sum no parts, so nothing is laid out, however long K is."""
     for m in (17, 64):
         assert hip.load().dli_hip_mx_linear_workspace(form, m, n, k) == 0
+
+
+@pytest.mark.parametrize("m,n,k,large", [
+    (257, 24576, 896, False), (2048, 9728, 896, False), (300, 37888, 3584, False),
+    (1024, 18944, 3584, False), (1025, 9856, 3584, True), (768, 18944, 3584, True),
+    (8192, 37888, 3584, True), (8192, 37888, 128, True), (4096, 3584, 3584, True), (2000, 3584, 18944, False)])
+def test_large_tiles_by_their_rounds(m, n, k, large):
+    """Large tiles read scales laid out in words; tiles of 128 read them as they are up to K = 4096."""
+    size = hip.load().dli_hip_mx_linear_workspace(hip.MX_FP8, m, n, k)
+    assert (size > 0) == (large or k > 4096)
