@@ -133,6 +133,28 @@ Plan planFor(int64_t m, int64_t n, int64_t k, bool words) {
   return {tile, static_cast<int>(parts), words && k / parts <= 4096, 128};
 }
 
+// The form of a product that has no workspace for `plan`. Tiles that read the scales as they are and
+// walk all of K take about 4.5 us for 1000 of its columns and round of workgroups, the stream 0.65 us for
+// 1000 of its units: 484 x 3584 x 18944 84.7 and 323 us (54.8 with the workspace), 2000 x 3584 x 18944 168
+// and 1287 (140), 70 x 9728 x 8192 38.9 and 54.9, 64 x 20000 x 8192 41.4 and 82; 100 x 3584 x 18944 88 and 79,
+// 64 x 3584 x 18944 77 and 47, 100 x 896 x 8192 28.6 and 11.7. Other scales than rows of words go to the
+// stream, whatever it takes.
+Plan planWithout(const Plan& plan, int64_t m, int64_t n, int64_t k, bool words) {
+  if (plan.tile < 0 || (plan.rows && plan.parts == 1)) return plan;
+  const int tile = m > 64 ? 1 : 2;
+  const int64_t at_once = tile == 1 ? 512 : 256;
+  const int64_t rounds = (tilesOf(tile, m, n) + at_once - 1) / at_once;
+  const int64_t units = (m + 15) / 16 * ((n + 15) / 16) * ((k + 255) / 256);
+  if (words && units > 7 * k * rounds) return {tile, 1, true, 128};
+  return {-1, 1, false, 0};
+}
+
+size_t workspaceOf(const Plan& plan, int64_t m, int64_t n, int64_t k) {
+  if (plan.tile < 0) return 0;
+  return static_cast<size_t>((plan.rows ? 0 : scaleWordBytes(m, n, k)) +
+                             (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
+}
+
 // 0 when dtype and format are valid and [rows, k] is a shape of whole blocks.
 int checkTensor(const char* op, int dtype, int format, int64_t rows, int64_t k, const char* name) {
   if (dtypeIndex(dtype) < 0)
@@ -239,10 +261,7 @@ int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up,
 
 size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k) {
   if (checkProduct("mx_linear", DLI_F32, x_format, m, n, k) != 0 || m == 0 || n == 0) return 0;
-  const Plan plan = planFor(m, n, k, k % 128 == 0);
-  if (plan.tile < 0) return 0;
-  return static_cast<size_t>((plan.rows ? 0 : scaleWordBytes(m, n, k)) +
-                             (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
+  return workspaceOf(planFor(m, n, k, k % 128 == 0), m, n, k);
 }
 
 int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
@@ -259,11 +278,10 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
     return badArg(op, "codes must be 16-byte aligned");
   const bool words = k % 128 == 0 && aligned(x_scales, 4) && aligned(w_scales, 4);
   Plan plan = planFor(m, n, k, words);
-  const int64_t scale_bytes = plan.rows ? 0 : scaleWordBytes(m, n, k);
-  const auto needed = static_cast<size_t>(scale_bytes + (plan.parts > 1 ? plan.parts * m * n * 4 : 0));
-  const bool room = workspace != nullptr && workspace_bytes >= needed && aligned(workspace, 16);
-  if (!room && plan.rows) plan.parts = 1;
-  if (plan.tile >= 0 && (room || plan.rows)) {
+  if (workspace == nullptr || workspace_bytes < workspaceOf(plan, m, n, k) || !aligned(workspace, 16))
+    plan = planWithout(plan, m, n, k, words);
+  if (plan.tile >= 0) {
+    const int64_t scale_bytes = plan.rows ? 0 : scaleWordBytes(m, n, k);
     const int64_t m_pad = padded256(m), n_pad = padded256(n), row_words = scaleWords(k);
     auto* const parts = plan.parts > 1 ? static_cast<char*>(workspace) + scale_bytes : nullptr;
     const void *xw = x_scales, *ww = w_scales;

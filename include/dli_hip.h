@@ -575,9 +575,10 @@ int dli_hip_silu_mul_mx(int dtype, int format, const void* gate, const void* up,
  * A workspace of dli_hip_mx_linear_workspace bytes, 16-byte aligned and of any content, holds the
  * scales in the order that the tile kernels read them and the partial sums of products with few
  * output tiles and a long k, added in a fixed order. It is 0 for up to 16 rows and for many other
- * shapes; with NULL or a smaller one the product runs in a form that needs none, at most of the
- * shapes slower. Two calls that may run at once need one each. codes must be 16-byte aligned; m is at
- * most 1048560, n 2^29, k 2^28 (of sizes that the product refuses the workspace is 0). */
+ * shapes; with NULL or a smaller one the product runs in a form that needs none, which is slower at
+ * most shapes: by up to a half with many rows where k is a multiple of 128 and both scales are 4-byte
+ * aligned, else several times. Two calls that may run at once need one each. codes must be 16-byte
+ * aligned; m is at most 1048560, n 2^29, k 2^28 (of sizes that the product refuses the workspace is 0). */
 size_t dli_hip_mx_linear_workspace(int x_format, int64_t m, int64_t n, int64_t k);
 int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const void* x_scales,
                       const void* w_codes, const void* w_scales, const void* bias,

@@ -4,8 +4,8 @@ import torch
 
 from support import run_op
 from test_mx_cpu import DTYPES, some
-from test_mx_gpu import TINY, UNIT
-from test_mx_stream_gpu import coded
+from test_mx_gpu import TINY, UNIT, c_linear
+from test_mx_stream_gpu import coded, values
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +47,25 @@ def test_runs_of_columns(form, out_dtype, m, n, k):
     (257, 24577, 896), (513, 16385, 1056), (2049, 9729, 640), (1025, 9857, 2560)])  # 128 x 128
 def test_large_and_smaller_tiles(form, out_dtype, m, n, k):
     check(form, out_dtype, m, n, k)
+
+
+@pytest.mark.parametrize("form", ["fp8", "fp4"])
+@pytest.mark.parametrize("m,n,k", [(300, 11520, 4224), (700, 5633, 4480), (64, 70001, 4224)])
+def test_tiles_without_a_workspace(form, m, n, k):
+    """Without room for laid-out scales the same tiles read them as they are: the same sums, bit for
+    bit. Products that a graph captures on a stream of its own run so."""
+    inputs, out = check(form, "float32", m, n, k)
+    assert torch.equal(c_linear(form, inputs, m, n, k), out)
+
+
+@pytest.mark.parametrize("form", ["fp8", "fp4"])
+@pytest.mark.parametrize("m,n,k", [(70, 896, 18944), (64, 3584, 8192), (300, 11520, 4256), (484, 3584, 8192),
+                                   (300, 20000, 4224), (3001, 4104, 4224)])
+def test_no_workspace(form, m, n, k):
+    """The stream, tiles that walk all of K, and large products in smaller tiles."""
+    inputs, out = check(form, "float32", m, n, k)
+    # both within half the bound of check: two orders of the same fp32 sums
+    terms = (values(inputs["x"], inputs["xs"]).abs() @ values(inputs["w"], inputs["ws"]).abs().t()
+             + inputs["b"].double().abs() + inputs["r"].double().abs())
+    got = c_linear(form, inputs, m, n, k)
+    assert ((got.double() - out.double()).abs() <= (k // 8 + 4) * 2.0 ** -22 * terms).all()

@@ -11,21 +11,27 @@ from test_mx_gpu import TINY, UNIT
 pytestmark = pytest.mark.gpu
 
 
+def values(codes, scales):
+    """What finite codes and scales on the GPU stand for, in float64."""
+    if codes.shape[1] == scales.shape[1] * 32:
+        e = torch.from_numpy(mx.E4M3).cuda()[(codes % 128).int()]
+        e = e * torch.where(codes >= 128, -1.0, 1.0)
+    else:
+        both = torch.stack([codes % 16, codes // 16], -1).flatten(1)
+        e = torch.from_numpy(mx.E2M1).cuda()[(both % 8).int()] * torch.where(both >= 8, -1.0, 1.0)
+    s = torch.exp2(scales.double() - 127)
+    return (e.view(*scales.shape, 32) * s.unsqueeze(-1)).flatten(1)
+
+
 def coded(rows, k, form, seed):
     """A microscaled tensor of random finite codes and scales 2^-4 .. 2^4, and its values."""
     g = torch.Generator().manual_seed(seed)
     scales = torch.randint(123, 132, (rows, k // 32), generator=g, dtype=torch.uint8).cuda()
+    codes = torch.randint(0, 254 if form == "fp8" else 256, (rows, k if form == "fp8" else k // 2),
+                          generator=g, dtype=torch.uint8).cuda()
     if form == "fp8":
-        codes = torch.randint(0, 254, (rows, k), generator=g, dtype=torch.uint8).cuda()
         codes = codes + (codes >= 127).to(torch.uint8)  # 127 and 255 are NaN
-        table = torch.from_numpy(mx.E4M3).cuda()
-        e = table[(codes % 128).int()] * torch.where(codes >= 128, -1.0, 1.0)
-    else:
-        codes = torch.randint(0, 256, (rows, k // 2), generator=g, dtype=torch.uint8).cuda()
-        both = torch.stack([codes % 16, codes // 16], -1).flatten(1)
-        e = torch.from_numpy(mx.E2M1).cuda()[(both % 8).int()] * torch.where(both >= 8, -1.0, 1.0)
-    s = torch.exp2(scales.double() - 127)
-    return codes, scales, (e.view(rows, -1, 32) * s.unsqueeze(-1)).view(rows, k)
+    return codes, scales, values(codes, scales)
 
 
 # the waves that share K, and units of 256 columns per wave: K in whole words of scales, then not
