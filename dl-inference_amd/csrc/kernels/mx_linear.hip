@@ -674,7 +674,11 @@ __device__ __forceinline__ void mx_linear_big(const uint8_t* x, const uint32_t* 
   stage(s, Int<2>{});
 
   // ---- epilogue: through LDS, so that rows of out are written whole ----
+  // Every wave has read the last stage. The wait is written out: the compiler moves MFMAs of the last
+  // step behind the barrier and, with them, its own wait for the fragments that they use.
+  waitLdsReads();
   __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
   float* const slab = reinterpret_cast<float*>(smem) + wave * 32 * kPitch;
   float* const part = parts == nullptr ? nullptr : parts + blockIdx.z * M * N;
   const bool vec = N % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
