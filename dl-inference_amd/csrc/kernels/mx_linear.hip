@@ -902,7 +902,7 @@ MX_BIG_FORMS(mx_tile_128r_fp4, MxFp4, 128, 128, 2, 2, 256, 2, 2, true)
 MX_BIG_FORMS(mx_tile_64r_fp8, MxFp8, 64, 128, 2, 2, 256, 2, 2, true)
 MX_BIG_FORMS(mx_tile_64r_fp4, MxFp4, 64, 128, 2, 2, 256, 3, 2, true)
 // One workgroup to a CU, of as many columns as the launch says: three stages of 48 KB. 64 x 37888 x 3584
-// from memory: 24.0 us, 3.2 TB/s (e2m1 rows 21.2). The cache hands a CU about a line per 2 cycles, and
+// from memory: 24.0 us, 3.2 TB/s (e2m1 rows 23.4). The cache hands a CU about a line per 2 cycles, and
 // of the 704 of a stage 320 are for 8 bytes of scales each (3 us in all).
 MX_BIG_FORMS(mx_tile_64w_fp8, MxFp8, 64, 256, 2, 4, 256, 3, 2, true)
 MX_BIG_FORMS(mx_tile_64w_fp4, MxFp4, 64, 256, 2, 4, 256, 3, 2, true)
