@@ -310,10 +310,10 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
   const int form = m == 1 ? 0 : m <= 4 ? 1 : 2, rows = form == 0 ? 1 : form == 1 ? 4 : 16;
   // The waves that share K: about 2048 in all, up to two for a unit of 256 columns and four for 512 (half
   // of them without a unit then: their places hold fewer tiles to a workgroup, which is no slower for few
-  // outputs: 1152 of them, 16 rows, K = 256 on one wave and two 3.63 and 3.42 us, K = 512 on two and four
-  // 3.85 and 3.61; 9728, one row, 3.60 and 3.46, 3.86 and 3.87; but 9728, 16 rows in fp8, K = 512 on four take
-  // 5.73, on two 4.24: the workgroups of four no longer fit on the card at once). Eight share from 4096 on (4608 x 3584, one
-  // row: 7.8 us on 8, 5.4 on 4; 3584 x 18944: 9.9 and 10.6).
+  // outputs). us: 1152 outputs, 16 rows, K = 256 on one wave and two 3.63 and 3.42, K = 512 on two and four
+  // 3.85 and 3.61; 9728, one row, 3.60 and 3.46, 3.86 and 3.87; but 9728, 16 rows in fp8, K = 512 on two and
+  // four 4.24 and 5.73, as the workgroups of four no longer fit on the card at once. Eight share from 4096
+  // on (4608 x 3584, one row: 7.8 us on 8, 5.4 on 4; 3584 x 18944: 9.9 and 10.6).
   const int64_t tiles = (n + 15) / 16;
   int split = 0;
   while (split < 3 && (tiles << split) < 2048 && k >= (split < 2 ? 256 << split : 4096)) ++split;
