@@ -1,0 +1,816 @@
+// Attention over the 8-bit paged KV cache on gfx950 (formats in kv_fp8.h): softmax(q k^T * scale
+// [+ causal mask]) v with k and v = element * scale of the token, in T = bf16, f16 or fp32.
+//
+// The elements (4 bits of significand) are exact in bf16 and f16, so both products run on the 16-bit
+// MFMA with fp32 sums and lose nothing to the cache's format:
+//   S^T = K Q^T    elements as bf16 (T bf16 and fp32, whose q is the exact sum of three bf16 terms)
+//                  or f16 (T f16); the token's key scale multiplies the score in fp32.
+//   O^T += V^T P^T elements as f16, P as f16: one term (11 bits) where the output is bf16 (8 bits),
+//                  two terms (22 bits) else. A probability is 2^13 at the running reference, at most
+//                  2^15, so that f16's normal range covers 2^-27 of the largest; it carries the token's
+//                  value scale relative to the largest seen, which the running output is kept in.
+// A token's scales stand one to a lane and reach the 16 lanes of a row as DPP operands of the
+// multiplications. A token whose row was not finite (scale 255) makes the score NaN, so rows that
+// see it are NaN and rows that do not see it are untouched.
+#include "kv_fp8.h"
+#include "skinny.h"
+
+using namespace dk;
+
+namespace {
+
+constexpr int kTileK = 64;
+// log2 of a probability at the running reference, and what the reference lags behind at most
+constexpr float kLift = 13.f, kSlack = 2.f;
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// T's part in the products: the type that K's elements and q's terms take, q's and P's terms
+template <class T>
+struct Kv8Type;
+template <>
+struct Kv8Type<bf16> {
+  static constexpr int kQ = 1, kP = 1;
+};
+template <>
+struct Kv8Type<f16> {
+  static constexpr int kQ = 1, kP = 2;
+};
+template <>
+struct Kv8Type<float> {
+  static constexpr int kQ = 3, kP = 2;
+};
+
+// 8 codes -> the 16-bit values that they stand for, exactly
+__device__ __forceinline__ U128 codesToF16(uint32_t w0, uint32_t w1) {
+  return U128{
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.f, true)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.f, true))};
+}
+__device__ __forceinline__ U128 codesToBf16(uint32_t w0, uint32_t w1) {
+  return U128{
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, 1.f, true)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, 1.f, true))};
+}
+
+template <class T>
+__device__ __forceinline__ U128 keyFragment(uint32_t w0, uint32_t w1) {
+  if constexpr (__is_same(T, f16))
+    return codesToF16(w0, w1);
+  else
+    return codesToBf16(w0, w1);
+}
+
+template <class T>
+__device__ __forceinline__ f32x4 keyMma(const U128& a, const U128& b, const f32x4& c) {
+  if constexpr (__is_same(T, f16))
+    return F16::mma(a, b, c);
+  else
+    return Bf16::mma(a, b, c);
+}
+
+// 8 elements of q as terms: q itself, or three bf16 numbers (8 bits each, cut off) that add up to it
+template <class T>
+__device__ __forceinline__ void queryFragment(const T* q, U128 (&f)[Kv8Type<T>::kQ]) {
+  if constexpr (sizeof(T) == 2) {
+    f[0] = gload16(q);
+  } else {
+    const U128 lo = gload16(q), hi = gload16(q + 4);
+    uint32_t x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[u][j] = (x[2 * j] >> 16) | (x[2 * j + 1] & 0xFFFF0000u);
+#pragma unroll
+        for (int i = 2 * j; i < 2 * j + 2; ++i)
+          x[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xFFFF0000u));
+      }
+  }
+}
+
+// The value of lane 16 g + n in the lanes 16 g .. 16 g + 15; n is a constant once loops are unrolled,
+// and the move becomes an operand of the multiplication it feeds.
+template <int n>
+__device__ __forceinline__ float rowLane(float v) {
+  return __uint_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x150 + n, 0xF, 0xF, true));
+}
+
+// s[kk][i] *= the factor of key 16 g + 4 kk + i of the lane's row of lanes
+template <int n = 0>
+__device__ __forceinline__ void timesKeys(f32x4 (&s)[4], float factor) {
+  if constexpr (n < 16) {
+    s[n / 4][n % 4] *= rowLane<n>(factor);
+    timesKeys<n + 1>(s, factor);
+  }
+}
+
+// The score factor and value scale of the lane's key. nan: neither finite
+struct KeyScales {
+  float k;      // 2^(key scale) * softmax scale * log2(e); NaN where a scale is 255
+  uint32_t v;   // value scale code, 0 where a scale is 255 or the key is not live
+};
+__device__ __forceinline__ KeyScales keyScales(uint32_t kc, uint32_t vc, bool live,
+                                               float scale_log2) {
+  const bool bad = kc == 255u || vc == 255u;
+  return {mxScaleValue(bad ? 255u : kc) * scale_log2, bad || !live ? 0u : vc};
+}
+
+// 2^(code - top) for code <= top
+__device__ __forceinline__ float valueFactor(uint32_t code, uint32_t top) {
+  const int e = 127 + static_cast<int>(code) - static_cast<int>(top);
+  return e > 0 ? __uint_as_float(static_cast<uint32_t>(e) << 23) : 0.f;
+}
+
+__device__ __forceinline__ uint32_t waveMaxU(uint32_t v) {
+#pragma unroll
+  for (int off = kWave / 2; off > 0; off >>= 1) {
+    const uint32_t o = __shfl_xor(v, off, kWave);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// Bytes i < 16 of w whose bit i is clear become 0.
+__device__ __forceinline__ void keepBytes(U128& w, uint32_t bits) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t b = bits >> (4 * j);
+    w[j] &= ((b & 1u) ? 0xFFu : 0u) | ((b & 2u) ? 0xFF00u : 0u) | ((b & 4u) ? 0xFF0000u : 0u) |
+            ((b & 8u) ? 0xFF000000u : 0u);
+  }
+}
+
+// Probabilities of 16 keys -> two B fragments of f16 (keys 0..7 and 8..15), kP terms
+template <int kP>
+__device__ __forceinline__ void packWeights(const f32x4 (&w)[4], U128 (&f)[kP][2]) {
+#pragma unroll
+  for (int st = 0; st < 2; ++st)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = w[2 * st + j / 2][2 * (j % 2)], b = w[2 * st + j / 2][2 * (j % 2) + 1];
+      const f16x2 hi = {static_cast<f16>(a), static_cast<f16>(b)};
+      f[0][st][j] = __builtin_bit_cast(uint32_t, hi);
+      if constexpr (kP == 2) {
+        const f16x2 lo = {static_cast<f16>(a - static_cast<float>(hi[0])),
+                          static_cast<f16>(b - static_cast<float>(hi[1]))};
+        f[1][st][j] = __builtin_bit_cast(uint32_t, lo);
+      }
+    }
+}
+
+// keys that row i of the queries sees, in [0, capacity]
+__device__ __forceinline__ int visibleKeys(const Kv8AttentionArgs& a, int64_t past, int i) {
+  const int64_t n = past + (a.causal ? i + 1 : a.seq_q);
+  return static_cast<int>(n < 0 ? 0 : (n > a.capacity ? a.capacity : n));
+}
+
+// Row p of a (sequence, KV head) pair: query p / group of head p % group.
+struct RowAt {
+  int i, h;
+};
+__device__ __forceinline__ RowAt rowAt(int p, int group, int kvh) {
+  const int i = p / group;
+  return {i, kvh * group + p - i * group};
+}
+
+// element 0 of a row in q, [batch, q_heads, seq_q, D], and in out
+__device__ __forceinline__ int64_t queryAt(const Kv8AttentionArgs& a, int64_t b, RowAt r, int D) {
+  return ((b * a.q_heads + r.h) * a.seq_q + r.i) * D;
+}
+__device__ __forceinline__ int64_t outAt(const Kv8AttentionArgs& a, int64_t b, RowAt r, int D) {
+  return a.out_bshd ? ((b * a.seq_q + r.i) * a.q_heads + r.h) * D : queryAt(a, b, r, D);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Few rows (at most 16 of a (sequence, KV head) pair: the group's heads of one new token, or of a
+// few): each key is used once, so the keys stream from memory into registers. A workgroup of
+// kDecWaves waves takes split blockIdx.x of pair blockIdx.y; its waves take 64-key tiles in turn, the
+// next one's loads in flight while one is computed, and join their results in LDS. A lane (r, g) of a
+// wave loads 16-byte runs: of K the row of key 16 (r / 4) + 4 kk + r % 4 at the dims 16 g + 64 j, of
+// V the dims 16 dt + r at the keys 16 g. The order in which the MFMA takes dims and keys is free as
+// long as both operands share it, so those runs are its fragments as they come, and the scores come
+// out as 16 consecutive keys a lane: V's order.
+// ---------------------------------------------------------------------------------------------
+constexpr int kDecWaves = 8;
+
+// A tile's codes and this lane's key's scales; ids of its pages, -1 where a page holds nothing
+template <int D>
+struct KeyTile {
+  U128 k[4][D / 64];
+  U128 v[D / 16];
+  uint32_t kc, vc;
+  bool live;  // the lane's key is in a page
+};
+
+template <class T, int D>
+struct DecodeLds {
+  float m[kDecWaves][16];
+  float l[kDecWaves][16];
+  uint32_t top[kDecWaves];
+  float o[kDecWaves][D][17];
+};
+
+// kSmall: pages of 16 or 32 tokens (else a multiple of 64)
+template <class T, int D, bool kSmall>
+__device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
+  using Ty = Kv8Type<T>;
+  constexpr int J = D / 64, DT = D / 16;
+  __shared__ DecodeLds<T, D> lds;
+  const Kv8Pages& pg = a.pages;
+  const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int r = lane % 16, g = lane / 16;
+  const int pair = blockIdx.y, b = pair / pg.heads, kvh = pair - b * pg.heads;
+  const int group = a.q_heads / pg.heads, rows = group * a.seq_q;
+  const int bs = pg.block_size;
+  const int stride = a.splits * kDecWaves, first = blockIdx.x * kDecWaves + wave;
+  const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
+  const int64_t past = kv8First(pg, b);
+  const int most = visibleKeys(a, past, a.seq_q - 1);
+  const int tiles = (most + kTileK - 1) / kTileK;
+
+  // Page ids, a lane each: of kIds tiles of this wave (kSmall: 4 runs of 16 keys a tile).
+  constexpr int kIds = kSmall ? 16 : 64;
+  int ids = -1;
+  auto loadIds = [&](int ordinal) {  // of the tiles ordinal .. ordinal + kIds - 1
+    const int tile = first + (ordinal + (kSmall ? lane / 4 : lane)) * stride;
+    ids = -1;
+    if (tile < tiles) {
+      const int64_t key = static_cast<int64_t>(tile) * kTileK + (kSmall ? 16 * (lane % 4) : 0);
+      if (key < a.capacity) ids = gp(table)[key / bs];
+    }
+    if (ids >= pg.num_blocks) ids = -1;
+  };
+  KeyTile<D> buf[2];
+  auto fetch = [&](KeyTile<D>& x, int tile, int ordinal) {
+    const int64_t head = static_cast<int64_t>(bs) * D;
+    int id_k, id_v, slot_k, slot_v;
+    if constexpr (kSmall) {
+      const int at = (ordinal % kIds) * 4;
+      id_k = __shfl(ids, at + r / 4, kWave);
+      id_v = __shfl(ids, at + g, kWave);
+      slot_k = 16 * (r / 4) % bs;
+      slot_v = 16 * g % bs;
+    } else {
+      id_k = id_v = __builtin_amdgcn_readlane(ids, ordinal % kIds);
+      const int in_page = static_cast<int>(static_cast<uint32_t>(tile) * kTileK % static_cast<uint32_t>(bs));
+      slot_k = in_page + 16 * (r / 4);
+      slot_v = in_page + 16 * g;
+    }
+    x.live = id_v >= 0;
+    // a page that holds nothing: page 0 is read in its place and masked
+    const int64_t hk = static_cast<int64_t>(id_k < 0 ? 0 : id_k) * pg.heads + kvh;
+    const int64_t hv = static_cast<int64_t>(id_v < 0 ? 0 : id_v) * pg.heads + kvh;
+    const uint8_t* kb = pg.key + hk * head + static_cast<int64_t>(slot_k + r % 4) * D + 16 * g;
+    const uint8_t* vb = pg.value + hv * head + static_cast<int64_t>(r) * bs + slot_v;
+    const uint8_t* sb = pg.scales + hv * 2 * bs + slot_v + r;
+    x.kc = gp(sb)[0];
+    x.vc = gp(sb)[bs];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int j = 0; j < J; ++j) x.k[kk][j] = gload16(kb + 4 * kk * D + 64 * j);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) x.v[dt] = gload16(vb + static_cast<int64_t>(16 * dt) * bs);
+  };
+
+  if (first < tiles) loadIds(0);
+  // q: rows past the last are zero and not stored
+  U128 qf[J][2][Ty::kQ];
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int u = 0; u < Ty::kQ; ++u) qf[j][half][u] = zero16();
+  int lim = most;  // keys of this lane's row
+  if (r < rows) {
+    const RowAt at = rowAt(r, group, kvh);
+    lim = visibleKeys(a, past, at.i);
+    const T* q = static_cast<const T*>(a.q) + queryAt(a, b, at, D) + 16 * g;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) queryFragment<T>(q + 64 * j + 8 * half, qf[j][half]);
+  }
+  const int all_see = visibleKeys(a, past, 0);  // keys that every row sees
+
+  float m = -INFINITY, l = 0.f;
+  uint32_t top = 0;
+  f32x4 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto attend = [&](KeyTile<D>& x, int tile) {
+    const int k0 = tile * kTileK;
+    f32x4 s[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      s[kk] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const U128 ka = keyFragment<T>(x.k[kk][j][2 * half], x.k[kk][j][2 * half + 1]);
+#pragma unroll
+          for (int u = Ty::kQ - 1; u >= 0; --u) s[kk] = keyMma<T>(ka, qf[j][half][u], s[kk]);
+        }
+    }
+    const bool live = x.live && k0 + lane < most;
+    const uint64_t lives = __builtin_amdgcn_ballot_w64(live);
+    const KeyScales sc = keyScales(x.kc, x.vc, live, a.scale_log2);
+    timesKeys(s, sc.k);
+    if (lives != ~uint64_t{0} || k0 + kTileK > all_see) {  // uniform
+      const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu;
+      const int key0 = k0 + 16 * g;
+#pragma unroll
+      for (int n = 0; n < 16; ++n)
+        if (!(mine >> n & 1u) || key0 + n >= lim) s[n / 4][n % 4] = -INFINITY;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) keepBytes(x.v[dt], mine);
+    }
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) tmax = fmaxf(tmax, s[n / 4][n % 4]);
+    tmax = rowsMax(tmax);
+    const bool grow = tmax > m + kSlack;  // false while tmax is -inf
+    if (__builtin_amdgcn_ballot_w64(grow)) {
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m - tmax) : 1.f;  // 0 from -inf
+      m = grow ? tmax : m;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+    }
+    if (__builtin_amdgcn_ballot_w64(sc.v > top)) {
+      const uint32_t next = waveMaxU(sc.v);  // > top
+      const float down = valueFactor(top, next);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= down;
+      top = next;
+    }
+    const float base = (m == -INFINITY ? 0.f : m) - kLift;
+    float sum = 0.f;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      s[n / 4][n % 4] = __builtin_amdgcn_exp2f(s[n / 4][n % 4] - base);
+      sum += s[n / 4][n % 4];
+    }
+    l += sum;
+    timesKeys(s, valueFactor(sc.v, top));
+    U128 pf[Ty::kP][2];
+    packWeights<Ty::kP>(s, pf);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const U128 va = codesToF16(x.v[dt][2 * st], x.v[dt][2 * st + 1]);
+#pragma unroll
+        for (int u = Ty::kP - 1; u >= 0; --u) o[dt] = F16::mma(va, pf[u][st], o[dt]);
+      }
+  };
+
+  if (first < tiles) fetch(buf[0], first, 0);
+  for (int tile = first, n = 0; tile < tiles; tile += 2 * stride, n += 2) {
+    const int second = tile + stride, third = second + stride;
+    if (second < tiles) fetch(buf[1], second, n + 1);
+    attend(buf[0], tile);
+    if (second >= tiles) break;
+    if (third < tiles) {
+      if ((n + 2) % kIds == 0) loadIds(n + 2);
+      fetch(buf[0], third, n + 2);
+    }
+    attend(buf[1], second);
+  }
+
+  // join the waves: the row's largest reference and value scale
+  const float l_row = rowsSum(l);
+  if (g == 0) {
+    lds.m[wave][r] = m;
+    lds.l[wave][r] = l_row;
+  }
+  if (lane == 0) lds.top[wave] = top;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds.o[wave][16 * dt + 4 * g + i][r] = o[dt][i];
+  __syncthreads();
+  for (int e = t; e < rows * D; e += kDecWaves * kWave) {
+    const int p = e / D, d = e % D;
+    float M = -INFINITY;
+    uint32_t high = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) {
+      M = fmaxf(M, lds.m[w][p]);
+      high = lds.top[w] > high ? lds.top[w] : high;
+    }
+    float L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) {
+      const float f = lds.m[w][p] == -INFINITY ? (lds.l[w][p] == 0.f ? 0.f : 1.f)
+                                               : __builtin_amdgcn_exp2f(lds.m[w][p] - M);
+      L += f * lds.l[w][p];
+      acc += f * valueFactor(lds.top[w], high) * lds.o[w][d][p];
+    }
+    const RowAt at = rowAt(p, group, kvh);
+    // 2^(high - 127) * acc / L; the quotient first, so that neither overflows
+    const float result =
+        L == 0.f ? 0.f : __builtin_ldexpf(acc / L, static_cast<int>(high) - 127);
+    if (a.splits == 1) {
+      st(static_cast<T*>(a.out) + outAt(a, b, at, D) + d, result);
+    } else {
+      const int64_t part = (queryAt(a, b, at, 1) * a.splits + blockIdx.x);
+      if (d == 0) {
+        a.part_ml[part * 2] = M;
+        a.part_ml[part * 2 + 1] = L;
+      }
+      a.part_o[part * D + d] = result;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows (a chunk of new tokens, a prompt): the group's heads and the queries are one row index,
+// so a staged tile serves every head of the group. A workgroup of 4 waves owns 64 QB rows of a pair
+// (16 QB a wave) and a range of 64-key tiles; grid.z splits the keys where rows alone leave CUs idle.
+// A tile's codes are converted once, on their way into LDS: K [key][dim], keys in the order in which
+// the scores come out as 16 consecutive keys a lane, and V^T [dim][key] as it lies in the page, its 16-byte
+// chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks.
+// ---------------------------------------------------------------------------------------------
+constexpr int kChunkThreads = 256;
+
+__device__ __forceinline__ int valueChunk(int d, int chunk) {
+  return d * kTileK + (chunk ^ ((d >> 1) & 7)) * 8;
+}
+
+template <class T, int D, int QB, bool kSmall>
+__device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
+  using Ty = Kv8Type<T>;
+  constexpr int kPitch = D + 8;  // 16 rows start on 16 distinct groups of 4 banks
+  constexpr int DT = D / 16, DK = D / 32, kPer = D / 64;
+  constexpr int kParts = D / 16;  // 16-code chunks of a key
+  __shared__ __attribute__((aligned(16))) uint16_t Ks[kTileK * kPitch];
+  __shared__ __attribute__((aligned(16))) uint16_t Vt[D * kTileK];
+  const Kv8Pages& pg = a.pages;
+  const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int r = lane % 16, g = lane / 16;
+  const int group = a.q_heads / pg.heads, rows = a.seq_q * group, bs = pg.block_size;
+  // the pair is the fast index (consecutive workgroups go to different XCDs), the row tile the slow
+  // one, last tile first: under a causal mask the longest workgroups start first
+  const uint32_t lin = blockIdx.x + gridDim.x * blockIdx.y;
+  const int pair = static_cast<int>(lin % gridDim.y), b = pair / pg.heads, kvh = pair - b * pg.heads;
+  const int p0 = static_cast<int>(gridDim.x - 1 - lin / gridDim.y) * 64 * QB;
+  const int pw = p0 + wave * 16 * QB;  // the wave's first row
+  const bool active = pw < rows;       // uniform over the wave
+  const int64_t past = kv8First(pg, b);
+  auto clamped = [&](int p) { return p < rows ? p : rows - 1; };
+
+  U128 qf[QB][DK][Ty::kQ];
+  int lim[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const RowAt at = rowAt(clamped(pw + qb * 16 + r), group, kvh);  // clamped: not stored
+    const T* q = static_cast<const T*>(a.q) + queryAt(a, b, at, D) + g * 8;
+#pragma unroll
+    for (int c = 0; c < DK; ++c) queryFragment<T>(q + c * 32, qf[qb][c]);
+    lim[qb] = visibleKeys(a, past, at.i);
+  }
+  const int wg_keys = visibleKeys(a, past, clamped(p0 + 64 * QB - 1) / group);
+  const int wave_full = visibleKeys(a, past, clamped(pw) / group);  // keys every row of the wave sees
+
+  const int all_tiles = (wg_keys + kTileK - 1) / kTileK;
+  const int per = (all_tiles + a.splits - 1) / a.splits;
+  const int kt0 = static_cast<int>(blockIdx.z) * per;
+  const int kt1 = kt0 + per < all_tiles ? kt0 + per : all_tiles;
+
+  // page ids of the next tile's four runs of 16 keys (one page where pages are not small)
+  const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
+  int id[4];
+  auto loadIds = [&](int kt) {
+#pragma unroll
+    for (int u = 0; u < (kSmall ? 4 : 1); ++u) {
+      const int64_t key = static_cast<int64_t>(kt) * kTileK + 16 * u;
+      int x = -1;
+      if (kt < kt1 && key < a.capacity) x = gp(table)[static_cast<uint32_t>(key) / static_cast<uint32_t>(bs)];
+      id[u] = x < pg.num_blocks ? x : -1;
+    }
+    if (!kSmall) id[1] = id[2] = id[3] = id[0];
+  };
+  auto pick = [&](int u) { return u == 0 ? id[0] : u == 1 ? id[1] : u == 2 ? id[2] : id[3]; };
+  auto headOf = [&](int page) {  // a page that holds nothing: page 0 is read in its place and masked
+    return static_cast<int64_t>(page < 0 ? 0 : page) * pg.heads + kvh;
+  };
+  U128 kr[kPer], vr[kPer];
+  uint32_t kc = 0, vc = 0;
+  bool in_page = false;
+  auto fetch = [&](int kt) {
+    const int slot0 = kSmall ? 0 : static_cast<int>(static_cast<uint32_t>(kt) * kTileK % static_cast<uint32_t>(bs));
+    const int64_t head = static_cast<int64_t>(bs) * D;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = t + i * kChunkThreads;
+      const int key = c / kParts, part = c % kParts;
+      const int ks = kSmall ? key % bs : slot0 + key;
+      kr[i] = gload16(pg.key + headOf(pick(key / 16)) * head + static_cast<int64_t>(ks) * D + part * 16);
+      const int d = c / 4, run = c % 4;
+      const int vs = kSmall ? 16 * run % bs : slot0 + 16 * run;
+      vr[i] = gload16(pg.value + headOf(pick(run)) * head + static_cast<int64_t>(d) * bs + vs);
+    }
+    const int page = pick(g);
+    in_page = page >= 0;
+    const uint8_t* sb = pg.scales + headOf(page) * 2 * bs + (kSmall ? lane % bs : slot0 + lane);
+    kc = gp(sb)[0];
+    vc = gp(sb)[bs];
+  };
+  auto stash = [&](uint64_t lives) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = t + i * kChunkThreads;
+      const int key = c / kParts, part = c % kParts;
+      // the score of row 4 g + i of the 16-key group kk is that of key 16 g + 4 kk + i
+      const int row = 16 * (key % 16 / 4) + 4 * (key / 16) + key % 4;
+      U128* ko = reinterpret_cast<U128*>(&Ks[row * kPitch + part * 16]);
+      ko[0] = keyFragment<T>(kr[i][0], kr[i][1]);
+      ko[1] = keyFragment<T>(kr[i][2], kr[i][3]);
+      const int d = c / 4, run = c % 4;
+      if (lives != ~uint64_t{0}) keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
+      *reinterpret_cast<U128*>(&Vt[valueChunk(d, 2 * run)]) = codesToF16(vr[i][0], vr[i][1]);
+      *reinterpret_cast<U128*>(&Vt[valueChunk(d, 2 * run + 1)]) = codesToF16(vr[i][2], vr[i][3]);
+    }
+  };
+
+  f32x4 o[QB][DT];
+  float m[QB], l[QB];
+  uint32_t top = 0;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    m[qb] = -INFINITY;
+    l[qb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (kt0 < kt1) {
+    loadIds(kt0);
+    fetch(kt0);
+    loadIds(kt0 + 1);
+  }
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int k0 = kt * kTileK;
+    const uint64_t lives = __builtin_amdgcn_ballot_w64(in_page && k0 + lane < wg_keys);
+    const KeyScales sc = keyScales(kc, vc, in_page && k0 + lane < wg_keys, a.scale_log2);
+    __syncthreads();  // the previous tile is no longer read
+    stash(lives);
+    __syncthreads();
+    if (kt + 1 < kt1) {
+      fetch(kt + 1);
+      loadIds(kt + 2);
+    }
+    if (!active) continue;
+    if (__builtin_amdgcn_ballot_w64(sc.v > top)) {
+      const uint32_t next = waveMaxU(sc.v);
+      const float down = valueFactor(top, next);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= down;
+      top = next;
+    }
+    const float vf = valueFactor(sc.v, top);
+
+    f32x4 s[QB][4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) s[qb][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < DK; ++c) {
+        const U128 ka = load16(&Ks[(kk * 16 + r) * kPitch + c * 32 + g * 8]);
+#pragma unroll
+        for (int u = Ty::kQ - 1; u >= 0; --u)
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) s[qb][kk] = keyMma<T>(ka, qf[qb][c][u], s[qb][kk]);
+      }
+    }
+    const bool full = lives == ~uint64_t{0} && k0 + kTileK <= wave_full;
+    U128 pf[QB][Ty::kP][2];
+#pragma unroll
+    for (int qb = 0; qb < QB; ++qb) {
+      timesKeys(s[qb], sc.k);
+      if (!full) {
+        const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu;
+        const int key0 = k0 + 16 * g;
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          if (!(mine >> n & 1u) || key0 + n >= lim[qb]) s[qb][n / 4][n % 4] = -INFINITY;
+      }
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) tmax = fmaxf(tmax, s[qb][n / 4][n % 4]);
+      tmax = rowsMax(tmax);
+      const bool grow = tmax > m[qb] + kSlack;
+      if (__builtin_amdgcn_ballot_w64(grow)) {
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m[qb] - tmax) : 1.f;
+        m[qb] = grow ? tmax : m[qb];
+        l[qb] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+      }
+      const float base = (m[qb] == -INFINITY ? 0.f : m[qb]) - kLift;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        s[qb][n / 4][n % 4] = __builtin_amdgcn_exp2f(s[qb][n / 4][n % 4] - base);
+        sum += s[qb][n / 4][n % 4];
+      }
+      l[qb] += sum;
+      timesKeys(s[qb], vf);
+      packWeights<Ty::kP>(s[qb], pf[qb]);
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const U128 va = load16(&Vt[valueChunk(16 * dt + r, 2 * g + st)]);
+#pragma unroll
+        for (int u = Ty::kP - 1; u >= 0; --u)
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) o[qb][dt] = F16::mma(va, pf[qb][u][st], o[qb][dt]);
+      }
+  }
+
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const float L = rowsSum(l[qb]);
+    const int p = pw + qb * 16 + r;
+    if (p >= rows) continue;
+    const RowAt at = rowAt(p, group, kvh);
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // no key, or none of any weight: zeros
+    const int e = static_cast<int>(top) - 127;
+    if (a.splits == 1) {
+      T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st(out + 16 * dt + i, __builtin_ldexpf(o[qb][dt][i] * inv, e));
+    } else {
+      const int64_t part = queryAt(a, b, at, 1) * a.splits + blockIdx.z;
+      if (g == 0) {
+        a.part_ml[part * 2] = m[qb];
+        a.part_ml[part * 2 + 1] = L;
+      }
+      float* out = a.part_o + part * D + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[16 * dt + i] = __builtin_ldexpf(o[qb][dt][i] * inv, e);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Rows of any number: the splits' results of row blockIdx.x * 4 + wave joined.
+// ---------------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a, int D) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.seq_q;
+  if (row >= rows) return;
+  const int i = static_cast<int>(row % a.seq_q);
+  const int64_t bh = row / a.seq_q, b = bh / a.q_heads;
+  float M = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, gp(a.part_ml)[(row * a.splits + s) * 2]);
+  float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t part = row * a.splits + s;
+    const float m = gp(a.part_ml)[part * 2], l = gp(a.part_ml)[part * 2 + 1];
+    const float f = (m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M)) * l;
+    L += f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (lane + u * kWave < D) acc[u] = fmaf(f, gp(a.part_o)[part * D + lane + u * kWave], acc[u]);
+  }
+  const RowAt at = {i, static_cast<int>(bh % a.q_heads)};
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + u * kWave < D)
+      st(static_cast<T*>(a.out) + outAt(a, b, at, D) + lane + u * kWave, L == 0.f ? 0.f : acc[u] / L);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Any head_dim up to 256, page size, scale and alignment: one wave per row, 64 keys a round.
+// ---------------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
+  __shared__ float q_lds[256];
+  __shared__ float p_lds[kWave];
+  __shared__ int64_t at_lds[kWave];
+  const Kv8Pages& pg = a.pages;
+  const int lane = threadIdx.x, D = pg.head_dim;
+  const int64_t row = blockIdx.x;
+  const int i = static_cast<int>(row % a.seq_q);
+  const int64_t bh = row / a.seq_q, b = bh / a.q_heads;
+  const int h = static_cast<int>(bh % a.q_heads), kvh = h / (a.q_heads / pg.heads);
+  const int lim = visibleKeys(a, kv8First(pg, b), i);
+  for (int d = lane; d < D; d += kWave) q_lds[d] = ld(static_cast<const T*>(a.q) + row * D + d);
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0; j0 < lim; j0 += kWave) {
+    const int j = j0 + lane;
+    float s = -INFINITY, vs = 0.f;
+    int64_t at = -1;
+    if (j < lim) {
+      const int64_t page = kv8Page(pg, b, j);
+      if (page >= 0) {
+        const int slot = j % pg.block_size;
+        const int64_t head = page * pg.heads + kvh;
+        const uint32_t kc = pg.scales[head * 2 * pg.block_size + slot];
+        const uint32_t vc = pg.scales[(head * 2 + 1) * pg.block_size + slot];
+        const uint8_t* k = pg.key + (head * pg.block_size + slot) * D;
+        float dot = 0.f;
+        for (int d = 0; d < D; ++d)
+          dot = fmaf(q_lds[d], __builtin_amdgcn_cvt_f32_fp8(k[d], 0), dot);
+        s = dot * (mxScaleValue(kc == 255u || vc == 255u ? 255u : kc) * a.scale_log2);
+        vs = vc == 255u ? 0.f : mxScaleValue(vc);
+        at = head * D * pg.block_size + slot;
+      }
+    }
+    const float next = fmaxf(m, waveMax(s));
+    const float base = next == -INFINITY ? 0.f : next;
+    const float p = at >= 0 ? __builtin_amdgcn_exp2f(s - base) : 0.f;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);  // 0 on the first round
+    l = l * alpha + waveSum(p);
+    m = next;
+    p_lds[lane] = p * vs;
+    at_lds[lane] = at;
+    __syncthreads();
+    const int n = lim - j0 < kWave ? lim - j0 : kWave;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = lane + u * kWave;
+      if (d >= D) break;
+      float x = acc[u] * alpha;
+      for (int jj = 0; jj < n; ++jj)
+        if (at_lds[jj] >= 0)
+          x = fmaf(p_lds[jj], __builtin_amdgcn_cvt_f32_fp8(
+                                  pg.value[at_lds[jj] + static_cast<int64_t>(d) * pg.block_size], 0), x);
+      acc[u] = x;
+    }
+    __syncthreads();
+  }
+  T* out = static_cast<T*>(a.out) + outAt(a, b, {i, h}, D);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    if (lane + u * kWave < D) st(out + lane + u * kWave, l == 0.f ? 0.f : acc[u] / l);
+}
+
+}  // namespace
+
+#define KV8_CHUNK(suffix, T, D, QB)                                                             \
+  extern "C" __global__ void __launch_bounds__(kChunkThreads)                                   \
+      kv8_chunk_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                                   \
+    kv8_chunk<T, D, QB, false>(a);                                                              \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(kChunkThreads)                                   \
+      kv8_chunk_small_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                             \
+    kv8_chunk<T, D, QB, true>(a);                                                               \
+  }
+
+#define KV8_ATTENTION(suffix, T)                                                                \
+  extern "C" __global__ void __launch_bounds__(kDecWaves * kWave)                               \
+      kv8_decode_d64_##suffix(Kv8AttentionArgs a) {                                             \
+    kv8_decode<T, 64, false>(a);                                                                \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(kDecWaves * kWave)                               \
+      kv8_decode_d128_##suffix(Kv8AttentionArgs a) {                                            \
+    kv8_decode<T, 128, false>(a);                                                               \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(kDecWaves * kWave)                               \
+      kv8_decode_small_d64_##suffix(Kv8AttentionArgs a) {                                       \
+    kv8_decode<T, 64, true>(a);                                                                 \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(kDecWaves * kWave)                               \
+      kv8_decode_small_d128_##suffix(Kv8AttentionArgs a) {                                      \
+    kv8_decode<T, 128, true>(a);                                                                \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(256) kv8_merge_##suffix(Kv8AttentionArgs a) {    \
+    kv8_merge<T>(a, a.pages.head_dim);                                                          \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(64) kv8_rows_##suffix(Kv8AttentionArgs a) {      \
+    kv8_rows<T>(a);                                                                             \
+  }                                                                                             \
+  KV8_CHUNK(suffix, T, 64, 1)                                                                   \
+  KV8_CHUNK(suffix, T, 64, 2)                                                                   \
+  KV8_CHUNK(suffix, T, 128, 1)                                                                  \
+  KV8_CHUNK(suffix, T, 128, 2)
+
+KV8_ATTENTION(f32, float)
+KV8_ATTENTION(bf16, bf16)
+KV8_ATTENTION(f16, f16)

@@ -126,6 +126,14 @@ _SIGNATURES = {
     "dli_hip_mx_linear_workspace": [_int, _i64, _i64, _i64],
     "dli_hip_mx_linear": [_int, _int] + [_c_void_p] * 7 + [_i64] * 3 + [_c_void_p, _size,
                                                                         _c_void_p],
+    "dli_hip_kv_append_fp8": [_int] + [_c_void_p] * 6 + [_i64] * 8 + [_c_void_p, _int, _c_void_p],
+    "dli_hip_rope_append_fp8": [_int] + [_c_void_p] * 3 + [_i64] * 2 + [_c_void_p] * 5 + [_i64] * 9
+    + [_c_void_p, _int, _c_void_p],
+    "dli_hip_kv_read_fp8": [_int] + [_c_void_p] * 4 + [_i64] + [_c_void_p] * 2 + [_i64] * 7
+    + [_c_void_p, _int, _c_void_p],
+    "dli_hip_paged_attention_fp8_workspace": [_i64] * 7,
+    "dli_hip_paged_attention_fp8": [_int] + [_c_void_p] * 5 + [_i64, _c_void_p] + [_i64] * 8
+    + [_c_void_p, _int, _int, _float, _int, _c_void_p, _size, _c_void_p],
     "dli_hip_stream_is_capturing": [_c_void_p, ctypes.POINTER(_int)],
 }
 _RESTYPES = {
@@ -137,6 +145,7 @@ _RESTYPES = {
     "dli_hip_mx_linear_workspace": _size,
     "dli_hip_paged_attention_workspace": _size,
     "dli_hip_chunk_attention_workspace": _size,
+    "dli_hip_paged_attention_fp8_workspace": _size,
     "dli_hip_splitk_workspace": _size,
     "dli_hip_linear_residual_rows_workspace": _size,
     "dli_hip_qkv_rope_append_workspace": _size,

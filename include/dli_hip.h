@@ -95,8 +95,8 @@ int dli_hip_set_device(int device);
  * any grid dimension 0 returns 0 without touching the runtime (cuda_driver.cc:123). */
 int dli_hip_module_load(const void* image, size_t image_bytes, void** module);
 /* Image of the library's embedded gfx950 code object `name` ("attention", "conv", "decode",
- * "elementwise", "flash_attention", "gemm", "mfma_gemm", "mx_linear", "mx_quantize", "norm",
- * "stack"), for dli_hip_module_load. The reference's counterpart is the cubin file its plugin reads
+ * "elementwise", "flash_attention", "gemm", "kv_fp8", "kv_fp8_attention", "mfma_gemm", "mx_linear",
+ * "mx_quantize", "norm", "stack"), for dli_hip_module_load. The reference's counterpart is the cubin file its plugin reads
  * next to itself (CudaAotKernel::load, cuda_driver.cc:107-117); here the images live inside the
  * library.
  * The image stays valid while the library is loaded. */
@@ -587,6 +587,77 @@ int dli_hip_mx_linear(int x_format, int out_dtype, const void* x_codes, const vo
                       const void* w_codes, const void* w_scales, const void* bias,
                       const void* residual, void* out, int64_t m, int64_t n, int64_t k,
                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * 5. The 8-bit paged KV cache. No counterpart in the reference, whose cache holds fp32.
+ *
+ *    The pages of include/dli/kv_cache.h with e4m3 elements and two scales per token and KV head,
+ *    powers of two:
+ *      key_codes    uint8 [num_blocks, heads, block_size, head_dim]
+ *      value_codes  uint8 [num_blocks, heads, head_dim, block_size]
+ *      scales       uint8 [num_blocks, heads, 2, block_size], the keys' and then the values':
+ *                   2^(code - 127); 255: the row held an infinity or a NaN, and stands for NaN
+ *    A row is quantised with the least scale that brings its largest magnitude to at most 448, its
+ *    elements value / scale rounded to nearest even; one with an infinity or a NaN to zeros.
+ *    block_table int32 [batch, max_blocks]: the page of positions [block_size * i, + block_size) of a
+ *    sequence. An id outside [0, num_blocks) is a page that holds nothing: nothing is written to it,
+ *    it reads as zeros, and attention passes over its tokens. Pages may be shared for reading; two
+ *    sequences of one call must not write the same slot.
+ *    dtype (fp32, bf16, f16) is that of the values outside the cache. positions (int32 or int64
+ *    [batch], DLI_I32 / DLI_I64) are the sequences' first positions where non-NULL, else all are at
+ *    `start` / `past`. head_dim <= 256; a sequence's pages hold fewer than 2^30 tokens. Fast forms:
+ *    head_dim 64 and 128, 16-byte aligned tensors, block_size a multiple of 16 (attention: 16, 32 or
+ *    a multiple of 64); other calls run row by row.
+ * ------------------------------------------------------------------------------------- */
+
+/* Quantises key, value [batch, heads, seq, head_dim] into the cache: token s of sequence b goes to
+ * position start + s (positions[b] + s). Tokens at positions outside the pages are dropped. */
+int dli_hip_kv_append_fp8(int dtype, const void* key, const void* value, void* key_codes,
+                          void* value_codes, void* scales, const int32_t* block_table,
+                          int64_t num_blocks, int64_t batch, int64_t heads, int64_t seq,
+                          int64_t head_dim, int64_t block_size, int64_t max_blocks, int64_t start,
+                          const void* positions, int positions_dtype, void* stream);
+
+/* dli_hip_rotary on the q and k heads of a joined projection's output and then the append, in one
+ * launch: qkv [batch, seq, (q_heads + 2 kv_heads) * head_dim], rows q | k | v; q_out [batch, q_heads,
+ * seq, head_dim]; cos/sin fp32 [max_pos, pairs]. q_out and the keys before their quantisation are
+ * rounded to dtype, as where the rotation is a call of its own. */
+int dli_hip_rope_append_fp8(int dtype, const void* qkv, const float* cos_table, const float* sin_table,
+                            int64_t max_pos, int64_t pairs, void* q_out, void* key_codes,
+                            void* value_codes, void* scales, const int32_t* block_table,
+                            int64_t num_blocks, int64_t batch, int64_t seq, int64_t q_heads,
+                            int64_t kv_heads, int64_t head_dim, int64_t block_size,
+                            int64_t max_blocks, int64_t start, const void* positions,
+                            int positions_dtype, void* stream);
+
+/* key, value [batch, heads, seq, head_dim] = what the cache holds at positions start .. start + seq - 1
+ * (positions[b] ..), rounded to dtype; zeros at positions outside the pages. */
+int dli_hip_kv_read_fp8(int dtype, const void* key_codes, const void* value_codes, const void* scales,
+                        const int32_t* block_table, int64_t num_blocks, void* key, void* value,
+                        int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
+                        int64_t block_size, int64_t max_blocks, int64_t start, const void* positions,
+                        int positions_dtype, void* stream);
+
+/* Attention of q [batch, q_heads, seq_q, head_dim] over the cache, seq_q >= 1, as
+ * dli_hip_paged_attention: sequence b holds past + seq_q tokens (positions[b] + seq_q), the query at
+ * index i sits at position past + i and, when causal, sees keys at positions <= past + i. A query
+ * that sees no token, or whose every score is -infinity, gets zeros. out is [batch, q_heads, seq_q, head_dim], with out_bshd
+ * [batch, seq_q, q_heads, head_dim]. A row that sees a NaN token is NaN. Elements must be those that
+ * the appends write (not e4m3's own NaN, 0x7F and 0xFF), but for tokens that no query sees.
+ * A workspace of dli_hip_paged_attention_fp8_workspace bytes, 4-byte aligned and of any content, lets
+ * the keys of a row be split over workgroups, their results joined in a fixed order; a smaller one or
+ * NULL means fewer splits. Two calls that may run at once need one each. */
+size_t dli_hip_paged_attention_fp8_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                             int64_t seq_q, int64_t head_dim, int64_t block_size,
+                                             int64_t max_blocks);
+int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
+                                const void* value_codes, const void* scales,
+                                const int32_t* block_table, int64_t num_blocks, void* out,
+                                int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
+                                int64_t head_dim, int64_t block_size, int64_t max_blocks,
+                                int64_t past, const void* positions, int positions_dtype, int causal,
+                                float scale, int out_bshd, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
