@@ -111,10 +111,11 @@ PYBIND11_MODULE(_dli_native, m) {
       .def("operator_names", [](const dli::Engine& e) { return e.registry().names(); })
       .def(
           "configure_kv_cache",
-          [](dli::Engine& e, std::int64_t block_size, std::int64_t max_seq_len) {
-            e.kvCache().configure(block_size, max_seq_len);
+          [](dli::Engine& e, std::int64_t block_size, std::int64_t max_seq_len,
+             const std::string& format) {
+            e.kvCache().configure(block_size, max_seq_len, format);
           },
-          py::arg("block_size") = 64, py::arg("max_seq_len") = 4096)
+          py::arg("block_size") = 64, py::arg("max_seq_len") = 4096, py::arg("format") = "")
       .def("clear_kv_cache", [](dli::Engine& e) { e.kvCache().clear(); })
       .def("kv_cache_size", [](const dli::Engine& e) { return e.kvCache().size(); })
       .def("set_kv_cache_length",
@@ -131,15 +132,34 @@ PYBIND11_MODULE(_dli_native, m) {
             d["block_size"] = entry->block_size;
             d["max_blocks"] = entry->max_blocks;
             d["length"] = entry->length;
+            if (entry->quantized()) d["scales"] = py::cast(entry->scales.torchTensor());
             return d;
           },
           py::arg("name"))
+      .def(
+          "read_kv_cache",
+          [](dli::Engine& e, const std::string& name, std::int64_t start, std::int64_t length,
+             const std::string& dtype, std::uintptr_t stream) {
+            std::pair<dli::Tensor, dli::Tensor> out;
+            {
+              py::gil_scoped_release release;
+              e.setStream(streamFrom(stream));
+              const dli::KVCacheEntry* entry = e.kvCache().get(name);
+              out = e.kvCache().read(name, start, length,
+                                     !dtype.empty()     ? dli::dtypeFromString(dtype)
+                                     : entry != nullptr ? entry->dtype
+                                                        : dli::DType::Float32);
+            }
+            return py::make_tuple(out.first.torchTensor(), out.second.torchTensor());
+          },
+          py::arg("name"), py::arg("start"), py::arg("length"), py::arg("dtype") = "",
+          py::arg("stream") = 0)
       .def(
           "reserve_kv_cache",
           [](dli::Engine& e, const std::string& name, const std::string& dtype, std::int64_t batch,
              std::int64_t heads, std::int64_t head_dim, int device_id) {
             e.kvCache().reserve(name, dli::dtypeFromString(dtype), batch, heads, head_dim,
-                                device_id);
+                                device_id, true);
           },
           py::arg("name"), py::arg("dtype"), py::arg("batch"), py::arg("heads"),
           py::arg("head_dim"), py::arg("device_id") = 0);
@@ -147,15 +167,16 @@ PYBIND11_MODULE(_dli_native, m) {
   py::class_<dli::GreedyDecoder>(m, "GreedyDecoder")
       .def(py::init([](dli::Engine& engine, const dli::Graph& graph, const py::dict& weights,
                        std::int64_t batch, std::int64_t block_size, std::int64_t max_seq_len,
-                       bool capture) {
+                       bool capture, const std::string& kv_format) {
              auto tensors = toTensorMap(weights);
              py::gil_scoped_release release;
              return std::make_unique<dli::GreedyDecoder>(
                  engine, graph, std::move(tensors), batch,
-                 dli::GreedyOptions{block_size, max_seq_len, capture});
+                 dli::GreedyOptions{block_size, max_seq_len, capture, kv_format});
            }),
            py::arg("engine"), py::arg("graph"), py::arg("weights"), py::arg("batch"),
            py::arg("block_size") = 64, py::arg("max_seq_len") = 4096, py::arg("capture") = true,
+           py::arg("kv_format") = "",
            py::keep_alive<1, 2>())
       .def_property_readonly("batch", &dli::GreedyDecoder::batch)
       .def_property_readonly("captured", &dli::GreedyDecoder::captured)

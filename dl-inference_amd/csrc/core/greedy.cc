@@ -157,7 +157,7 @@ GreedyDecoder::GreedyDecoder(Engine& engine, Graph graph, TensorMap weights, std
   s.inputs["input_ids"] = s.ids;
   s.inputs["positions"] = s.positions;
   s.has_status = listed(s.graph.outputs, "status");
-  engine.kvCache().configure(options.block_size, options.max_seq_len);
+  engine.kvCache().configure(options.block_size, options.max_seq_len, options.kv_format);
 }
 
 GreedyDecoder::~GreedyDecoder() = default;

@@ -120,6 +120,33 @@ class CallScratch {
   Tensor buffer_;
 };
 
+// Attention of q [B, Hq, S, D] over a quantised cache entry that holds the queries' own tokens too:
+// those of sequence b start at positions[b], or all at `past` (positions nullptr).
+inline void quantizedAttention(const KVCacheEntry& e, const Tensor& q, const Tensor* positions,
+                               std::int64_t past, bool causal, float scale, bool bshd, Tensor& out,
+                               void* stream, const std::string& op) {
+  int current = 0;
+  check(dli_hip_get_device(&current), op);
+  if (q.deviceId() != current || e.key_pool.deviceId() != current)
+    throw std::invalid_argument(op + " expects its tensors and the cache on the current device");
+  if (e.batch != q.dim(0) || e.head_dim != q.dim(3) || e.dtype != q.dtype())
+    throw std::invalid_argument(op + ": q does not match the cache entry");
+  if (q.dim(1) % e.heads != 0)
+    throw std::invalid_argument(op + ": q heads must be a multiple of the cache entry's heads");
+  // partial results of the key splits
+  CallScratch ws(dli_hip_paged_attention_fp8_workspace(e.batch, q.dim(1), e.heads, q.dim(2), e.head_dim,
+                                                       e.block_size, e.max_blocks),
+                 q.deviceId());
+  check(dli_hip_paged_attention_fp8(
+            hipDtype(q.dtype()), ptr(q), ptr(e.key_pool), ptr(e.value_pool), ptr(e.scales),
+            static_cast<const std::int32_t*>(ptr(e.block_table)), e.key_pool.dim(0), ptr(out), e.batch,
+            q.dim(1), e.heads, q.dim(2), e.head_dim, e.block_size, e.max_blocks, past,
+            positions != nullptr ? ptr(*positions) : nullptr,
+            positions != nullptr ? hipDtype(positions->dtype()) : DLI_I64, causal ? 1 : 0, scale,
+            bshd ? 1 : 0, ws.data(), ws.bytes(), stream),
+        op);
+}
+
 template <typename Op>
 void add(OperatorRegistry* registry) {
   registry->registerFactory(Op().type(), [] { return std::make_unique<Op>(); });

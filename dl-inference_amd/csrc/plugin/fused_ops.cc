@@ -6,6 +6,8 @@
 //                          append
 //   qkv_rope_heads         q/k/v_proj, reshapes, [B,S,H,D] -> [B,H,S,D] transposes and
 //                          rotary_embedding of a prompt (prefill)
+//   rope_append            reshapes, rotary_embedding and KV append of an 8-bit cache, after one
+//                          q|k|v projection
 //   paged_attention        attention over the already appended paged KV cache (decode)
 //   linear_residual        o_proj + attention_residual, down_proj + mlp_residual
 //   linear_residual_norm   the same plus the RMSNorm that follows the residual update
@@ -116,7 +118,55 @@ class QkvRopeHeadsOp final : public Operator {
   }
 };
 
-// Decode attention over a cache entry whose newest token (at positions[b]) is already written.
+// inputs: qkv [B, N] (one token per sequence) or [B, S, N], rows q | k | v of N = (Hq + 2 Hkv) D, cos, sin
+// [max_pos, pairs], positions [B]; attrs q_heads, kv_heads, head_dim, kv_cache. RoPE on q and k of
+// sequence b's tokens at positions[b] + s; k and v quantised into the cache entry; output q
+// [B, Hq, S, D]. Only for caches of the 8-bit format.
+class RopeAppendOp final : public Operator {
+ public:
+  std::string type() const override { return "rope_append"; }
+  void compute(const std::vector<const Tensor*>& in, const std::vector<Tensor*>& out,
+               const Attributes& attrs, ExecutionContext& ctx) const override {
+    requireArity(in, out, 4, 4, 1, type());
+    requireCudaInputs(in, type());
+    const Tensor &x = *in[0], &cos = *in[1], &sin = *in[2], &pos = *in[3];
+    requireFloating(x, type());
+    requireFloat(cos, type());
+    requireFloat(sin, type());
+    requireIndex(pos, type(), "positions");
+    int current = 0;
+    check(dli_hip_get_device(&current), type());
+    for (const Tensor* t : in)
+      if (t->deviceId() != current)
+        throw std::invalid_argument("rope_append expects its tensors on the current device");
+    const auto hq = attrs.require<std::int64_t>("q_heads");
+    const auto hkv = attrs.require<std::int64_t>("kv_heads");
+    const auto d = attrs.require<std::int64_t>("head_dim");
+    const std::string& cache_name = attrs.require<std::string>("kv_cache");
+    if (hq <= 0 || hkv <= 0 || d <= 0 || (x.rank() != 2 && x.rank() != 3) ||
+        x.shape().back() != (hq + 2 * hkv) * d)
+      throw std::invalid_argument("rope_append expects [B, (S,) (q_heads + 2 kv_heads) * head_dim]");
+    const std::int64_t B = x.dim(0), S = x.rank() == 3 ? x.dim(1) : 1;
+    if (cos.rank() != 2 || cos.shape() != sin.shape() || 2 * cos.dim(1) > d)
+      throw std::invalid_argument("rope_append cos/sin must be [max_pos, up to head_dim/2]");
+    if (static_cast<std::int64_t>(pos.numel()) != B)
+      throw std::invalid_argument("rope_append positions must have one entry per sequence");
+    if (ctx.kv_cache == nullptr) throw std::invalid_argument("rope_append missing KV cache");
+    KVCacheEntry& e = ctx.kv_cache->reserve(cache_name, x.dtype(), B, hkv, d, x.deviceId(), true);
+    if (!e.quantized()) throw std::invalid_argument("rope_append needs a KV cache of format fp8");
+    *out[0] = Tensor::cuda(x.dtype(), {B, hq, S, d}, x.deviceId());
+    check(dli_hip_rope_append_fp8(
+              hipDtype(x.dtype()), ptr(x), static_cast<const float*>(ptr(cos)),
+              static_cast<const float*>(ptr(sin)), cos.dim(0), cos.dim(1), ptr(*out[0]),
+              ptr(e.key_pool), ptr(e.value_pool), ptr(e.scales),
+              static_cast<const std::int32_t*>(ptr(e.block_table)), e.key_pool.dim(0), B, S, hq, hkv, d,
+              e.block_size, e.max_blocks, 0, ptr(pos), hipDtype(pos.dtype()), ctx.stream),
+          type());
+  }
+};
+
+// Attention over a cache entry whose newest token (at positions[b]) is already written; over an entry
+// of the 8-bit format also several queries per sequence, the first at positions[b].
 class PagedAttentionOp final : public Operator {
  public:
   std::string type() const override { return "paged_attention"; }
@@ -128,17 +178,27 @@ class PagedAttentionOp final : public Operator {
     const Tensor& pos = *in[1];
     requireFloating(q, type());
     requireIndex(pos, type(), "positions");
-    if (q.rank() != 4 || q.dim(2) != 1) throw std::invalid_argument("paged_attention expects q [B, H, 1, D]");
+    if (q.rank() != 4) throw std::invalid_argument("paged_attention expects q [B, H, S, D]");
     if (ctx.kv_cache == nullptr) throw std::invalid_argument("paged_attention missing KV cache");
     const KVCacheEntry* e = ctx.kv_cache->get(attrs.require<std::string>("kv_cache"));
     if (e == nullptr) throw std::invalid_argument("paged_attention: unknown kv_cache entry");
-    if (e->batch != q.dim(0) || e->head_dim != q.dim(3) || e->key_pool.dtype() != q.dtype())
+    if (static_cast<std::int64_t>(pos.numel()) != q.dim(0) && e->quantized())
+      throw std::invalid_argument("paged_attention positions must have one entry per sequence");
+    if (!e->quantized() && q.dim(2) != 1)
+      throw std::invalid_argument("paged_attention expects q [B, H, 1, D]");
+    if (e->batch != q.dim(0) || e->head_dim != q.dim(3) || e->dtype != q.dtype())
       throw std::invalid_argument("paged_attention: q does not match the cache entry");
     const std::int64_t B = q.dim(0), Hq = q.dim(1), D = q.dim(3);
     const float scale = static_cast<float>(attrDouble(attrs, "scale", 1.0 / std::sqrt(static_cast<double>(D))));
     // key-range splits per (sequence, kv head); 0 = about one workgroup per CU
     const auto splits = static_cast<int>(attrs.value_or<std::int64_t>("attention_splits", 0));
     *out[0] = Tensor::cuda(q.dtype(), q.shape(), q.deviceId());
+    if (e->quantized()) {
+      if (splits != 0)
+        throw std::invalid_argument("paged_attention: attention_splits of an 8-bit cache must be 0");
+      quantizedAttention(*e, q, &pos, 0, true, scale, false, *out[0], ctx.stream, type());
+      return;
+    }
     const std::size_t ws_bytes = dli_hip_paged_attention_workspace(B, Hq, 1, D, e->capacity());
     check(dli_hip_paged_attention(hipDtype(q.dtype()), ptr(q), ptr(e->key_pool), ptr(e->value_pool),
                                   static_cast<const std::int32_t*>(ptr(e->block_table)), ptr(*out[0]),
@@ -463,6 +523,7 @@ class ArgmaxOp final : public Operator {
 void registerFusedOps(OperatorRegistry* registry) {
   add<QkvRopeAppendOp>(registry);
   add<QkvRopeHeadsOp>(registry);
+  add<RopeAppendOp>(registry);
   add<PagedAttentionOp>(registry);
   add<LinearResidualOp>(registry);
   add<LinearResidualNormOp>(registry);

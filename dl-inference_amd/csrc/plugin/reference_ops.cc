@@ -269,6 +269,11 @@ class AttentionOp final : public Operator {
       past = before ? before->length : 0;
       cache.append(cache_name, k, v);
     }
+    if (cache.get(cache_name)->quantized()) {  // every query sees what the cache holds
+      quantizedAttention(*cache.get(cache_name), q, positions, past, causal, scale, bshd, *out[0],
+                         ctx.stream, type());
+      return;
+    }
     if (positions == nullptr && past == 0) {
       // A prompt from an empty cache: the cache now holds exactly k and v, so attending over
       // them directly is the same computation, and runs on the contiguous (flash) kernel.

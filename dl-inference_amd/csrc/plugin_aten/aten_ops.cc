@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/TensorIndexing.h>
 
+#include <algorithm>
 #include <cmath>
 #include <memory>
 #include <stdexcept>
@@ -329,6 +330,18 @@ class AttentionOp final : public Operator {
         for (auto& p : past) p = length;
       }
       const KVCacheEntry& e = *cache.get(cache_name);
+      if (e.quantized()) {
+        std::int64_t most = 0;
+        for (const std::int64_t p : past) most = std::max(most, p + Sq);
+        const auto [keys, values] = cache.read(cache_name, 0, most, DType::Float32);
+        for (std::int64_t b = 0; b < B; ++b) {
+          const std::int64_t p = past[static_cast<std::size_t>(b)];
+          attend(b, keys.torchTensor()[b].narrow(1, 0, p + Sq),
+                 values.torchTensor()[b].narrow(1, 0, p + Sq).transpose(-1, -2), p);
+        }
+        *out[0] = result(o.view({B, Hq, Sq, D}), q.dtype());
+        return;
+      }
       const at::Tensor& kp = e.key_pool.torchTensor();    // [B, Hkv, capacity, D]
       const at::Tensor& vp = e.value_pool.torchTensor();  // [B, Hkv, D, capacity]
       for (std::int64_t b = 0; b < B; ++b) {

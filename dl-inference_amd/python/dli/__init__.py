@@ -48,6 +48,17 @@ class Engine(_dli_native.Engine):
                 stream = _torch._C._cuda_getCurrentRawStream(_torch._C._cuda_getDevice())
         return super().run(graph, inputs, int(stream), profile)
 
+    def read_kv_cache(self, name, start, length, dtype="", stream=None):
+        """Keys and values [B, H, length, D] that entry `name` holds at positions start .. start +
+        length - 1 of every sequence, as `dtype` (the entry's own by default); zeros where nothing was
+        written."""
+        if stream is None:
+            stream = 0
+            entry = self.kv_cache_entry(name)
+            if entry is not None and entry["key_pool"].is_cuda:
+                stream = _torch._C._cuda_getCurrentRawStream(_torch._C._cuda_getDevice())
+        return super().read_kv_cache(name, start, length, dtype, int(stream))
+
     def load_aten_plugin(self) -> "Engine":
         """Loads the ATen CPU reference plugin (graphs then run on host tensors)."""
         path = aten_plugin_path()

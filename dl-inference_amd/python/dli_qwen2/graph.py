@@ -18,6 +18,11 @@ has a third output, `status` (int32 [1], the launch status the decoder_stack nod
 non-zero when a wait in the persistent launch gave up and the step's outputs are invalid), which
 the decode drivers check where they synchronize anyway.
 
+8-bit KV cache (kv="fp8", any of these but the stack graph; the engine's cache configured alike): the
+fused graphs' qkv_rope_append becomes linear (over the packed q|k|v) and rope_append, which quantises
+keys and values as it writes them; the other graphs' attention nodes append and read by the cache's
+format and stay as they are.
+
 microscaled graph (mx="fp8" or "fp4"): the layers' linears on 4-bit weights (mx_linear), their
 inputs quantised to `mx` by the nodes before them (rms_norm_mx, mx_quantize, silu_mul_mx).
 pack_mx_weights makes its weights. Both plugins run it; prompts have a form of it too.
@@ -89,7 +94,29 @@ def _reference_nodes(cfg: Qwen2Config, batch: int, nodes: list):
     _node(nodes, "greedy", "argmax", ["logits"], ["next_ids"])
 
 
-def _large_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, fused: bool = False):
+def _qkv_nodes(cfg: Qwen2Config, nodes: list, i: int, h: str, norm: str | None, kv: str | None):
+    """A fused graph's nodes from a layer's input to q and the appended cache: `norm` the name of the
+    input norm's weight (None: h is normalized)."""
+    p, t = f"model.layers.{i}.self_attn", f"layers_{i}"
+    heads = {"kv_cache": f"layer_{i}", "q_heads": cfg.heads, "kv_heads": cfg.kv_heads,
+             "head_dim": cfg.head_dim}
+    weights = [f"{p}.qkv_proj.weight", f"{p}.qkv_proj.bias"]
+    where = ["rotary_cos", "rotary_sin", "positions"]
+    if kv is None:
+        _node(nodes, f"{p}.qkv_rope_append", "qkv_rope_append",
+              [h] + ([] if norm is None else [norm]) + weights + where, [f"{t}_q_rotary"],
+              {**heads, "eps": cfg.eps})
+        return
+    if norm is not None:
+        _node(nodes, f"model.layers.{i}.input_layernorm", "rms_norm", [h, norm], [f"{t}_input_norm"],
+              {"eps": cfg.eps})
+        h = f"{t}_input_norm"
+    _node(nodes, f"{p}.qkv_proj", "linear", [h] + weights, [f"{t}_qkv"])
+    _node(nodes, f"{p}.rope_append", "rope_append", [f"{t}_qkv"] + where, [f"{t}_q_rotary"], heads)
+
+
+def _large_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, fused: bool = False,
+                 kv: str | None = None):
     """Decode step for hidden sizes the fused norm-prologue kernels do not hold in registers
     (hidden > 1024, e.g. the Qwen2-7B shape). Attention over the paged cache runs on the MFMA
     decode kernel for head_dim 64 or 128.
@@ -116,12 +143,7 @@ def _large_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, fused:
             next_norm = "model.norm.weight" if last else \
                 f"model.layers.{i + 1}.input_layernorm.weight"
             next_xn = "norm_hidden" if last else f"layers_{i + 1}_input_norm"
-            _node(nodes, f"{p}.self_attn.qkv_rope_append", "qkv_rope_append",
-                  [f"{t}_input_norm", f"{p}.self_attn.qkv_proj.weight",
-                   f"{p}.self_attn.qkv_proj.bias", "rotary_cos", "rotary_sin", "positions"],
-                  [f"{t}_q_rotary"],
-                  {"kv_cache": f"layer_{i}", "q_heads": cfg.heads, "kv_heads": cfg.kv_heads,
-                   "head_dim": cfg.head_dim, "eps": cfg.eps})
+            _qkv_nodes(cfg, nodes, i, f"{t}_input_norm", None, kv)
             _node(nodes, f"{p}.self_attn.attention", "paged_attention",
                   [f"{t}_q_rotary", "positions"], [f"{t}_attention"],
                   {"kv_cache": f"layer_{i}", "attention_splits": splits.get("attn", 0)})
@@ -268,17 +290,13 @@ def _plain_head_nodes(cfg: Qwen2Config, nodes: list, h: str):
     _node(nodes, "greedy", "argmax", ["logits"], ["next_ids"])
 
 
-def _fused_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, logits_dtype: str):
+def _fused_nodes(cfg: Qwen2Config, batch: int, nodes: list, splits: dict, logits_dtype: str,
+                 kv: str | None = None):
     h = "hidden_states"
     for i in range(cfg.layers):
         p = f"model.layers.{i}"
         t = f"layers_{i}"
-        _node(nodes, f"{p}.self_attn.qkv_rope_append", "qkv_rope_append",
-              [h, f"{p}.input_layernorm.weight", f"{p}.self_attn.qkv_proj.weight",
-               f"{p}.self_attn.qkv_proj.bias", "rotary_cos", "rotary_sin", "positions"],
-              [f"{t}_q_rotary"],
-              {"kv_cache": f"layer_{i}", "q_heads": cfg.heads, "kv_heads": cfg.kv_heads,
-               "head_dim": cfg.head_dim, "eps": cfg.eps})
+        _qkv_nodes(cfg, nodes, i, h, f"{p}.input_layernorm.weight", kv)
         _node(nodes, f"{p}.self_attn.attention", "paged_attention", [f"{t}_q_rotary", "positions"],
               [f"{t}_attention"],
               {"kv_cache": f"layer_{i}", "attention_splits": splits.get("attn", 0)})
@@ -363,8 +381,9 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
                        splits: dict | None = None, logits_dtype: str = "float32",
                        stack: bool = False, check_status: bool = False,
                        large_fused: bool = False, stack_trace: bool = False,
-                       mx: str | None = None, dtype: str = "bfloat16") -> "dli.Graph":
-    """mx: the layers on microscaled linears with activations in that format ("fp8", "fp4") and
+                       mx: str | None = None, dtype: str = "bfloat16",
+                       kv: str | None = None) -> "dli.Graph":
+    """kv: the format of the engine's cache, None or "fp8" (_qkv_nodes). mx: the layers on microscaled linears with activations in that format ("fp8", "fp4") and
     hidden states in `dtype` (_mx_layer_nodes), whatever the forms below; fused then only says
     that the head may be one lm_head_argmax node, where that takes it (fused_head_fits). Else fused=False: the reference's node sequence; fused=True: five launches per layer;
     stack=True (with fused): all layers in one decoder_stack node (check_status: the node waits
@@ -374,6 +393,10 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
     splits: {"o", "down": K splits, "attn": attention key-range splits, 0 = each call's own
     choice}; stack_trace: the decoder_stack node records its stage timeline into graph input
     "stack_trace" (int64, layers x CUs x 24)."""
+    if kv not in (None, "fp8"):
+        raise ValueError(f"kv must be None or fp8, not {kv!r}")
+    if kv is not None and fused and stack and mx is None and not uses_large_graph(cfg, fused):
+        raise ValueError("the decoder stack takes no 8-bit KV cache")
     nodes: list = []
     if mx is not None or not (fused and stack) or uses_large_graph(cfg, fused):  # the stack gathers it itself
         _node(nodes, "model.embed_tokens", "embedding", ["input_ids", "model.embed_tokens.weight"],
@@ -391,14 +414,14 @@ def build_decode_graph(cfg: Qwen2Config, batch: int, fused: bool = True,
                  "inputs": INPUTS, "outputs": OUTPUTS, "nodes": nodes}
         return dli.Graph.from_json(json.dumps(graph))
     if uses_large_graph(cfg, fused):
-        _large_nodes(cfg, batch, nodes, splits or large_splits(batch), large_fused)
+        _large_nodes(cfg, batch, nodes, splits or large_splits(batch), large_fused, kv)
         graph = {"format": "dli.graph.v1", "model_type": "qwen2_decode_large",
                  "inputs": INPUTS, "outputs": OUTPUTS, "nodes": nodes}
         return dli.Graph.from_json(json.dumps(graph))
     if fused and stack:
         _stack_nodes(cfg, nodes, splits or STACK_SPLITS, logits_dtype, check_status, stack_trace)
     elif fused:
-        _fused_nodes(cfg, batch, nodes, splits or DEFAULT_SPLITS, logits_dtype)
+        _fused_nodes(cfg, batch, nodes, splits or DEFAULT_SPLITS, logits_dtype, kv)
     else:
         _reference_nodes(cfg, batch, nodes)
     model_type = "qwen2_decode" if not fused else ("qwen2_decode_stack" if stack else "qwen2_decode_fused")

@@ -21,11 +21,15 @@ class DecodeSession:
                  fused: bool = True, engine: "dli.Engine | None" = None, splits: dict | None = None,
                  block_size: int = 64, logits_dtype: str = "float32", device: str = "cuda",
                  stack: bool = False, check_status: bool = False, prefill: bool = False,
-                 stack_trace: "torch.Tensor | None" = None, mx: str | None = None):
+                 stack_trace: "torch.Tensor | None" = None, mx: str | None = None,
+                 kv: str | None = None):
         """mx ("fp8" or "fp4"): the layers' linears run on 4-bit weights, quantised here (or taken as
         pack_mx_weights made them), with activations in that format; decode steps and prompts alike.
         It has no stack form, so small models (the 0.5B shape) take fewer bytes but more time a step
-        than in bfloat16."""
+        than in bfloat16.
+        kv ("fp8"): keys and values are cached in 8 bits, quantised as they are written, half the bytes
+        of 16-bit ones to hold and to read. Every query attends over what the cache holds, a prompt's
+        own tokens included. It has no stack form either."""
         if mx is not None and stack:
             raise ValueError("the microscaled graph has no decoder stack form")
         self.cfg = cfg
@@ -36,7 +40,8 @@ class DecodeSession:
         self._mx = {} if mx is None else {
             "mx": mx, "dtype": str(weights["model.norm.weight"].dtype).removeprefix("torch.")}
         self.engine = engine or dli.Engine().load_plugin()
-        self.engine.configure_kv_cache(block_size=block_size, max_seq_len=max_seq_len)
+        self.engine.configure_kv_cache(block_size=block_size, max_seq_len=max_seq_len,
+                                       format=kv or "")
         # the large-hidden graph's GPU form (fused q|k|v, residual + RMSNorm and MLP nodes of
         # the GPU plugin; the ATen CPU plugin runs the reference's nodes)
         large_fused = uses_large_graph(cfg, fused) and device != "cpu" and not prefill
@@ -47,7 +52,7 @@ class DecodeSession:
         self.graph = build_decode_graph(cfg, batch, fused=fused, splits=splits,
                                         logits_dtype=logits_dtype, stack=stack,
                                         check_status=check_status, large_fused=large_fused,
-                                        stack_trace=stack_trace is not None, **self._mx)
+                                        stack_trace=stack_trace is not None, kv=kv, **self._mx)
         # prefill=True: generate() runs the prompt through one prefill graph (the layers over
         # [B, S] tokens at once), which reads the unpacked q/k/v and gate/up weights
         self.prefill = prefill

@@ -27,6 +27,7 @@
 
 #include <cstdint>
 #include <memory>
+#include <string>
 
 #include "dli/engine.h"
 
@@ -36,6 +37,7 @@ struct GreedyOptions {
   std::int64_t block_size = 64;     // KV cache block size (tokens)
   std::int64_t max_seq_len = 4096;  // KV capacity per sequence; later positions are rejected
   bool capture = true;              // HIP graph capture/replay of the step (device weights)
+  std::string kv_format;            // KVCache::configure's format: "" or "fp8"
 };
 
 class GreedyDecoder {

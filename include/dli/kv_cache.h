@@ -22,10 +22,20 @@
 // the same structure with one block per sequence (block_size = capacity, identity table), so a
 // sequence's keys are [heads, capacity, head_dim] and its values [heads, head_dim, capacity],
 // each contiguous; they do not grow beyond the configured max_seq_len.
+//
+// Format "fp8" (configure): the pools hold e4m3 elements (uint8), quantised as they are written, and
+// a third pool holds two scales per token and head, powers of two (one byte each):
+//
+//   scales [num_blocks, heads, 2, block_size]   the keys', then the values'
+//
+// Every reader of such an entry sees what it holds: a prompt's own queries attend over the quantised
+// keys and values too, so results do not depend on how a prompt is cut into runs. The quantisation
+// rule is that of dli_hip_kv_append_fp8 (include/dli_hip.h).
 
 #include <cstdint>
 #include <map>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "dli/tensor.h"
@@ -48,8 +58,11 @@ struct KVCacheEntry {
   std::int64_t block_size = 0;
   std::int64_t max_blocks = 0;  // per sequence
   std::int64_t length = 0;      // host-tracked tokens per sequence (append() path)
+  Tensor scales;                // format "fp8" only
+  DType dtype = DType::Float32;  // of the keys and values that go in and come out
 
   std::int64_t capacity() const { return max_blocks * block_size; }
+  bool quantized() const { return scales.defined(); }
 };
 
 class KVCache {
@@ -67,12 +80,22 @@ class KVCache {
                 const Tensor& positions);
 
   // Allocates (or returns) an entry ahead of time. Capacity per sequence is max_seq_len
-  // rounded up to whole blocks.
+  // rounded up to whole blocks. A caller that binds the pools itself as `dtype` gets no quantised
+  // entry (std::invalid_argument) unless it says that it takes any format.
   KVCacheEntry& reserve(const std::string& name, DType dtype, std::int64_t batch,
-                        std::int64_t heads, std::int64_t head_dim, int device_id);
+                        std::int64_t heads, std::int64_t head_dim, int device_id,
+                        bool any_format = false);
   KVCacheEntry* find(const std::string& name);
 
-  void configure(std::int64_t block_size, std::int64_t max_seq_len);
+  // Keys and values [B, H, length, D] that the entry holds at positions start .. start + length - 1 of
+  // every sequence, as `dtype`; zeros where nothing was written. Quantised entries on the device are
+  // read on the cache's stream, others on torch's current one.
+  std::pair<Tensor, Tensor> read(const std::string& name, std::int64_t start, std::int64_t length,
+                                 DType dtype);
+
+  // format: "" (pools in the tensors' type) or "fp8"; entries made earlier keep theirs.
+  void configure(std::int64_t block_size, std::int64_t max_seq_len, const std::string& format = "");
+  const std::string& format() const { return format_; }
   std::int64_t blockSize() const { return block_size_; }
   std::int64_t maxSeqLen() const { return max_seq_len_; }
   // Stream used by the scatter kernels (nullptr = the null stream).
@@ -86,6 +109,7 @@ class KVCache {
   std::int64_t block_size_ = 64;
   std::int64_t max_seq_len_ = 4096;
   void* stream_ = nullptr;
+  std::string format_;
 
   void grow(KVCacheEntry& entry, std::int64_t needed_tokens);
 };

@@ -1,8 +1,10 @@
 """The 8-bit paged KV cache in plain numpy: float64 and exact e4m3 arithmetic (formats in
-include/dli_hip.h). Pools are numpy uint8 arrays, positions and tables plain lists."""
+include/dli_hip.h). Pools are numpy uint8 arrays, positions and tables plain lists. check_attention
+holds an attention's output against it."""
 from __future__ import annotations
 
 import numpy as np
+import torch
 
 LARGEST = 448.0
 
@@ -135,3 +137,32 @@ class Cache:
                     level[b, h, i] = (np.abs(Vh) / one).sum(0) * one.max()
                     spread[b, h, i] = (np.abs(Kh) @ np.abs(q[b, h, i])).max() * abs(scale)
         return out, mag, spread, level
+
+
+def check_attention(out, want, dtype, keys, dim):
+    """want: (value, magnitude A = sum p |v|, spread = largest sum |q k| scale, level = sum |element|
+    times the largest value scale) in float64. The output is rounded once (half a step, and another half
+    of the least subnormal; half a step past the largest number to infinity). A weight is rounded to f16 once
+    (bf16 outputs) or kept to 22 bits; a score's fp32 sum of `dim` products, its scaling and
+    the exponential shift it by at most (dim + 8) 2^-24 of the row's spread and the largest exponent
+    argument, which moves a weight by that share and its sum likewise; the outputs' fp32 sums run
+    over at most 4 steps a 64-key tile and the joins. f16's least step is 2^-24, so a weight (and the
+    rest of one in two terms) is off by up to 2^-25 in any case; the row's sum of weights is at least
+    2^13 in those units and an element's factor at most the largest value scale: 2^-38 of the level."""
+    value, mag, spread, level = want
+    got = out.double().cpu().numpy()
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    weight = 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -22
+    score = 2 * (dim + 8) * 2.0 ** -24 * (spread + 30)
+    sums = (4 * (keys / 64) + 96) * 2.0 ** -24
+    bound = half * np.abs(value) + (1 + half) * (weight + score + sums) * mag + tiny
+    bound += 2.0 ** -38 * level
+    nan = np.isnan(value)
+    assert np.array_equal(np.isnan(got), nan)
+    over = np.abs(np.nan_to_num(value)) > (1 + half) * torch.finfo(dtype).max
+    assert np.array_equal(got[over], np.copysign(np.inf, value[over]))
+    with np.errstate(invalid="ignore"):
+        err = np.where(nan | over, 0.0, np.abs(got - value))
+    worst = np.nanmax(np.where(bound > 0, err / np.maximum(bound, 1e-300), err > 0)) if err.size else 0
+    assert worst <= 1, worst
