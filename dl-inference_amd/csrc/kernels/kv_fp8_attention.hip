@@ -442,19 +442,54 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks.
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunkThreads = 256;
+// exponent of a staged value's factor at the largest value scale: elements reach 448 * 2^7 there, and a
+// token's elements stay exact in f16 down to 2^-22 of that scale
+constexpr int kValueLift = 7;
+constexpr float kNoReference = 1e30f;
 
 __device__ __forceinline__ int valueChunk(int d, int chunk) {
   return d * kTileK + (chunk ^ ((d >> 1) & 7)) * 8;
 }
 
+// 2^(code - top + kValueLift) as f16, 0 below its least subnormal
+__device__ __forceinline__ uint16_t valueFactorF16(uint32_t code, uint32_t top) {
+  const int e = static_cast<int>(code) - static_cast<int>(top) + kValueLift + 15;
+  return static_cast<uint16_t>(e > 0 ? e << 10 : e > -10 ? 1 << (9 + e) : 0);
+}
+
+// 8 value codes times their tokens' factors
+__device__ __forceinline__ U128 valueFragment(uint32_t w0, uint32_t w1, const U128& factors) {
+  return __builtin_bit_cast(U128, __builtin_bit_cast(f16x8, codesToF16(w0, w1)) *
+                                      __builtin_bit_cast(f16x8, factors));
+}
+
+// 8 key codes times 2^e as bf16 (exact: a bf16 has fp32's exponents)
+__device__ __forceinline__ U128 scaledKey(uint32_t w0, uint32_t w1, float scale) {
+  return U128{
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true))};
+}
+
+template <class T, int D>
+struct ChunkLds {
+  static constexpr int kPitch = D + 8;  // 16 rows start on 16 distinct groups of 4 banks
+  uint16_t k[2][kTileK * kPitch];
+  uint16_t v[2][D * kTileK];
+  float kf[4][kTileK];     // each wave's own copy of the tile's key scales
+  uint16_t vf[4][kTileK];  // and of the value factors
+};
+
 template <class T, int D, int QB, bool kSmall>
 __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   using Ty = Kv8Type<T>;
-  constexpr int kPitch = D + 8;  // 16 rows start on 16 distinct groups of 4 banks
+  using Lds = ChunkLds<T, D>;
+  // f16 keys stay unscaled (their range would not hold a scaled one), the score takes the scale
+  constexpr bool kScaleKeys = !__is_same(T, f16);
   constexpr int DT = D / 16, DK = D / 32, kPer = D / 64;
   constexpr int kParts = D / 16;  // 16-code chunks of a key
-  __shared__ __attribute__((aligned(16))) uint16_t Ks[kTileK * kPitch];
-  __shared__ __attribute__((aligned(16))) uint16_t Vt[D * kTileK];
+  __shared__ __attribute__((aligned(16))) Lds lds;
   const Kv8Pages& pg = a.pages;
   const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int r = lane % 16, g = lane / 16;
@@ -487,15 +522,17 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   const int kt0 = static_cast<int>(blockIdx.z) * per;
   const int kt1 = kt0 + per < all_tiles ? kt0 + per : all_tiles;
 
-  // page ids of the next tile's four runs of 16 keys (one page where pages are not small)
+  // page ids of a tile's four runs of 16 keys (one page where pages are not small)
   const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
+  const uint32_t last_run = static_cast<uint32_t>((a.capacity - 1) / 16);
+  const uint32_t runs_per_page = static_cast<uint32_t>(bs) / 16;
   int id[4];
-  auto loadIds = [&](int kt) {
+  auto loadIds = [&](int kt) {  // runs past the pages repeat the last one and are masked
 #pragma unroll
     for (int u = 0; u < (kSmall ? 4 : 1); ++u) {
-      const int64_t key = static_cast<int64_t>(kt) * kTileK + 16 * u;
-      int x = -1;
-      if (kt < kt1 && key < a.capacity) x = gp(table)[static_cast<uint32_t>(key) / static_cast<uint32_t>(bs)];
+      uint32_t run = static_cast<uint32_t>(kt) * 4 + u;
+      run = run < last_run ? run : last_run;
+      const int x = gp(table)[run / runs_per_page];
       id[u] = x < pg.num_blocks ? x : -1;
     }
     if (!kSmall) id[1] = id[2] = id[3] = id[0];
@@ -504,55 +541,64 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   auto headOf = [&](int page) {  // a page that holds nothing: page 0 is read in its place and masked
     return static_cast<int64_t>(page < 0 ? 0 : page) * pg.heads + kvh;
   };
+  // offsets of this thread's chunks within a page's head
+  const int64_t head = static_cast<int64_t>(bs) * D;
+  uint32_t ko[kPer], vo[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int c = t + i * kChunkThreads;
+    ko[i] = kSmall ? static_cast<uint32_t>(c / kParts % bs * D + c % kParts * 16)
+                   : static_cast<uint32_t>(c * 16);
+    vo[i] = static_cast<uint32_t>(c / 4) * static_cast<uint32_t>(bs) +
+            static_cast<uint32_t>(kSmall ? 16 * (c % 4) % bs : 16 * (c % 4));
+  }
   U128 kr[kPer], vr[kPer];
   uint32_t kc = 0, vc = 0;
   bool in_page = false;
   auto fetch = [&](int kt) {
-    const int slot0 = kSmall ? 0 : static_cast<int>(static_cast<uint32_t>(kt) * kTileK % static_cast<uint32_t>(bs));
-    const int64_t head = static_cast<int64_t>(bs) * D;
+    if constexpr (kSmall) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = t + i * kChunkThreads;
-      const int key = c / kParts, part = c % kParts;
-      const int ks = kSmall ? key % bs : slot0 + key;
-      kr[i] = gload16(pg.key + headOf(pick(key / 16)) * head + static_cast<int64_t>(ks) * D + part * 16);
-      const int d = c / 4, run = c % 4;
-      const int vs = kSmall ? 16 * run % bs : slot0 + 16 * run;
-      vr[i] = gload16(pg.value + headOf(pick(run)) * head + static_cast<int64_t>(d) * bs + vs);
-    }
-    const int page = pick(g);
-    in_page = page >= 0;
-    const uint8_t* sb = pg.scales + headOf(page) * 2 * bs + (kSmall ? lane % bs : slot0 + lane);
-    kc = gp(sb)[0];
-    vc = gp(sb)[bs];
-  };
-  auto stash = [&](uint64_t lives) {
+      for (int i = 0; i < kPer; ++i) {
+        const int c = t + i * kChunkThreads;
+        kr[i] = gload16(pg.key + headOf(pick(c / kParts / 16)) * head + ko[i]);
+        vr[i] = gload16(pg.value + headOf(pick(c % 4)) * head + vo[i]);
+      }
+      const int page = pick(g);
+      in_page = page >= 0;
+      const uint8_t* sb = pg.scales + headOf(page) * 2 * bs + lane % bs;
+      kc = gp(sb)[0];
+      vc = gp(sb)[bs];
+    } else {
+      const uint32_t slot = static_cast<uint32_t>(kt) % (runs_per_page / 4) * kTileK;
+      const int64_t hb = headOf(id[0]);
+      const uint8_t* kb = pg.key + hb * head + static_cast<int64_t>(slot) * D;
+      const uint8_t* vb = pg.value + hb * head + slot;
+      const uint8_t* sb = pg.scales + hb * 2 * bs + slot;
+      in_page = id[0] >= 0;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int c = t + i * kChunkThreads;
-      const int key = c / kParts, part = c % kParts;
-      // the score of row 4 g + i of the 16-key group kk is that of key 16 g + 4 kk + i
-      const int row = 16 * (key % 16 / 4) + 4 * (key / 16) + key % 4;
-      U128* ko = reinterpret_cast<U128*>(&Ks[row * kPitch + part * 16]);
-      ko[0] = keyFragment<T>(kr[i][0], kr[i][1]);
-      ko[1] = keyFragment<T>(kr[i][2], kr[i][3]);
-      const int d = c / 4, run = c % 4;
-      if (lives != ~uint64_t{0}) keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
-      *reinterpret_cast<U128*>(&Vt[valueChunk(d, 2 * run)]) = codesToF16(vr[i][0], vr[i][1]);
-      *reinterpret_cast<U128*>(&Vt[valueChunk(d, 2 * run + 1)]) = codesToF16(vr[i][2], vr[i][3]);
+      for (int i = 0; i < kPer; ++i) {
+        kr[i] = gload16(kb + ko[i]);
+        vr[i] = gload16(vb + vo[i]);
+      }
+      kc = gp(sb)[lane];
+      vc = gp(sb + bs)[lane];
     }
   };
 
   f32x4 o[QB][DT];
-  float m[QB], l[QB];
-  uint32_t top = 0;
+  f32x4 ls[QB];        // element 0 of the lanes g = 0: the sum of row r's weights
+  float shift[QB];     // kLift less the row's reference
+  uint32_t top = 0;    // the largest value scale seen, which o is kept in
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    m[qb] = -INFINITY;
-    l[qb] = 0.f;
+    shift[qb] = kNoReference;
+    ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  const float score_scale = kScaleKeys ? a.scale_log2 : 1.f;
+  const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
+  const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
 
   if (kt0 < kt1) {
     loadIds(kt0);
@@ -560,19 +606,14 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     loadIds(kt0 + 1);
   }
   for (int kt = kt0; kt < kt1; ++kt) {
-    const int k0 = kt * kTileK;
-    const uint64_t lives = __builtin_amdgcn_ballot_w64(in_page && k0 + lane < wg_keys);
-    const KeyScales sc = keyScales(kc, vc, in_page && k0 + lane < wg_keys, a.scale_log2);
-    __syncthreads();  // the previous tile is no longer read
-    stash(lives);
-    __syncthreads();
-    if (kt + 1 < kt1) {
-      fetch(kt + 1);
-      loadIds(kt + 2);
-    }
-    if (!active) continue;
-    if (__builtin_amdgcn_ballot_w64(sc.v > top)) {
-      const uint32_t next = waveMaxU(sc.v);
+    const int k0 = kt * kTileK, buf = kt & 1;
+    const bool live = in_page && k0 + lane < wg_keys;
+    const bool bad = kc == 255u || vc == 255u;
+    const uint64_t lives = __builtin_amdgcn_ballot_w64(live);
+    const uint64_t bads = __builtin_amdgcn_ballot_w64(live && bad);
+    const uint32_t vcode = bad || !live ? 0u : vc;
+    if (__builtin_amdgcn_ballot_w64(vcode > top)) {  // every wave comes to the same
+      const uint32_t next = waveMaxU(vcode);
       const float down = valueFactor(top, next);
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
@@ -580,7 +621,43 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
         for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= down;
       top = next;
     }
-    const float vf = valueFactor(sc.v, top);
+    const float kf = mxScaleValue(bad ? 255u : kc) * (kScaleKeys ? 1.f : a.scale_log2);
+    if constexpr (kScaleKeys) lds.kf[wave][lane] = kf;
+    lds.vf[wave][lane] = valueFactorF16(vcode, top);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' factors are read below
+    const U128 vf0 = load16(&lds.vf[wave][16 * (t % 4)]), vf1 = load16(&lds.vf[wave][16 * (t % 4) + 8]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int c = t + i * kChunkThreads;
+      const int key = c / kParts, part = c % kParts;
+      // the score of row 4 g + i of the 16-key group kk is that of key 16 g + 4 kk + i
+      const int row = 16 * (key % 16 / 4) + 4 * (key / 16) + key % 4;
+      U128* to = reinterpret_cast<U128*>(&lds.k[buf][row * Lds::kPitch + part * 16]);
+      U128 k0v, k1v;
+      if constexpr (kScaleKeys) {
+        const float f = lds.kf[wave][key];
+        k0v = scaledKey(kr[i][0], kr[i][1], f);
+        k1v = scaledKey(kr[i][2], kr[i][3], f);
+        if (bads != 0 && (bads >> key & 1)) k0v = k1v = U128{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+      } else {
+        k0v = keyFragment<T>(kr[i][0], kr[i][1]);
+        k1v = keyFragment<T>(kr[i][2], kr[i][3]);
+      }
+      to[0] = k0v;
+      to[1] = k1v;
+      const int d = c / 4, run = c % 4;
+      if (lives != ~uint64_t{0}) keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
+      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, 2 * run)]) = valueFragment(vr[i][0], vr[i][1], vf0);
+      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, 2 * run + 1)]) =
+          valueFragment(vr[i][2], vr[i][3], vf1);
+    }
+    if (kt + 1 < kt1) {
+      fetch(kt + 1);
+      loadIds(kt + 2);
+    }
+    // one barrier a tile: the other buffer was last read before the previous one
+    __syncthreads();
+    if (!active) continue;
 
     f32x4 s[QB][4];
 #pragma unroll
@@ -589,7 +666,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
       for (int qb = 0; qb < QB; ++qb) s[qb][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < DK; ++c) {
-        const U128 ka = load16(&Ks[(kk * 16 + r) * kPitch + c * 32 + g * 8]);
+        const U128 ka = load16(&lds.k[buf][(kk * 16 + r) * Lds::kPitch + c * 32 + g * 8]);
 #pragma unroll
         for (int u = Ty::kQ - 1; u >= 0; --u)
 #pragma unroll
@@ -600,57 +677,60 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     U128 pf[QB][Ty::kP][2];
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      timesKeys(s[qb], sc.k);
+      if constexpr (!kScaleKeys) timesKeys(s[qb], kf);
       if (!full) {
-        const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu;
-        const int key0 = k0 + 16 * g;
+        const int seen = lim[qb] - k0 - 16 * g;
+        const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu &
+                              (seen >= 16 ? 0xFFFFu : seen > 0 ? (1u << seen) - 1u : 0u);
 #pragma unroll
         for (int n = 0; n < 16; ++n)
-          if (!(mine >> n & 1u) || key0 + n >= lim[qb]) s[qb][n / 4][n % 4] = -INFINITY;
+          if (!(mine >> n & 1u)) s[qb][n / 4][n % 4] = -INFINITY;
       }
-      float tmax = -INFINITY;
+      float smax = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) tmax = fmaxf(tmax, s[qb][n / 4][n % 4]);
-      tmax = rowsMax(tmax);
-      const bool grow = tmax > m[qb] + kSlack;
-      if (__builtin_amdgcn_ballot_w64(grow)) {
-        const float alpha = grow ? __builtin_amdgcn_exp2f(m[qb] - tmax) : 1.f;
-        m[qb] = grow ? tmax : m[qb];
-        l[qb] *= alpha;
+      for (int n = 0; n < 16; ++n) smax = fmaxf(smax, s[qb][n / 4][n % 4]);
+      // the reference moves only when a weight would pass 2^(kLift + kSlack)
+      if (__builtin_amdgcn_ballot_w64(fmaf(smax, score_scale, shift[qb]) > kLift + kSlack)) {
+        const float tmax = rowsMax(smax) * score_scale;  // the same in a row's four lanes
+        const bool grow = tmax + shift[qb] > kLift + kSlack;
+        const float next = kLift - tmax;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(next - shift[qb]) : 1.f;  // 0 at first
+        shift[qb] = grow ? next : shift[qb];
+        ls[qb] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
       }
-      const float base = (m[qb] == -INFINITY ? 0.f : m[qb]) - kLift;
-      float sum = 0.f;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        s[qb][n / 4][n % 4] = __builtin_amdgcn_exp2f(s[qb][n / 4][n % 4] - base);
-        sum += s[qb][n / 4][n % 4];
-      }
-      l[qb] += sum;
-      timesKeys(s[qb], vf);
+      for (int n = 0; n < 16; ++n)
+        s[qb][n / 4][n % 4] =
+            __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], score_scale, shift[qb]));
       packWeights<Ty::kP>(s[qb], pf[qb]);
     }
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int u = Ty::kP - 1; u >= 0; --u)
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) ls[qb] = F16::mma(ones, pf[qb][u][st], ls[qb]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const U128 va = load16(&Vt[valueChunk(16 * dt + r, 2 * g + st)]);
+        const U128 va = load16(&lds.v[buf][valueChunk(16 * dt + r, 2 * g + st)]);
 #pragma unroll
         for (int u = Ty::kP - 1; u >= 0; --u)
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[qb][dt] = F16::mma(va, pf[qb][u][st], o[qb][dt]);
       }
+    }
   }
 
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const float L = rowsSum(l[qb]);
+    const float L = __shfl(ls[qb][0], r, kWave);
     const int p = pw + qb * 16 + r;
     if (p >= rows) continue;
     const RowAt at = rowAt(p, group, kvh);
     const float inv = L == 0.f ? 0.f : 1.f / L;  // no key, or none of any weight: zeros
-    const int e = static_cast<int>(top) - 127;
+    const int e = static_cast<int>(top) - 127 - kValueLift;
     if (a.splits == 1) {
       T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + 4 * g;
 #pragma unroll
@@ -661,7 +741,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     } else {
       const int64_t part = queryAt(a, b, at, 1) * a.splits + blockIdx.z;
       if (g == 0) {
-        a.part_ml[part * 2] = m[qb];
+        a.part_ml[part * 2] = L == 0.f ? -INFINITY : kLift - shift[qb];
         a.part_ml[part * 2 + 1] = L;
       }
       float* out = a.part_o + part * D + 4 * g;
@@ -774,11 +854,11 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
 }  // namespace
 
 #define KV8_CHUNK(suffix, T, D, QB)                                                             \
-  extern "C" __global__ void __launch_bounds__(kChunkThreads)                                   \
+  extern "C" __global__ void __launch_bounds__(kChunkThreads, 2)                                \
       kv8_chunk_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                                   \
     kv8_chunk<T, D, QB, false>(a);                                                              \
   }                                                                                             \
-  extern "C" __global__ void __launch_bounds__(kChunkThreads)                                   \
+  extern "C" __global__ void __launch_bounds__(kChunkThreads, 2)                                \
       kv8_chunk_small_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                             \
     kv8_chunk<T, D, QB, true>(a);                                                               \
   }
