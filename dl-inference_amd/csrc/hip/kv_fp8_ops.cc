@@ -37,12 +37,15 @@ DeviceKernel k_read_any[3] = KV8_DTYPES("kv_fp8", "kv8_read_any");
 // [small pages][head_dim][dtype]
 DeviceKernel k_decode[2][2][3] = {KV8_DIMS("kv_fp8_attention", "kv8_decode_", ""),
                                   KV8_DIMS("kv_fp8_attention", "kv8_decode_small_", "")};
-// [small pages][64 or 128 rows][head_dim][dtype]
-DeviceKernel k_chunk[2][2][2][3] = {{KV8_DIMS("kv_fp8_attention", "kv8_chunk_", "_q1"),
-                                     KV8_DIMS("kv_fp8_attention", "kv8_chunk_", "_q2")},
-                                    {KV8_DIMS("kv_fp8_attention", "kv8_chunk_small_", "_q1"),
-                                     KV8_DIMS("kv_fp8_attention", "kv8_chunk_small_", "_q2")}};
-DeviceKernel k_merge[3] = KV8_DTYPES("kv_fp8_attention", "kv8_merge");
+// [small pages][head_dim][dtype], 64 rows a workgroup
+DeviceKernel k_chunk[2][2][3] = {KV8_DIMS("kv_fp8_attention", "kv8_chunk_", "_r64"),
+                                 KV8_DIMS("kv_fp8_attention", "kv8_chunk_small_", "_r64")};
+// [small pages]: 128 rows, bf16 of head_dim 64 and 128, f16 of 128
+#define KV8_LARGE(base)                                                                          \
+  { {"kv_fp8_attention", base "d64_r128_bf16"}, {"kv_fp8_attention", base "d128_r128_bf16"},      \
+    {"kv_fp8_attention", base "d128_r128_f16"} }
+DeviceKernel k_chunk_large[2][3] = {KV8_LARGE("kv8_chunk_"), KV8_LARGE("kv8_chunk_small_")};
+DeviceKernel k_merge[2][3] = KV8_DIMS("kv_fp8_attention", "kv8_merge_", "");
 DeviceKernel k_rows[3] = KV8_DTYPES("kv_fp8_attention", "kv8_rows");
 
 constexpr int64_t kMostTokens = int64_t{1} << 30;  // of a sequence, and rows of a pair: 32-bit indexes
@@ -116,11 +119,11 @@ int launchWrite(const Kv8WriteArgs& a, bool tiles, int rows, int di, DeviceKerne
 // How attention runs: 0 one wave per row, 1 decode (at most 16 rows of a pair), 2 chunk.
 struct AttentionPlan {
   int form;
-  int row_blocks;  // chunk: 64-row blocks of a workgroup, 1 or 2
+  int size;  // chunk: 0 for 64 rows a workgroup, 1 for 128
   int64_t splits;
 };
 
-AttentionPlan attentionPlan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
+AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
                             int64_t head_dim, int64_t block_size, int64_t max_blocks) {
   const int64_t units = batch * kv_heads, rows = q_heads / kv_heads * seq_q;
   const bool paged = block_size % 64 == 0 || block_size == 16 || block_size == 32;
@@ -134,14 +137,25 @@ AttentionPlan attentionPlan(int64_t batch, int64_t q_heads, int64_t kv_heads, in
     splits = splits < most ? splits : most;
     return {1, 0, splits < 32 ? splits : 32};
   }
-  const int64_t big = units * ((rows + 127) / 128);
-  const int row_blocks = big >= 128 ? 2 : 1;
-  const int64_t blocks = units * ((rows + 64 * row_blocks - 1) / (64 * row_blocks));
+  // 128 rows share a staged tile where they still fill half the card. 64 and 128 rows, us: bf16, 2 x
+  // 300 tokens over 3000 (28 / 4 heads x 128, 136 workgroups of 128) 90 and 66; 1 x 2048 over 8192 484 and
+  // 347; 4 x 2048 tokens (14 / 2 x 64) 63 and 54. f16 holds its weights in two terms and pays from more
+  // workgroups on, with head_dim 128 only: 2 x 500 over 2000 80 and 87, 1 x 2000 over 3000 246 and 211, 4 x 1000
+  // over 500 (x 64) 45 and 47. fp32 (three terms of q) never: 92 and 113, 36 and 40.
+  const int64_t large = units * ((rows + 127) / 128);
+  const int size = dtype == DLI_BF16  ? large >= 128
+                   : dtype == DLI_F16 ? large >= 384 && head_dim == 128
+                                      : 0;
+  const int64_t tile_rows = int64_t{64} << size;
+  const int64_t blocks = units * ((rows + tile_rows - 1) / tile_rows);
+  // keys split until two workgroups stand on every CU, each with 4 tiles at least; a split's results
+  // are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4 heads
+  // x 128: 41 us, 65 in two splits)
   int64_t splits = 512 / blocks;
   const int64_t most = tiles / 4;
   splits = splits < most ? splits : most;
   splits = splits < 32 ? splits : 32;
-  return {2, row_blocks, splits > 1 ? splits : 1};
+  return {2, size, splits > 1 ? splits : 1};
 }
 
 size_t partBytes(int64_t rows, int64_t head_dim, int64_t splits) {
@@ -242,9 +256,13 @@ size_t dli_hip_paged_attention_fp8_workspace(int64_t batch, int64_t q_heads, int
       seq_q >= kMostTokens || block_size >= kMostTokens || max_blocks >= kMostTokens ||
       block_size * max_blocks >= kMostTokens)
     return 0;
-  const AttentionPlan plan =
-      attentionPlan(batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
-  return partBytes(batch * q_heads * seq_q, head_dim, plan.splits);
+  int64_t splits = 1;  // the most of any data type
+  for (int dtype : {DLI_F32, DLI_BF16, DLI_F16}) {
+    const AttentionPlan plan =
+        attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
+    splits = splits > plan.splits ? splits : plan.splits;
+  }
+  return partBytes(batch * q_heads * seq_q, head_dim, splits);
 }
 
 int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
@@ -268,7 +286,7 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
   const int64_t rows = batch * q_heads * seq_q;
   if (rows >= (int64_t{1} << 31)) return badArg(op, "too many query rows");
   AttentionPlan plan =
-      attentionPlan(batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
+      attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
   // the MFMA forms take 16-byte loads and put masked scores to -inf before the scale's sign could
   // matter, as the other attention kernels do
   if (!(scale > 0.f) || !std::isfinite(scale) || !aligned16(q) || !aligned16(out) ||
@@ -299,14 +317,16 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
     rc = launch(k_decode[small][dim][di], {static_cast<unsigned>(plan.splits), units}, {512}, 0, stream,
                 a);
   } else {
-    const int64_t tile = 64 * plan.row_blocks, pair_rows = q_heads / kv_heads * seq_q;
-    rc = launch(k_chunk[small][plan.row_blocks - 1][dim][di],
+    const int64_t tile = int64_t{64} << plan.size, pair_rows = q_heads / kv_heads * seq_q;
+    DeviceKernel& chunk = plan.size == 0 ? k_chunk[small][dim][di]
+                                         : k_chunk_large[small][dtype == DLI_F16 ? 2 : dim];
+    rc = launch(chunk,
                 {static_cast<unsigned>((pair_rows + tile - 1) / tile), units,
                  static_cast<unsigned>(plan.splits)},
                 {256}, 0, stream, a);
   }
   if (rc != 0 || plan.splits == 1) return rc;
-  return launch(k_merge[di], {blocksFor(rows, 4)}, {256}, 0, stream, a);
+  return launch(k_merge[dim][di], {blocksFor(rows, 4)}, {256}, 0, stream, a);
 }
 
 }  // extern "C"

@@ -6,11 +6,11 @@
 //   S^T = K Q^T    elements as bf16 (T bf16 and fp32, whose q is the exact sum of three bf16 terms)
 //                  or f16 (T f16); the token's key scale multiplies the score in fp32.
 //   O^T += V^T P^T elements as f16, P as f16: one term (11 bits) where the output is bf16 (8 bits),
-//                  two terms (22 bits) else. A probability is 2^13 at the running reference, at most
-//                  2^15, so that f16's normal range covers 2^-27 of the largest; it carries the token's
-//                  value scale relative to the largest seen, which the running output is kept in.
-// A token's scales stand one to a lane and reach the 16 lanes of a row as DPP operands of the
-// multiplications. A token whose row was not finite (scale 255) makes the score NaN, so rows that
+//                  two terms (22 bits) else. A probability is 2^11 at the running reference and at most
+//                  2^15.5, so that f16's normal range reaches down to 2^-25 of the reference. The token's
+//                  value scale, relative to the largest seen, goes into P (few rows) or V (many); the
+//                  running output is kept in units of that largest scale.
+// A token whose row was not finite (scale 255) makes the score NaN, so rows that
 // see it are NaN and rows that do not see it are untouched.
 #include "kv_fp8.h"
 #include "skinny.h"
@@ -20,8 +20,9 @@ using namespace dk;
 namespace {
 
 constexpr int kTileK = 64;
-// log2 of a probability at the running reference, and what the reference lags behind at most
-constexpr float kLift = 13.f, kSlack = 2.f;
+// log2 of a probability at the running reference, and what the reference lags behind at most: a lag of
+// 2 (and 2^13 at the reference) moves it more often, 53.8 us for 4 x 2048 prompt tokens (52.2)
+constexpr float kLift = 11.f, kSlack = 4.5f;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
@@ -135,6 +136,9 @@ __device__ __forceinline__ uint32_t waveMaxU(uint32_t v) {
   }
   return v;
 }
+
+// In a branch that is seldom taken: keeps the compiler from computing both sides and selecting.
+__device__ __forceinline__ void rarely() { asm volatile(""); }
 
 // Bytes i < 16 of w whose bit i is clear become 0.
 __device__ __forceinline__ void keepBytes(U128& w, uint32_t bits) {
@@ -441,20 +445,31 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // the scores come out as 16 consecutive keys a lane, and V^T [dim][key] as it lies in the page, its 16-byte
 // chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks.
 // ---------------------------------------------------------------------------------------------
-constexpr int kChunkThreads = 256;
+constexpr int kChunkWaves = 4;
 // exponent of a staged value's factor at the largest value scale: elements reach 448 * 2^7 there, and a
 // token's elements stay exact in f16 down to 2^-22 of that scale
 constexpr int kValueLift = 7;
 constexpr float kNoReference = 1e30f;
 
-__device__ __forceinline__ int valueChunk(int d, int chunk) {
-  return d * kTileK + (chunk ^ ((d >> 1) & 7)) * 8;
+// Places of 16-byte chunks (8 elements) in LDS. A ds_read_b128 serves 16 lanes a cycle: lanes 0-3,
+// 12-15 and 20-27 together, then 4-11, 16-19 and 28-31, and the upper half alike (found by timing pairs
+// of lanes on one bank). With r the row of a fragment read and g or g + 4 st the chunk, chunk ^ r over rows
+// of 16 chunks and chunk ^ r / 2 over rows of 8 put those lanes on distinct banks.
+template <int D>
+__device__ __forceinline__ int keyChunk(int row, int chunk) {
+  return row * D + (chunk ^ (D == 128 ? row & 15 : (row >> 1) & 7)) * 8;
+}
+// keys 8 half .. 8 half + 7 of the run of 16
+__device__ __forceinline__ int valueChunk(int d, int run, int half) {
+  return d * kTileK + ((run + 4 * half) ^ ((d >> 1) & 7)) * 8;
 }
 
 // 2^(code - top + kValueLift) as f16, 0 below its least subnormal
 __device__ __forceinline__ uint16_t valueFactorF16(uint32_t code, uint32_t top) {
-  const int e = static_cast<int>(code) - static_cast<int>(top) + kValueLift + 15;
-  return static_cast<uint16_t>(e > 0 ? e << 10 : e > -10 ? 1 << (9 + e) : 0);
+  int e = 127 + kValueLift + static_cast<int>(code) - static_cast<int>(top);
+  e = e > 0 ? e : 0;
+  return __builtin_bit_cast(uint16_t,
+                            static_cast<f16>(__uint_as_float(static_cast<uint32_t>(e) << 23)));
 }
 
 // 8 value codes times their tokens' factors
@@ -472,24 +487,23 @@ __device__ __forceinline__ U128 scaledKey(uint32_t w0, uint32_t w1, float scale)
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true))};
 }
 
-template <class T, int D>
+template <int D>
 struct ChunkLds {
-  static constexpr int kPitch = D + 8;  // 16 rows start on 16 distinct groups of 4 banks
-  uint16_t k[2][kTileK * kPitch];
+  uint16_t k[2][kTileK * D];
   uint16_t v[2][D * kTileK];
-  float kf[4][kTileK];     // each wave's own copy of the tile's key scales
-  uint16_t vf[4][kTileK];  // and of the value factors
+  float kf[kChunkWaves][kTileK];     // each wave's own copy of the tile's key scales
+  uint16_t vf[kChunkWaves][kTileK];  // and of the value factors
 };
 
 template <class T, int D, int QB, bool kSmall>
 __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   using Ty = Kv8Type<T>;
-  using Lds = ChunkLds<T, D>;
   // f16 keys stay unscaled (their range would not hold a scaled one), the score takes the scale
   constexpr bool kScaleKeys = !__is_same(T, f16);
-  constexpr int DT = D / 16, DK = D / 32, kPer = D / 64;
-  constexpr int kParts = D / 16;  // 16-code chunks of a key
-  __shared__ __attribute__((aligned(16))) Lds lds;
+  constexpr int DT = D / 16, DK = D / 32, kThreads = kChunkWaves * kWave, kRows = 16 * QB * kChunkWaves;
+  constexpr int kParts = D / 16;         // 16-code chunks of a key
+  constexpr int kPer = 4 * D / kThreads;  // chunks of K, and of V^T, a thread
+  __shared__ __attribute__((aligned(16))) ChunkLds<D> lds;
   const Kv8Pages& pg = a.pages;
   const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int r = lane % 16, g = lane / 16;
@@ -498,7 +512,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   // one, last tile first: under a causal mask the longest workgroups start first
   const uint32_t lin = blockIdx.x + gridDim.x * blockIdx.y;
   const int pair = static_cast<int>(lin % gridDim.y), b = pair / pg.heads, kvh = pair - b * pg.heads;
-  const int p0 = static_cast<int>(gridDim.x - 1 - lin / gridDim.y) * 64 * QB;
+  const int p0 = static_cast<int>(gridDim.x - 1 - lin / gridDim.y) * kRows;
   const int pw = p0 + wave * 16 * QB;  // the wave's first row
   const bool active = pw < rows;       // uniform over the wave
   const int64_t past = kv8First(pg, b);
@@ -514,7 +528,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     for (int c = 0; c < DK; ++c) queryFragment<T>(q + c * 32, qf[qb][c]);
     lim[qb] = visibleKeys(a, past, at.i);
   }
-  const int wg_keys = visibleKeys(a, past, clamped(p0 + 64 * QB - 1) / group);
+  const int wg_keys = visibleKeys(a, past, clamped(p0 + kRows - 1) / group);
   const int wave_full = visibleKeys(a, past, clamped(pw) / group);  // keys every row of the wave sees
 
   const int all_tiles = (wg_keys + kTileK - 1) / kTileK;
@@ -522,67 +536,91 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   const int kt0 = static_cast<int>(blockIdx.z) * per;
   const int kt1 = kt0 + per < all_tiles ? kt0 + per : all_tiles;
 
-  // page ids of a tile's four runs of 16 keys (one page where pages are not small)
+  // Where a tile lies: the page ids of its four runs of 16 keys (one page where pages are not small),
+  // -1 for a page that holds nothing, and its first slot. Tiles past the last one repeat it; runs past
+  // the pages repeat the last one and are masked.
+  struct Where {
+    int id[4];
+    int slot;
+  };
   const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
-  const uint32_t last_run = static_cast<uint32_t>((a.capacity - 1) / 16);
-  const uint32_t runs_per_page = static_cast<uint32_t>(bs) / 16;
-  int id[4];
-  auto loadIds = [&](int kt) {  // runs past the pages repeat the last one and are masked
+  const int kt_last = kt1 - 1;
+  const int tiles_per_page = kSmall ? 1 : bs / kTileK;
+  const int last_run = static_cast<int>((a.capacity - 1) / 16), run_shift = bs == 32 ? 1 : 0;
+  int next_kt = kt0, next_page = kSmall ? 0 : kt0 / tiles_per_page;
+  int next_slot = kSmall ? 0 : (kt0 - next_page * tiles_per_page) * kTileK;
+  Where coming;  // as loaded
+  auto loadIds = [&] {  // of tile next_kt, which then moves on
 #pragma unroll
     for (int u = 0; u < (kSmall ? 4 : 1); ++u) {
-      uint32_t run = static_cast<uint32_t>(kt) * 4 + u;
-      run = run < last_run ? run : last_run;
-      const int x = gp(table)[run / runs_per_page];
-      id[u] = x < pg.num_blocks ? x : -1;
+      int page = next_page;
+      if constexpr (kSmall) {
+        const int run = next_kt * 4 + u;
+        page = (run < last_run ? run : last_run) >> run_shift;
+      }
+      coming.id[u] = gp(table)[page];
     }
-    if (!kSmall) id[1] = id[2] = id[3] = id[0];
+    coming.slot = next_slot;
+    if (next_kt < kt_last) {
+      ++next_kt;
+      next_slot += kTileK;
+      if (next_slot >= bs) {
+        next_slot = 0;
+        ++next_page;
+      }
+    }
   };
-  auto pick = [&](int u) { return u == 0 ? id[0] : u == 1 ? id[1] : u == 2 ? id[2] : id[3]; };
+  auto takeIds = [&] {  // once they are there; the same in every lane
+    Where w = coming;
+#pragma unroll
+    for (int u = 0; u < (kSmall ? 4 : 1); ++u) {
+      const int x = __builtin_amdgcn_readfirstlane(coming.id[u]);
+      w.id[u] = x < pg.num_blocks ? x : -1;
+    }
+    return w;
+  };
+  auto pick = [&](const Where& w, int u) {
+    return !kSmall || u == 0 ? w.id[0] : u == 1 ? w.id[1] : u == 2 ? w.id[2] : w.id[3];
+  };
   auto headOf = [&](int page) {  // a page that holds nothing: page 0 is read in its place and masked
     return static_cast<int64_t>(page < 0 ? 0 : page) * pg.heads + kvh;
   };
   // offsets of this thread's chunks within a page's head
   const int64_t head = static_cast<int64_t>(bs) * D;
   uint32_t ko[kPer], vo[kPer];
+  auto chunkOf = [&](int i) { return t + i * kThreads; };
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int c = t + i * kChunkThreads;
+    const int c = chunkOf(i);
     ko[i] = kSmall ? static_cast<uint32_t>(c / kParts % bs * D + c % kParts * 16)
                    : static_cast<uint32_t>(c * 16);
     vo[i] = static_cast<uint32_t>(c / 4) * static_cast<uint32_t>(bs) +
             static_cast<uint32_t>(kSmall ? 16 * (c % 4) % bs : 16 * (c % 4));
   }
+  // A tile's codes on their way to LDS, and the scales of this lane's key.
   U128 kr[kPer], vr[kPer];
   uint32_t kc = 0, vc = 0;
   bool in_page = false;
-  auto fetch = [&](int kt) {
-    if constexpr (kSmall) {
+  auto fetchScales = [&](const Where& w) {
+    const int page = pick(w, g);
+    in_page = page >= 0;
+    const uint8_t* sb = pg.scales + headOf(page) * 2 * bs + (kSmall ? 0 : w.slot);
+    const uint32_t at = static_cast<uint32_t>(kSmall ? lane % bs : lane);
+    kc = gp(sb)[at];
+    vc = gp(sb + bs)[at];
+  };
+  auto fetchKeys = [&](const Where& w) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int c = t + i * kChunkThreads;
-        kr[i] = gload16(pg.key + headOf(pick(c / kParts / 16)) * head + ko[i]);
-        vr[i] = gload16(pg.value + headOf(pick(c % 4)) * head + vo[i]);
-      }
-      const int page = pick(g);
-      in_page = page >= 0;
-      const uint8_t* sb = pg.scales + headOf(page) * 2 * bs + lane % bs;
-      kc = gp(sb)[0];
-      vc = gp(sb)[bs];
-    } else {
-      const uint32_t slot = static_cast<uint32_t>(kt) % (runs_per_page / 4) * kTileK;
-      const int64_t hb = headOf(id[0]);
-      const uint8_t* kb = pg.key + hb * head + static_cast<int64_t>(slot) * D;
-      const uint8_t* vb = pg.value + hb * head + slot;
-      const uint8_t* sb = pg.scales + hb * 2 * bs + slot;
-      in_page = id[0] >= 0;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        kr[i] = gload16(kb + ko[i]);
-        vr[i] = gload16(vb + vo[i]);
-      }
-      kc = gp(sb)[lane];
-      vc = gp(sb + bs)[lane];
+    for (int i = 0; i < kPer; ++i) {
+      const uint8_t* kb = pg.key + headOf(pick(w, (chunkOf(i)) / kParts / 16)) * head +
+                          (kSmall ? 0 : static_cast<int64_t>(w.slot) * D);
+      kr[i] = gload16(kb + ko[i]);
     }
+  };
+  auto fetchValues = [&](const Where& w) {
+    const uint8_t* vb = pg.value + headOf(pick(w, t % 4)) * head + (kSmall ? 0 : w.slot);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) vr[i] = gload16(vb + vo[i]);
   };
 
   f32x4 o[QB][DT];
@@ -600,10 +638,17 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
   const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
   const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
 
+  Where at{};
+  auto fetch = [&] {
+    at = takeIds();
+    loadIds();
+    fetchScales(at);
+    fetchKeys(at);
+    fetchValues(at);
+  };
   if (kt0 < kt1) {
-    loadIds(kt0);
-    fetch(kt0);
-    loadIds(kt0 + 1);
+    loadIds();
+    fetch();
   }
   for (int kt = kt0; kt < kt1; ++kt) {
     const int k0 = kt * kTileK, buf = kt & 1;
@@ -625,36 +670,40 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     if constexpr (kScaleKeys) lds.kf[wave][lane] = kf;
     lds.vf[wave][lane] = valueFactorF16(vcode, top);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' factors are read below
-    const U128 vf0 = load16(&lds.vf[wave][16 * (t % 4)]), vf1 = load16(&lds.vf[wave][16 * (t % 4) + 8]);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int c = t + i * kChunkThreads;
+      const int c = chunkOf(i);
       const int key = c / kParts, part = c % kParts;
       // the score of row 4 g + i of the 16-key group kk is that of key 16 g + 4 kk + i
       const int row = 16 * (key % 16 / 4) + 4 * (key / 16) + key % 4;
-      U128* to = reinterpret_cast<U128*>(&lds.k[buf][row * Lds::kPitch + part * 16]);
       U128 k0v, k1v;
       if constexpr (kScaleKeys) {
         const float f = lds.kf[wave][key];
         k0v = scaledKey(kr[i][0], kr[i][1], f);
         k1v = scaledKey(kr[i][2], kr[i][3], f);
-        if (bads != 0 && (bads >> key & 1)) k0v = k1v = U128{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+        if (bads != 0) {
+          rarely();
+          if (bads >> key & 1) k0v = k1v = U128{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+        }
       } else {
         k0v = keyFragment<T>(kr[i][0], kr[i][1]);
         k1v = keyFragment<T>(kr[i][2], kr[i][3]);
       }
-      to[0] = k0v;
-      to[1] = k1v;
-      const int d = c / 4, run = c % 4;
-      if (lives != ~uint64_t{0}) keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
-      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, 2 * run)]) = valueFragment(vr[i][0], vr[i][1], vf0);
-      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, 2 * run + 1)]) =
-          valueFragment(vr[i][2], vr[i][3], vf1);
+      *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(row, 2 * part)]) = k0v;
+      *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(row, 2 * part + 1)]) = k1v;
     }
-    if (kt + 1 < kt1) {
-      fetch(kt + 1);
-      loadIds(kt + 2);
+    const U128 vf0 = load16(&lds.vf[wave][16 * (t % 4)]), vf1 = load16(&lds.vf[wave][16 * (t % 4) + 8]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int d = chunkOf(i) / 4, run = t % 4;
+      if (lives != ~uint64_t{0}) {
+        rarely();
+        keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
+      }
+      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, run, 0)]) = valueFragment(vr[i][0], vr[i][1], vf0);
+      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, run, 1)]) = valueFragment(vr[i][2], vr[i][3], vf1);
     }
+    fetch();
     // one barrier a tile: the other buffer was last read before the previous one
     __syncthreads();
     if (!active) continue;
@@ -666,7 +715,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
       for (int qb = 0; qb < QB; ++qb) s[qb][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < DK; ++c) {
-        const U128 ka = load16(&lds.k[buf][(kk * 16 + r) * Lds::kPitch + c * 32 + g * 8]);
+        const U128 ka = load16(&lds.k[buf][keyChunk<D>(kk * 16 + r, 4 * c + g)]);
 #pragma unroll
         for (int u = Ty::kQ - 1; u >= 0; --u)
 #pragma unroll
@@ -714,7 +763,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
         for (int qb = 0; qb < QB; ++qb) ls[qb] = F16::mma(ones, pf[qb][u][st], ls[qb]);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
-        const U128 va = load16(&lds.v[buf][valueChunk(16 * dt + r, 2 * g + st)]);
+        const U128 va = load16(&lds.v[buf][valueChunk(16 * dt + r, g, st)]);
 #pragma unroll
         for (int u = Ty::kP - 1; u >= 0; --u)
 #pragma unroll
@@ -755,33 +804,55 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Rows of any number: the splits' results of row blockIdx.x * 4 + wave joined.
+// The splits' results of a row joined, one wave a row: every lane's loads go out before the first is
+// used (a merge is a launch and one trip to memory). D / 4 lanes hold a split's row, 256 / D splits are
+// read at a time, their sums joined at the end in a fixed order.
 // ---------------------------------------------------------------------------------------------
-template <class T>
-__device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a, int D) {
-  const int lane = threadIdx.x % kWave;
+template <class T, int D>
+__device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
+  constexpr int kLanes = D / 4, kAtOnce = kWave / kLanes, kDepth = 8;
+  const int lane = threadIdx.x % kWave, mine = lane / kLanes, d = 4 * (lane % kLanes);
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / kWave;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.seq_q;
-  if (row >= rows) return;
+  if (row >= static_cast<int64_t>(a.batch) * a.q_heads * a.seq_q) return;
+  const float* ml = a.part_ml + row * a.splits * 2;
+  const float* o = a.part_o + row * a.splits * D + d;
+  const bool have = lane < a.splits;
+  const float m = have ? gp(ml)[2 * lane] : -INFINITY, l = have ? gp(ml)[2 * lane + 1] : 0.f;
+  f32x4 x[kDepth];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int s = s0 + u * kAtOnce + mine;
+      x[u] = s < a.splits ? *gp(reinterpret_cast<const f32x4*>(o + static_cast<int64_t>(s) * D))
+                          : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  load(0);
+  const float M = waveMax(m);
+  // no key, or none of any weight: 0; a NaN sum stays one whatever its maximum
+  const float f = (m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M)) * l;
+  const float L = waveSum(f);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < a.splits; s0 += kDepth * kAtOnce) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int u = 0; u < kDepth; ++u) {
+      const int s = s0 + u * kAtOnce + mine;
+      const float w = __shfl(f, s % kWave, kWave);
+      if (s < a.splits) acc += x[u] * w;
+    }
+  }
+#pragma unroll
+  for (int off = kLanes; off < kWave; off *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], off, kWave);
+  if (mine != 0) return;
   const int i = static_cast<int>(row % a.seq_q);
   const int64_t bh = row / a.seq_q, b = bh / a.q_heads;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, gp(a.part_ml)[(row * a.splits + s) * 2]);
-  float L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t part = row * a.splits + s;
-    const float m = gp(a.part_ml)[part * 2], l = gp(a.part_ml)[part * 2 + 1];
-    const float f = (m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M)) * l;
-    L += f;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (lane + u * kWave < D) acc[u] = fmaf(f, gp(a.part_o)[part * D + lane + u * kWave], acc[u]);
-  }
   const RowAt at = {i, static_cast<int>(bh % a.q_heads)};
+  T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + d;
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    if (lane + u * kWave < D)
-      st(static_cast<T*>(a.out) + outAt(a, b, at, D) + lane + u * kWave, L == 0.f ? 0.f : acc[u] / L);
+  for (int u = 0; u < 4; ++u) st(out + u, L == 0.f ? 0.f : acc[u] / L);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -853,14 +924,15 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
 
 }  // namespace
 
-#define KV8_CHUNK(suffix, T, D, QB)                                                             \
-  extern "C" __global__ void __launch_bounds__(kChunkThreads, 2)                                \
-      kv8_chunk_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                                   \
-    kv8_chunk<T, D, QB, false>(a);                                                              \
+// 64 or 128 rows a workgroup
+#define KV8_CHUNK(suffix, T, D, ROWS)                                                           \
+  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, 2)                           \
+      kv8_chunk_d##D##_r##ROWS##_##suffix(Kv8AttentionArgs a) {                                 \
+    kv8_chunk<T, D, ROWS / 64, false>(a);                                                       \
   }                                                                                             \
-  extern "C" __global__ void __launch_bounds__(kChunkThreads, 2)                                \
-      kv8_chunk_small_d##D##_q##QB##_##suffix(Kv8AttentionArgs a) {                             \
-    kv8_chunk<T, D, QB, true>(a);                                                               \
+  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, 2)                           \
+      kv8_chunk_small_d##D##_r##ROWS##_##suffix(Kv8AttentionArgs a) {                           \
+    kv8_chunk<T, D, ROWS / 64, true>(a);                                                        \
   }
 
 #define KV8_ATTENTION(suffix, T)                                                                \
@@ -880,17 +952,28 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
       kv8_decode_small_d128_##suffix(Kv8AttentionArgs a) {                                      \
     kv8_decode<T, 128, true>(a);                                                                \
   }                                                                                             \
-  extern "C" __global__ void __launch_bounds__(256) kv8_merge_##suffix(Kv8AttentionArgs a) {    \
-    kv8_merge<T>(a, a.pages.head_dim);                                                          \
+  extern "C" __global__ void __launch_bounds__(256) kv8_merge_d64_##suffix(Kv8AttentionArgs a) { \
+    kv8_merge<T, 64>(a);                                                                        \
+  }                                                                                             \
+  extern "C" __global__ void __launch_bounds__(256)                                             \
+      kv8_merge_d128_##suffix(Kv8AttentionArgs a) {                                             \
+    kv8_merge<T, 128>(a);                                                                       \
   }                                                                                             \
   extern "C" __global__ void __launch_bounds__(64) kv8_rows_##suffix(Kv8AttentionArgs a) {      \
     kv8_rows<T>(a);                                                                             \
-  }                                                                                             \
-  KV8_CHUNK(suffix, T, 64, 1)                                                                   \
-  KV8_CHUNK(suffix, T, 64, 2)                                                                   \
-  KV8_CHUNK(suffix, T, 128, 1)                                                                  \
-  KV8_CHUNK(suffix, T, 128, 2)
+  }
 
 KV8_ATTENTION(f32, float)
 KV8_ATTENTION(bf16, bf16)
 KV8_ATTENTION(f16, f16)
+
+// attentionPlan (csrc/hip/kv_fp8_ops.cc) chooses the rows
+KV8_CHUNK(f32, float, 64, 64)
+KV8_CHUNK(f32, float, 128, 64)
+KV8_CHUNK(bf16, bf16, 64, 64)
+KV8_CHUNK(bf16, bf16, 64, 128)
+KV8_CHUNK(bf16, bf16, 128, 64)
+KV8_CHUNK(bf16, bf16, 128, 128)
+KV8_CHUNK(f16, f16, 64, 64)
+KV8_CHUNK(f16, f16, 128, 64)
+KV8_CHUNK(f16, f16, 128, 128)

@@ -148,7 +148,8 @@ def check_attention(out, want, dtype, keys, dim):
     argument, which moves a weight by that share and its sum likewise; the outputs' fp32 sums run
     over at most 4 steps a 64-key tile and the joins. f16's least step is 2^-24, so a weight (and the
     rest of one in two terms) is off by up to 2^-25 in any case; the row's sum of weights is at least
-    2^13 in those units and an element's factor at most the largest value scale: 2^-38 of the level."""
+    2^11 in those units (its reference's own weight) and an element's factor at most the largest value
+    scale: 2^-36 of the level."""
     value, mag, spread, level = want
     got = out.double().cpu().numpy()
     half = torch.finfo(dtype).eps / 2
@@ -157,7 +158,7 @@ def check_attention(out, want, dtype, keys, dim):
     score = 2 * (dim + 8) * 2.0 ** -24 * (spread + 30)
     sums = (4 * (keys / 64) + 96) * 2.0 ** -24
     bound = half * np.abs(value) + (1 + half) * (weight + score + sums) * mag + tiny
-    bound += 2.0 ** -38 * level
+    bound += 2.0 ** -36 * level
     nan = np.isnan(value)
     assert np.array_equal(np.isnan(got), nan)
     over = np.abs(np.nan_to_num(value)) > (1 + half) * torch.finfo(dtype).max
