@@ -131,7 +131,12 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
     return {0, 0, 1};
   const int64_t tiles = (block_size * max_blocks + 63) / 64;
   if (rows <= 16) {
-    // about one workgroup of 8 waves per CU, each wave with a tile at least
+    // About one workgroup of 8 waves per CU, each wave with a tile at least. Joining the splits is a
+    // launch of its own, which costs more than two tiles to a wave: 1000 tokens of one sequence (14 / 2
+    // heads x 64) 7.6 us undivided and 8.9 in 2 splits; 8 x 2000 (28 / 4 x 128) 18.6, 15.5 and, in 4, 12.2.
+    // (Joined by the split that arrives last, in the same launch: 13.1 us for 32 x 4096 where two
+    // launches take 12.6, and 20.6 for 16 splits where they take 11.5.)
+    if (tiles <= 16) return {1, 0, 1};
     int64_t splits = (256 + units - 1) / units;
     const int64_t most = (tiles + 7) / 8;
     splits = splits < most ? splits : most;
@@ -293,7 +298,8 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
       !aligned16(key_codes) || !aligned16(value_codes))
     plan = {0, 0, 1};
   while (plan.splits > 1 &&
-         (workspace == nullptr || workspace_bytes < partBytes(rows, head_dim, plan.splits)))
+         (workspace == nullptr || !aligned16(workspace) ||
+          workspace_bytes < partBytes(rows, head_dim, plan.splits)))
     --plan.splits;
   a.q = q;
   a.out = out;

@@ -203,6 +203,18 @@ __device__ __forceinline__ int64_t outAt(const Kv8AttentionArgs& a, int64_t b, R
 // ---------------------------------------------------------------------------------------------
 constexpr int kDecWaves = 8;
 
+// Loads of lines that are read once. They pay where an instruction covers whole 128-byte lines: V's
+// rows of 64 keys stand one behind the other, and so do 4 rows of K with head_dim 64; with 128 an
+// instruction takes half of each line of K. 64 sequences of 8192 tokens (28 / 4 heads x 128): 91.6 us with
+// cached loads, 83.4 with V streamed, 84.2 with K too; 32 of 4096 (14 / 2 x 64) 14.0, 14.0 and 13.1.
+__device__ __forceinline__ U128 streamed16(const uint8_t* p) {
+  return __builtin_nontemporal_load(gp(reinterpret_cast<const U128*>(p)));
+}
+template <int D>
+__device__ __forceinline__ U128 keyLoad(const uint8_t* p) {
+  return D == 64 ? streamed16(p) : gload16(p);
+}
+
 // A tile's codes and this lane's key's scales; ids of its pages, -1 where a page holds nothing
 template <int D>
 struct KeyTile {
@@ -234,22 +246,21 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   const int bs = pg.block_size;
   const int stride = a.splits * kDecWaves, first = blockIdx.x * kDecWaves + wave;
   const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
-  const int64_t past = kv8First(pg, b);
-  const int most = visibleKeys(a, past, a.seq_q - 1);
-  const int tiles = (most + kTileK - 1) / kTileK;
-
   // Page ids, a lane each: of kIds tiles of this wave (kSmall: 4 runs of 16 keys a tile).
   constexpr int kIds = kSmall ? 16 : 64;
   int ids = -1;
   auto loadIds = [&](int ordinal) {  // of the tiles ordinal .. ordinal + kIds - 1
-    const int tile = first + (ordinal + (kSmall ? lane / 4 : lane)) * stride;
+    const int64_t tile = first + static_cast<int64_t>(ordinal + (kSmall ? lane / 4 : lane)) * stride;
+    const int64_t key = tile * kTileK + (kSmall ? 16 * (lane % 4) : 0);
     ids = -1;
-    if (tile < tiles) {
-      const int64_t key = static_cast<int64_t>(tile) * kTileK + (kSmall ? 16 * (lane % 4) : 0);
-      if (key < a.capacity) ids = gp(table)[key / bs];
-    }
+    // whatever the sequence holds: the ids are on their way while its position is
+    if (key < a.capacity) ids = gp(table)[static_cast<uint32_t>(key) / static_cast<uint32_t>(bs)];
     if (ids >= pg.num_blocks) ids = -1;
   };
+  loadIds(0);
+  const int64_t past = kv8First(pg, b);
+  const int most = visibleKeys(a, past, a.seq_q - 1);
+  const int tiles = (most + kTileK - 1) / kTileK;
   KeyTile<D> buf[2];
   auto fetch = [&](KeyTile<D>& x, int tile, int ordinal) {
     const int64_t head = static_cast<int64_t>(bs) * D;
@@ -278,12 +289,11 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int j = 0; j < J; ++j) x.k[kk][j] = gload16(kb + 4 * kk * D + 64 * j);
+      for (int j = 0; j < J; ++j) x.k[kk][j] = keyLoad<D>(kb + 4 * kk * D + 64 * j);
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) x.v[dt] = gload16(vb + static_cast<int64_t>(16 * dt) * bs);
+    for (int dt = 0; dt < DT; ++dt) x.v[dt] = streamed16(vb + static_cast<int64_t>(16 * dt) * bs);
   };
 
-  if (first < tiles) loadIds(0);
   // q: rows past the last are zero and not stored
   U128 qf[J][2][Ty::kQ];
 #pragma unroll

@@ -208,7 +208,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 
 def current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the raw stream of the current device, without the Stream object of torch.cuda.current_stream()
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def call(name: str, *args) -> int:

@@ -239,6 +239,39 @@ def test_attention(dtype, q_heads, heads, dim, block, seq, past, causal):
     assert torch.equal(rows.transpose(1, 2), split)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("q_heads,heads,dim,block", [(14, 2, 64, 64), (8, 1, 128, 16), (4, 2, 64, 32),
+                                                     (3, 1, 128, 192)])
+@pytest.mark.parametrize("seq,past", [(1, [2303, 40]), (1, [-1, 1471]), (2, [1100, 2302]),
+                                      (19, [2285, 7]), (33, [-40, 1300])])
+def test_long_contexts(dtype, q_heads, heads, dim, block, seq, past):
+    """Keys split over workgroups: sequences that fill all splits, few of them, none."""
+    t = DTYPES[dtype]
+    pools = Pools(2, heads, dim, block, 2304 // block, seed=seq)
+    q = torch.randn((2, q_heads, seq, dim), generator=rng(seq + 1)).to(t)
+    cache = pools.oracle()
+    pools.cuda()
+    ws = workspace(pools, q)
+    assert ws.numel() > 0
+    out = attend(pools, q.cuda(), past, ws=ws)
+    check_attention(out, cache.attention(q.double().numpy(), past, True, dim ** -0.5), t, 2304, dim)
+    # a workspace that holds fewer splits, or none
+    for part in (ws[:ws.numel() // 2], ws[:8], ws[1:]):
+        other = attend(pools, q.cuda(), past, ws=part)
+        check_attention(other, cache.attention(q.double().numpy(), past, True, dim ** -0.5), t, 2304, dim)
+
+
+@pytest.mark.parametrize("dim,q_heads,seq", [(64, 7, 1), (128, 16, 1), (64, 2, 10), (128, 1, 17)])
+def test_many_splits(dim, q_heads, seq):
+    """The most splits that a call may have, with a page that holds nothing among them."""
+    pools = Pools(1, 1, dim, 64, 300, missing=[(0, 100, -1)])
+    q = torch.randn((1, q_heads, seq, dim), generator=rng(1)).bfloat16()
+    cache = pools.oracle()
+    out = attend(pools.cuda(), q.cuda(), 19000, ws=workspace(pools, q))
+    check_attention(out, cache.attention(q.double().numpy(), [19000], True, dim ** -0.5), torch.bfloat16,
+                    19200, dim)
+
+
 @pytest.mark.parametrize("seq,q_heads", [(1, 7), (40, 7)])
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1.5])
 def test_attention_scales(seq, q_heads, scale):
