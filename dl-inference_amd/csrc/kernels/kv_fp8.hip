@@ -42,7 +42,7 @@ template <class T, int D, int kTokens, bool kRope>
 __device__ __forceinline__ void kv8_write(const Kv8WriteArgs& a) {
   constexpr int kGroups = D / 64;       // 16-element groups of a thread
   constexpr int kRuns = kTokens / 16;   // runs of 16 tokens in a tile
-  constexpr int kPitch = kTokens + 16;  // bytes between dims in LDS
+  constexpr int kPitch = kTokens + 8;  // bytes between dims in LDS: a quad's rows start on other banks
   __shared__ __attribute__((aligned(16))) uint8_t vs[D * kPitch];
   const Kv8Pages& p = a.pages;
   const int t = threadIdx.x, tok = t / 4, part = t % 4;
@@ -157,7 +157,9 @@ __device__ __forceinline__ void kv8_write(const Kv8WriteArgs& a) {
     const uint8_t* from = &vs[e * kPitch + 16 * (t % kRuns)];
     uint8_t* to = p.value + ((run_page * p.heads + h) * D + e) * p.block_size + slot;
     if (whole) {
-      *gp(reinterpret_cast<U32x4*>(to)) = *reinterpret_cast<const U32x4*>(from);
+      const U32x2 a0 = *reinterpret_cast<const U32x2*>(from);
+      const U32x2 a1 = *reinterpret_cast<const U32x2*>(from + 8);
+      *gp(reinterpret_cast<U32x4*>(to)) = U32x4{a0[0], a0[1], a1[0], a1[1]};
     } else {
       for (int i = 0; i < 16; ++i)
         if (run + i >= low && run + i < high) gp(to)[i] = from[i];
@@ -238,7 +240,7 @@ __device__ __forceinline__ void kv8_write_any(const Kv8WriteArgs& a) {
 // One workgroup: kTokens tokens of one head's keys or values (grid.y) of sequence blockIdx.z.
 template <class T, int D, int kTokens>
 __device__ __forceinline__ void kv8_read_tile(const Kv8ReadArgs& a) {
-  constexpr int kGroups = D / 64, kRuns = kTokens / 16, kPitch = kTokens + 16;
+  constexpr int kGroups = D / 64, kRuns = kTokens / 16, kPitch = kTokens + 8;
   __shared__ __attribute__((aligned(16))) uint8_t vs[D * kPitch];
   const Kv8Pages& p = a.pages;
   const int t = threadIdx.x, tok = t / 4, part = t % 4;
@@ -273,9 +275,13 @@ __device__ __forceinline__ void kv8_read_tile(const Kv8ReadArgs& a) {
     const int64_t run_page = run >= 0 && run < capacity ? kv8Page(p, b, run) : -1;
     if (run_page >= 0) {
       const int64_t slot = run % p.block_size;
-      for (int e = t / kRuns; e < D; e += kTokens * 4 / kRuns)
-        *reinterpret_cast<U32x4*>(&vs[e * kPitch + 16 * (t % kRuns)]) = *gp(
-            reinterpret_cast<const U32x4*>(p.value + ((run_page * p.heads + h) * D + e) * p.block_size + slot));
+      for (int e = t / kRuns; e < D; e += kTokens * 4 / kRuns) {
+        const U32x4 v = *gp(reinterpret_cast<const U32x4*>(
+            p.value + ((run_page * p.heads + h) * D + e) * p.block_size + slot));
+        U32x2* to = reinterpret_cast<U32x2*>(&vs[e * kPitch + 16 * (t % kRuns)]);
+        to[0] = U32x2{v[0], v[1]};
+        to[1] = U32x2{v[2], v[3]};
+      }
     }
     __syncthreads();
     if (page >= 0) {

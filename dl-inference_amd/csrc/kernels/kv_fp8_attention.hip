@@ -226,6 +226,9 @@ struct KeyTile {
 
 template <class T, int D>
 struct DecodeLds {
+  // q's terms where there are several: in registers they would push the tiles out (fp32, head_dim 128,
+  // 64 sequences of 4096 tokens: 80.7 us with 43 registers spilled, 48.8 so)
+  U128 q[Kv8Type<T>::kQ > 1 ? D / 64 * 2 * Kv8Type<T>::kQ : 1][kWave];
   float m[kDecWaves][16];
   float l[kDecWaves][16];
   uint32_t top[kDecWaves];
@@ -295,6 +298,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   };
 
   // q: rows past the last are zero and not stored
+  constexpr bool kSharedQ = Ty::kQ > 1;
   U128 qf[J][2][Ty::kQ];
 #pragma unroll
   for (int j = 0; j < J; ++j)
@@ -312,6 +316,17 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) queryFragment<T>(q + 64 * j + 8 * half, qf[j][half]);
   }
+  if constexpr (kSharedQ) {
+    if (wave == 0) {
+#pragma unroll
+      for (int x = 0; x < J * 2 * Ty::kQ; ++x)
+        lds.q[x][lane] = qf[x / (2 * Ty::kQ)][x / Ty::kQ % 2][x % Ty::kQ];
+    }
+    __syncthreads();
+  }
+  auto query = [&](int at, int j, int half, int u) {
+    return kSharedQ ? lds.q[(j * 2 + half) * Ty::kQ + u][at] : qf[j][half][u];
+  };
   const int all_see = visibleKeys(a, past, 0);  // keys that every row sees
 
   float m = -INFINITY, l = 0.f;
@@ -322,6 +337,8 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 
   auto attend = [&](KeyTile<D>& x, int tile) {
     const int k0 = tile * kTileK;
+    int q_lane = lane;
+    if constexpr (kSharedQ) asm volatile("" : "+v"(q_lane));  // read per tile, not held in registers
     f32x4 s[4];
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
@@ -332,7 +349,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
         for (int half = 0; half < 2; ++half) {
           const U128 ka = keyFragment<T>(x.k[kk][j][2 * half], x.k[kk][j][2 * half + 1]);
 #pragma unroll
-          for (int u = Ty::kQ - 1; u >= 0; --u) s[kk] = keyMma<T>(ka, qf[j][half][u], s[kk]);
+          for (int u = Ty::kQ - 1; u >= 0; --u) s[kk] = keyMma<T>(ka, query(q_lane, j, half, u), s[kk]);
         }
     }
     const bool live = x.live && k0 + lane < most;
@@ -456,6 +473,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks.
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunkWaves = 4;
+constexpr int kAhead = 3;  // LDS fragments read before they are needed
 // exponent of a staged value's factor at the largest value scale: elements reach 448 * 2^7 there, and a
 // token's elements stay exact in f16 down to 2^-22 of that scale
 constexpr int kValueLift = 7;
@@ -719,19 +737,30 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     if (!active) continue;
 
     f32x4 s[QB][4];
+    U128 frag[kAhead + 1];
+    constexpr int kSteps = 4 * DK;
+    auto keyRead = [&](int i) {
+      return load16(&lds.k[buf][keyChunk<D>(i / DK * 16 + r, 4 * (i % DK) + g)]);
+    };
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
+    for (int i = 0; i < kAhead; ++i) frag[i] = keyRead(i);
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) s[qb][kk] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kSteps; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < kSteps) frag[(i + kAhead) % (kAhead + 1)] = keyRead(i + kAhead);
 #pragma unroll
-      for (int c = 0; c < DK; ++c) {
-        const U128 ka = load16(&lds.k[buf][keyChunk<D>(kk * 16 + r, 4 * c + g)]);
+      for (int qb = 0; qb < QB; ++qb)
+        if (i % DK == 0) s[qb][i / DK] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int u = Ty::kQ - 1; u >= 0; --u)
+      for (int u = Ty::kQ - 1; u >= 0; --u)
 #pragma unroll
-          for (int qb = 0; qb < QB; ++qb) s[qb][kk] = keyMma<T>(ka, qf[qb][c][u], s[qb][kk]);
-      }
+        for (int qb = 0; qb < QB; ++qb)
+          s[qb][i / DK] = keyMma<T>(frag[i % (kAhead + 1)], qf[qb][i % DK][u], s[qb][i / DK]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    auto valueRead = [&](int i) {
+      return load16(&lds.v[buf][valueChunk(16 * (i % DT) + r, g, i / DT)]);
+    };
     const bool full = lives == ~uint64_t{0} && k0 + kTileK <= wave_full;
     U128 pf[QB][Ty::kP][2];
 #pragma unroll
@@ -766,20 +795,20 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
       packWeights<Ty::kP>(s[qb], pf[qb]);
     }
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
+    for (int i = 0; i < kAhead; ++i) frag[i] = valueRead(i);
+#pragma unroll
+    for (int i = 0; i < 2 * DT; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < 2 * DT) frag[(i + kAhead) % (kAhead + 1)] = valueRead(i + kAhead);
 #pragma unroll
       for (int u = Ty::kP - 1; u >= 0; --u)
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) ls[qb] = F16::mma(ones, pf[qb][u][st], ls[qb]);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const U128 va = load16(&lds.v[buf][valueChunk(16 * dt + r, g, st)]);
-#pragma unroll
-        for (int u = Ty::kP - 1; u >= 0; --u)
-#pragma unroll
-          for (int qb = 0; qb < QB; ++qb) o[qb][dt] = F16::mma(va, pf[qb][u][st], o[qb][dt]);
-      }
+        for (int qb = 0; qb < QB; ++qb) {
+          if (i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][u][i / DT], ls[qb]);
+          o[qb][i % DT] = F16::mma(frag[i % (kAhead + 1)], pf[qb][u][i / DT], o[qb][i % DT]);
+        }
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
 
 #pragma unroll
