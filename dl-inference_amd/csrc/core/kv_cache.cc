@@ -70,8 +70,17 @@ void allocatePools(KVCacheEntry& e, DType dtype, int device_id) {
   }
 }
 
+// The kernels of quantised entries run on the current device.
+void requireCurrentDevice(const KVCacheEntry& e) {
+  int current = 0;
+  hipCheck(dli_hip_get_device(&current), "KV cache");
+  if (e.key_pool.deviceId() != current)
+    throw std::invalid_argument("KV cache: an 8-bit entry is used with its device current only");
+}
+
 void appendQuantized(const KVCacheEntry& e, const Tensor& key, const Tensor& value,
                      std::int64_t start, const Tensor* positions, void* stream) {
+  requireCurrentDevice(e);
   hipCheck(dli_hip_kv_append_fp8(
                hipDtype(key.dtype()), key.deviceData(), value.deviceData(),
                const_cast<void*>(e.key_pool.deviceData()), const_cast<void*>(e.value_pool.deviceData()),
@@ -304,6 +313,7 @@ std::pair<Tensor, Tensor> KVCache::read(const std::string& name, std::int64_t st
                             std::to_string(e->capacity()) + " per sequence");
   const std::vector<std::int64_t> shape{e->batch, e->heads, length, e->head_dim};
   if (e->quantized() && e->key_pool.isCuda()) {
+    requireCurrentDevice(*e);
     const StreamScope scope(stream_);
     std::pair<Tensor, Tensor> out{Tensor::cuda(dtype, shape, e->key_pool.deviceId()),
                                   Tensor::cuda(dtype, shape, e->key_pool.deviceId())};

@@ -49,6 +49,7 @@ DeviceKernel k_merge[2][3] = KV8_DIMS("kv_fp8_attention", "kv8_merge_", "");
 DeviceKernel k_rows[3] = KV8_DTYPES("kv_fp8_attention", "kv8_rows");
 
 constexpr int64_t kMostTokens = int64_t{1} << 30;  // of a sequence, and rows of a pair: 32-bit indexes
+constexpr int64_t kMostPairs = int64_t{1} << 40;   // of a call's tokens: products with heads stay in range
 constexpr int64_t kMostGrid = 65535;               // of a grid's y and z
 
 // What every call has in common; fills `pages`. 0, or the recorded error.
@@ -64,7 +65,7 @@ int pagesOf(const char* op, int dtype, const void* key_codes, const void* value_
     return badArg(op, "block_size, max_blocks and num_blocks must be positive");
   if (block_size >= kMostTokens || max_blocks >= kMostTokens || block_size * max_blocks >= kMostTokens)
     return badArg(op, "a sequence's pages must hold fewer than 2^30 tokens");
-  if (heads > kMostGrid / 2 || batch >= kMostTokens || seq >= kMostTokens)
+  if (heads > kMostGrid / 2 || batch >= kMostTokens || seq >= kMostTokens || batch * seq >= kMostPairs)
     return badArg(op, "batch, seq or heads too large");
   if (positions != nullptr && positions_dtype != DLI_I64 && positions_dtype != DLI_I32)
     return badArg(op, "positions must be int64 or int32");
@@ -315,7 +316,7 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
   a.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   const int di = dtypeIndex(dtype);
   if (plan.form == 0)
-    return launch(k_rows[di], {static_cast<unsigned>(rows)}, {64}, 0, stream, a);
+    return launch(k_rows[di], {static_cast<unsigned>(rows < 65536 ? rows : 65536)}, {64}, 0, stream, a);
   const int small = block_size % 64 == 0 ? 0 : 1, dim = dimIndex(head_dim);
   const unsigned units = static_cast<unsigned>(batch * kv_heads);
   int rc;

@@ -17,8 +17,12 @@ __device__ __forceinline__ uint32_t kv8Scale(uint32_t most) {
   return e == 255 ? 255u : static_cast<uint32_t>(c > 0 ? c : 0);
 }
 
+// Position of sequence b's first token. Cut to +-2^40, past any page and any number of tokens, so that
+// sums with it stay in range.
 __device__ __forceinline__ int64_t kv8First(const Kv8Pages& p, int64_t b) {
-  return p.positions != nullptr ? loadIndex(p.positions, p.pos64, b) : p.start;
+  constexpr int64_t kFar = int64_t{1} << 40;
+  const int64_t at = p.positions != nullptr ? loadIndex(p.positions, p.pos64, b) : p.start;
+  return at < -kFar ? -kFar : (at > kFar ? kFar : at);
 }
 
 // Page of position pos (0 <= pos < capacity) of sequence b, or -1: it holds nothing.

@@ -42,7 +42,8 @@ ENTRIES = ["append", "rope", "read", "attention"]
     dict(dim=0), dict(dim=257), dict(block=0), dict(block=-64), dict(max_blocks=0), dict(num_blocks=0),
     dict(num_blocks=-1), dict(positions=P, pdtype=hip.F32), dict(key_codes=None), dict(value_codes=None),
     dict(scales=None), dict(table=None), dict(a=None), dict(block=1 << 29, max_blocks=2),
-    dict(block=1 << 40, max_blocks=1 << 40), dict(batch=1 << 40), dict(seq=1 << 40), dict(heads=1 << 40)])
+    dict(block=1 << 40, max_blocks=1 << 40), dict(batch=1 << 40), dict(seq=1 << 40), dict(heads=1 << 40),
+    dict(batch=1 << 21, seq=1 << 20)])
 def test_refusals(entry, change):
     assert status(entry, **change) == -1
     name = {"attention": "paged_attention", "rope": "rope_append"}.get(entry, f"kv_{entry}")

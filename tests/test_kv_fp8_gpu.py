@@ -446,3 +446,68 @@ def test_another_stream():
     pools.check(cache)
     check_attention(out, cache.attention(q.double().cpu().numpy(), [99, 99], True, 0.125),
                     torch.float16, 256, 64)
+
+
+@pytest.mark.parametrize("dim,block", [(64, 64), (128, 16), (80, 64)])
+def test_positions_at_the_ends_of_their_range(dim, block):
+    """Tokens before and past the pages: dropped, read as zeros; a query past them sees every key."""
+    pools = Pools(2, 2, dim, block, 128 // block)
+    cache = pools.oracle()
+    pools.cuda()
+    ends = [-(1 << 63), (1 << 63) - 1]
+    for seq in (1, 20, 70):
+        k = torch.randn((2, 2, seq, dim), generator=rng(seq)).bfloat16().cuda()
+        append(pools, k, k, ends)
+        pools.check(cache)
+        for x in read(pools, seq, ends, torch.bfloat16):
+            assert (x == 0).all()
+        q = torch.randn((2, 4, seq, dim), generator=rng(seq + 1)).bfloat16()
+        check_attention(attend(pools, q.cuda(), ends),
+                        cache.attention(q.double().numpy(), [-200, 128], True, dim ** -0.5),
+                        torch.bfloat16, 128, dim)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("seq", [1, 20])
+def test_scores_far_below_zero(dtype, dim, seq):
+    """Every score between -2^118 and -2^112: the largest takes all the weight."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 2)
+    pools.key[:] = 0
+    pools.key[..., 0] = 0x78  # 256
+    pools.scales[:, :, 0] = 127
+    best = int(pools.table[0, 1])
+    pools.key[best, 0, 3, 0] = 0x48  # 4, at position 67
+    q = torch.zeros((1, 2, seq, dim), dtype=t)
+    q[..., 0] = -2.0 ** 110
+    cache = pools.oracle()
+    out = attend(pools.cuda(), q.cuda(), 100, scale=1.0)
+    want = torch.from_numpy(cache.rows(0, 67)[1][0]).to(t)
+    assert torch.equal(out.cpu(), want.expand(out.shape))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("seq", [1, 20])
+def test_values_near_the_largest(dim, seq):
+    """Sums of values that pass the largest number while their mean does not."""
+    pools = Pools(1, 1, dim, 64, 3)
+    pools.scales[:, :, 1] = torch.where(torch.arange(64) % 3 == 0, 247, 240).to(torch.uint8)
+    pools.value[:] = 0x74  # 192: 2^120 times it is 3/4 of 2^128
+    q = torch.randn((1, 3, seq, dim), generator=rng(8))
+    cache = pools.oracle()
+    for t in (torch.float32, torch.bfloat16):
+        x = q.to(t)
+        check_attention(attend(pools.cuda(), x.cuda(), 150),
+                        cache.attention(x.double().numpy(), [150], True, dim ** -0.5), t, 192, dim)
+
+
+def test_more_rows_than_workgroups():
+    """The row-by-row form goes on from row to row: the same rows in shorter calls, bit for bit."""
+    pools = Pools(3, 1, 8, 8, 9).cuda()
+    q = torch.randn((3, 2, 13000, 8), generator=rng(9)).bfloat16().cuda()
+    past = torch.tensor([0, 40, -6000], device="cuda")
+    whole = attend(pools, q, past)
+    for at in range(0, 13000, 6500):
+        part = attend(pools, q[:, :, at:at + 6500].contiguous(), past + at)
+        assert torch.equal(part, whole[:, :, at:at + 6500])
