@@ -144,10 +144,10 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
     return {1, 0, splits < 32 ? splits : 32};
   }
   // 128 rows share a staged tile where they still fill half the card. 64 and 128 rows, us: bf16, 2 x
-  // 300 tokens over 3000 (28 / 4 heads x 128, 136 workgroups of 128) 90 and 66; 1 x 2048 over 8192 484 and
-  // 347; 4 x 2048 tokens (14 / 2 x 64) 63 and 54. f16 holds its weights in two terms and pays from more
-  // workgroups on, with head_dim 128 only: 2 x 500 over 2000 80 and 87, 1 x 2000 over 3000 246 and 211, 4 x 1000
-  // over 500 (x 64) 45 and 47. fp32 (three terms of q) never: 92 and 113, 36 and 40.
+  // 300 tokens over 3000 (28 / 4 heads x 128, 136 workgroups of 128) 87 and 64; 1 x 2048 over 8192 465 and
+  // 339; 4 x 2048 tokens (14 / 2 x 64) 60 and 51. f16 holds its weights in two terms and pays from more
+  // workgroups on, with head_dim 128 only: 2 x 500 over 2000 77 and 84, 1 x 2000 over 3000 235 and 209,
+  // 4 x 1000 over 500 (x 64) 45 and 47. fp32 (three terms of q) never: 92 and 113, 36 and 40.
   const int64_t large = units * ((rows + 127) / 128);
   const int size = dtype == DLI_BF16  ? large >= 128
                    : dtype == DLI_F16 ? large >= 384 && head_dim == 128
@@ -156,7 +156,7 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
   const int64_t blocks = units * ((rows + tile_rows - 1) / tile_rows);
   // keys split until two workgroups stand on every CU, each with 4 tiles at least; a split's results
   // are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4 heads
-  // x 128: 41 us, 65 in two splits)
+  // x 128: 37 us, 61 in two splits)
   int64_t splits = 512 / blocks;
   const int64_t most = tiles / 4;
   splits = splits < most ? splits : most;

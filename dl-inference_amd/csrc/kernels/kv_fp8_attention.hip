@@ -200,6 +200,11 @@ __device__ __forceinline__ int64_t outAt(const Kv8AttentionArgs& a, int64_t b, R
 // V the dims 16 dt + r at the keys 16 g. The order in which the MFMA takes dims and keys is free as
 // long as both operands share it, so those runs are its fragments as they come, and the scores come
 // out as 16 consecutive keys a lane: V's order.
+//
+// Long calls are bound by the stream of the cache: 64 sequences of 8192 tokens (28 / 4 heads x 128) 83 us,
+// 511 MB at 6.2 TB/s (part of it from the 256 MB cache). Short ones by latency: 32 of 4096 (14 / 2 x 64)
+// 13.1 us, 32 MB, of which two launches take 7.4; one of 1000 tokens 7.5, three trips to memory (table and
+// position, the tile, the store) and a join of 8 waves.
 // ---------------------------------------------------------------------------------------------
 constexpr int kDecWaves = 8;
 
@@ -470,7 +475,16 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // (16 QB a wave) and a range of 64-key tiles; grid.z splits the keys where rows alone leave CUs idle.
 // A tile's codes are converted once, on their way into LDS: K [key][dim], keys in the order in which
 // the scores come out as 16 consecutive keys a lane, and V^T [dim][key] as it lies in the page, its 16-byte
-// chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks.
+// chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks. One barrier a
+// tile: two buffers, and two workgroups on a CU that need not keep step.
+//
+// 2048 tokens over 8192 (28 / 4 heads x 128, bf16) take 337 us, 270 GFLOP at 803 TFLOP/s. No unit is full:
+// MFMA 33% busy, vector instructions 43%, LDS 33% (a quarter of it conflicts); a wave waits for its own chain
+// (scores, weights, products) and for the tile, and two waves a SIMD hide half of that. Left out one at a
+// time, staging saves 100 us, the softmax 60, the loads 42. Tried, in us: 64 rows a wave at one wave a
+// SIMD 635; 256 rows and 8 waves a workgroup 354; the same in two halves a phase apart, products in one
+// while the other has its softmax, 357; staging between the products 389 to 416; the next tile's scores
+// between this one's softmax 331 to 350, and slower with head_dim 64; wave priorities 342 to 361.
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunkWaves = 4;
 constexpr int kAhead = 3;  // LDS fragments read before they are needed
