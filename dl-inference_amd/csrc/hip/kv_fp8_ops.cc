@@ -128,7 +128,9 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
                             int64_t head_dim, int64_t block_size, int64_t max_blocks) {
   const int64_t units = batch * kv_heads, rows = q_heads / kv_heads * seq_q;
   const bool paged = block_size % 64 == 0 || block_size == 16 || block_size == 32;
-  if (dimIndex(head_dim) < 0 || !paged || units > kMostGrid || units == 0 || rows >= kMostTokens)
+  // offsets within a page's head are 32 bits
+  const bool near = block_size * head_dim < int64_t{1} << 31;
+  if (dimIndex(head_dim) < 0 || !paged || !near || units > kMostGrid || units == 0 || rows >= kMostTokens)
     return {0, 0, 1};
   const int64_t tiles = (block_size * max_blocks + 63) / 64;
   if (rows <= 16) {

@@ -78,6 +78,7 @@ def test_workspace():
     assert size(1, 14, 2, 1, 64, 64, 1) == 0        # one page
     assert size(512, 14, 2, 1, 64, 64, 64) == 0     # more pairs than CUs
     assert size(1, 14, 2, 1, 80, 64, 64) == 0 and size(1, 14, 2, 1, 64, 24, 64) == 0  # row by row
+    assert size(1, 14, 2, 1, 64, 1 << 25, 8) == 0   # row by row too: a page past 32-bit offsets
     for bad in ((0, 14, 2, 1, 64, 64, 64), (1, 13, 2, 1, 64, 64, 64), (1, 14, 0, 1, 64, 64, 64),
                 (1, 14, 2, 0, 64, 64, 64), (1, 14, 2, 1, 64, 0, 64), (1, 14, 2, 1, 64, 64, -1),
                 (1, 14, 2, 1, 64, 1 << 40, 1 << 40), (1 << 40, 14, 2, 1, 64, 64, 64),

@@ -511,3 +511,31 @@ def test_more_rows_than_workgroups():
     for at in range(0, 13000, 6500):
         part = attend(pools, q[:, :, at:at + 6500].contiguous(), past + at)
         assert torch.equal(part, whole[:, :, at:at + 6500])
+
+
+@pytest.mark.parametrize("seq", [1, 20])
+def test_a_page_past_32_bit_offsets(seq):
+    """A page of 2^33 bytes a head: the dims of the values lie past 32-bit offsets."""
+    block, dim = 1 << 26, 128
+    small = Pools(1, 1, dim, 64, 2, spare=0)
+    small.table[0] = torch.tensor([0, 1])
+    cache = small.oracle()
+    pools = Pools(1, 1, dim, 8, 1, spare=0)
+    pools.block, pools.count = block, 1
+    pools.key = torch.empty((1, 1, block, dim), dtype=torch.uint8, device="cuda")
+    pools.value = torch.empty((1, 1, dim, block), dtype=torch.uint8, device="cuda")
+    pools.scales = torch.empty((1, 1, 2, block), dtype=torch.uint8, device="cuda")
+    pools.table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+    pools.key[0, 0, :128] = small.key.view(128, dim).cuda()
+    for i in range(2):
+        pools.value[0, 0, :, 64 * i:64 * i + 64] = small.value[i, 0].cuda()
+        pools.scales[0, 0, :, 64 * i:64 * i + 64] = small.scales[i, 0].cuda()
+    q = torch.randn((1, 4, seq, dim), generator=rng(seq)).bfloat16()
+    out = attend(pools, q.cuda(), 100)
+    check_attention(out, cache.attention(q.double().numpy(), [100], True, dim ** -0.5), torch.bfloat16, 128,
+                    dim)
+    k = torch.randn((1, 1, seq, dim), generator=rng(3)).bfloat16()
+    cache.append(k.double().numpy(), k.double().numpy(), [50])
+    append(pools, k.cuda(), k.cuda(), 50)
+    for x, want in zip(read(pools, 128, 0, torch.float32), cache.read([0], 128)):
+        assert np.array_equal(x.cpu().double().numpy(), want)
