@@ -45,6 +45,7 @@ DeviceKernel k_chunk[2][2][3] = {KV8_DIMS("kv_fp8_attention", "kv8_chunk_", "_r6
   { {"kv_fp8_attention", base "d64_r128_bf16"}, {"kv_fp8_attention", base "d128_r128_bf16"},      \
     {"kv_fp8_attention", base "d128_r128_f16"} }
 DeviceKernel k_chunk_large[2][3] = {KV8_LARGE("kv8_chunk_"), KV8_LARGE("kv8_chunk_small_")};
+DeviceKernel k_phased = {"kv_fp8_attention", "kv8_phased_d128_bf16"};  // 256 rows
 DeviceKernel k_merge[2][3] = KV8_DIMS("kv_fp8_attention", "kv8_merge_", "");
 DeviceKernel k_rows[3] = KV8_DTYPES("kv_fp8_attention", "kv8_rows");
 
@@ -120,12 +121,13 @@ int launchWrite(const Kv8WriteArgs& a, bool tiles, int rows, int di, DeviceKerne
 // How attention runs: 0 one wave per row, 1 decode (at most 16 rows of a pair), 2 chunk.
 struct AttentionPlan {
   int form;
-  int size;  // chunk: 0 for 64 rows a workgroup, 1 for 128
+  int size;  // chunk: 64 << size rows a workgroup; 2 is the phased kernel
   int64_t splits;
 };
 
+// reach: tokens that a sequence holds at most, queries included.
 AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
-                            int64_t head_dim, int64_t block_size, int64_t max_blocks) {
+                            int64_t head_dim, int64_t block_size, int64_t max_blocks, int64_t reach) {
   const int64_t units = batch * kv_heads, rows = q_heads / kv_heads * seq_q;
   const bool paged = block_size % 64 == 0 || block_size == 16 || block_size == 32;
   // offsets within a page's head are 32 bits
@@ -154,16 +156,26 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
   const int size = dtype == DLI_BF16  ? large >= 128
                    : dtype == DLI_F16 ? large >= 384 && head_dim == 128
                                       : 0;
-  const int64_t tile_rows = int64_t{64} << size;
-  const int64_t blocks = units * ((rows + tile_rows - 1) / tile_rows);
+  const auto blocksOf = [&](int s) { return units * ((rows + (int64_t{64} << s) - 1) / (int64_t{64} << s)); };
   // keys split until two workgroups stand on every CU, each with 4 tiles at least; a split's results
   // are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4 heads
   // x 128: 37 us, 61 in two splits)
-  int64_t splits = 512 / blocks;
-  const int64_t most = tiles / 4;
-  splits = splits < most ? splits : most;
-  splits = splits < 32 ? splits : 32;
-  return {2, size, splits > 1 ? splits : 1};
+  const auto splitsOf = [&](int64_t blocks, int64_t places) {
+    int64_t splits = places / blocks;
+    const int64_t most = tiles / 4;
+    splits = splits < most ? splits : most;
+    splits = splits < 32 ? splits : 32;
+    return splits > 1 ? splits : 1;
+  };
+  if (dtype == DLI_BF16 && head_dim == 128 && size == 1 && block_size % 64 == 0 && reach > 2500) {
+    // A phased workgroup has a CU to itself, so it pays over long contexts, where its first and last
+    // steps count little, and where its rounds fill the card by two thirds. 128 rows and phased, us (28 / 4
+    // heads): 2 x 1000 tokens over nothing 37 and 42, over 1000 67 and 72, 2000 101 and 96, 4000 170 and
+    // 149; 1 x 4096 155 and 130; 2 x 300 over 3000 63 and 60; 8 x 300 over 3000, 288 workgroups, 185 and 191.
+    const int64_t blocks = blocksOf(2), splits = splitsOf(blocks, 256), all = blocks * splits;
+    if ((all + 255) / 256 * 256 * 2 <= all * 3) return {2, 2, splits};
+  }
+  return {2, size, splitsOf(blocksOf(size), 512)};
 }
 
 size_t partBytes(int64_t rows, int64_t head_dim, int64_t splits) {
@@ -264,11 +276,13 @@ size_t dli_hip_paged_attention_fp8_workspace(int64_t batch, int64_t q_heads, int
       seq_q >= kMostTokens || block_size >= kMostTokens || max_blocks >= kMostTokens ||
       block_size * max_blocks >= kMostTokens)
     return 0;
-  int64_t splits = 1;  // the most of any data type
+  int64_t splits = 1;  // the most of any data type and number of tokens held
   for (int dtype : {DLI_F32, DLI_BF16, DLI_F16}) {
-    const AttentionPlan plan =
-        attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
-    splits = splits > plan.splits ? splits : plan.splits;
+    for (int64_t reach : {int64_t{0}, block_size * max_blocks}) {
+      const AttentionPlan plan =
+          attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks, reach);
+      splits = splits > plan.splits ? splits : plan.splits;
+    }
   }
   return partBytes(batch * q_heads * seq_q, head_dim, splits);
 }
@@ -293,8 +307,11 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
   if (q == nullptr || out == nullptr) return badArg(op, "null input or output");
   const int64_t rows = batch * q_heads * seq_q;
   if (rows >= (int64_t{1} << 31)) return badArg(op, "too many query rows");
+  const int64_t capacity = block_size * max_blocks, before = past < 0 ? 0 : past;
+  const int64_t reach =
+      positions != nullptr || before >= capacity || before + seq_q > capacity ? capacity : before + seq_q;
   AttentionPlan plan =
-      attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks);
+      attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks, reach);
   // the MFMA forms take 16-byte loads and put masked scores to -inf before the scale's sign could
   // matter, as the other attention kernels do
   if (!(scale > 0.f) || !std::isfinite(scale) || !aligned16(q) || !aligned16(out) ||
@@ -309,7 +326,7 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
   a.splits = static_cast<int>(plan.splits);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = plan.splits > 1 ? a.part_o + rows * plan.splits * head_dim : nullptr;
-  a.capacity = block_size * max_blocks;
+  a.capacity = capacity;
   a.batch = static_cast<int>(batch);
   a.q_heads = static_cast<int>(q_heads);
   a.seq_q = static_cast<int>(seq_q);
@@ -327,12 +344,13 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
                 a);
   } else {
     const int64_t tile = int64_t{64} << plan.size, pair_rows = q_heads / kv_heads * seq_q;
-    DeviceKernel& chunk = plan.size == 0 ? k_chunk[small][dim][di]
-                                         : k_chunk_large[small][dtype == DLI_F16 ? 2 : dim];
+    DeviceKernel& chunk = plan.size == 0   ? k_chunk[small][dim][di]
+                          : plan.size == 1 ? k_chunk_large[small][dtype == DLI_F16 ? 2 : dim]
+                                           : k_phased;
     rc = launch(chunk,
                 {static_cast<unsigned>((pair_rows + tile - 1) / tile), units,
                  static_cast<unsigned>(plan.splits)},
-                {256}, 0, stream, a);
+                {plan.size == 2 ? 512u : 256u}, 0, stream, a);
   }
   if (rc != 0 || plan.splits == 1) return rc;
   return launch(k_merge[dim][di], {blocksFor(rows, 4)}, {256}, 0, stream, a);

@@ -478,13 +478,13 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks. One barrier a
 // tile: two buffers, and two workgroups on a CU that need not keep step.
 //
-// 2048 tokens over 8192 (28 / 4 heads x 128, bf16) take 337 us, 270 GFLOP at 803 TFLOP/s. No unit is full:
-// MFMA 33% busy, vector instructions 43%, LDS 33% (a quarter of it conflicts); a wave waits for its own chain
-// (scores, weights, products) and for the tile, and two waves a SIMD hide half of that. Left out one at a
-// time, staging saves 100 us, the softmax 60, the loads 42. Tried, in us: 64 rows a wave at one wave a
-// SIMD 635; 256 rows and 8 waves a workgroup 354; the same in two halves a phase apart, products in one
-// while the other has its softmax, 357; staging between the products 389 to 416; the next tile's scores
-// between this one's softmax 331 to 350, and slower with head_dim 64; wave priorities 342 to 361.
+// 2048 tokens over 8192 (28 / 4 heads x 128, bf16) take 339 us, 270 GFLOP at 798 TFLOP/s (290 phased, below).
+// No unit is full: MFMA 33% busy, vector instructions 43%, LDS 33% (a quarter of it conflicts); a wave waits
+// for its own chain (scores, weights, products) and for the tile, and two waves a SIMD hide half of
+// that. Left out one at a time, staging saves 100 us, the softmax 60, the loads 42. Tried, in us: 64 rows a
+// wave at one wave a SIMD 635; 256 rows and 8 waves a workgroup in step 354; the next tile's scores between
+// this one's softmax 331 to 350, and slower with head_dim 64; wave priorities 342 to 361; scales read by
+// their users, without LDS, 343.
 // ---------------------------------------------------------------------------------------------
 constexpr int kChunkWaves = 4;
 constexpr int kAhead = 3;  // LDS fragments read before they are needed
@@ -494,6 +494,36 @@ constexpr int kValueLift = 7;
 // a row's shift before its first key: any finite score added to it passes the slack, and -infinity
 // stays what it is
 constexpr float kNoReference = 0x1.fffffep127f;
+
+// A weight's exponent is score * scale + shift in one fma. From 2^23 on the shift's own rounding would show
+// in it (and past 2^27 pass what f16 holds): rows whose reference lies there subtract the score at the
+// reference first. Their scores are rounded to whole units and more, so only the largest matters.
+constexpr float kFarShift = 8388608.f;
+__device__ __forceinline__ bool farRow(float shift) {
+  return fabsf(shift) >= kFarShift && shift != kNoReference;
+}
+__device__ __forceinline__ float farExponent(float score, float ref, float shift, float scale) {
+  return farRow(shift) ? fmaf(score - ref, scale, kLift) : fmaf(score, scale, shift);
+}
+// Scores of a far row become those past its reference; what brings score * scale to its exponent.
+__device__ __forceinline__ float fromReference(f32x4 (&s)[4], float ref, float shift) {
+  const bool away = farRow(shift);
+#pragma unroll
+  for (int n = 0; n < 16; ++n) s[n / 4][n % 4] -= away ? ref : 0.f;
+  return away ? kLift : shift;
+}
+// Moves a row's reference to its largest score `most` if its weight would pass 2^(kLift + kSlack); the factor
+// of what was summed so far.
+__device__ __forceinline__ float moveReference(float most, float scale, float& ref, float& shift) {
+  const float top = rowsMax(most);  // the same in a row's four lanes
+  if (!(farExponent(top, ref, shift, scale) > kLift + kSlack)) return 1.f;
+  const float next = kLift - top * scale;
+  const float alpha =
+      __builtin_amdgcn_exp2f(farRow(shift) ? (ref - top) * scale : next - shift);  // 0 at first
+  ref = top;
+  shift = next;
+  return alpha;
+}
 
 // Places of 16-byte chunks (8 elements) in LDS. A ds_read_b128 serves 16 lanes a cycle: lanes 0-3,
 // 12-15 and 20-27 together, then 4-11, 16-19 and 28-31, and the upper half alike (found by timing pairs
@@ -529,6 +559,46 @@ __device__ __forceinline__ U128 scaledKey(uint32_t w0, uint32_t w1, float scale)
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true)),
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false)),
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true))};
+}
+
+// Rows first .. first + 16 QB - 1 of a wave, o in units of the value scale top: stored, or left with their
+// maximum and sum for the join.
+template <class T, int D, int QB>
+__device__ __forceinline__ void storeRows(const Kv8AttentionArgs& a, int b, int kvh, int group, int rows,
+                                          int first, const f32x4 (&o)[QB][D / 16],
+                                          const f32x4 (&ls)[QB], const float (&shift)[QB],
+                                          uint32_t top) {
+  constexpr int DT = D / 16;
+  const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    const float L = __shfl(ls[qb][0], r, kWave);
+    const int p = first + qb * 16 + r;
+    if (p >= rows) continue;
+    const RowAt at = rowAt(p, group, kvh);
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // no key, or none of any weight: zeros
+    const int e = static_cast<int>(top) - 127 - kValueLift;
+    if (a.splits == 1) {
+      T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st(out + 16 * dt + i, __builtin_ldexpf(o[qb][dt][i] * inv, e));
+    } else {
+      const int64_t part = queryAt(a, b, at, 1) * a.splits + blockIdx.z;
+      if (g == 0) {
+        a.part_ml[part * 2] = L == 0.f ? -INFINITY : fminf(kLift - shift[qb], kNoReference);
+        a.part_ml[part * 2 + 1] = L;
+      }
+      float* out = a.part_o + part * D + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          out[16 * dt + i] = __builtin_ldexpf(o[qb][dt][i] * inv, e);
+    }
+  }
 }
 
 template <int D>
@@ -669,11 +739,14 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 
   f32x4 o[QB][DT];
   f32x4 ls[QB];        // element 0 of the lanes g = 0: the sum of row r's weights
-  float shift[QB];     // kLift less the row's reference
+  float shift[QB];     // kLift less the row's reference, times the scale
+  float ref[QB];       // the reference, a score
+  bool far = false;    // a row of the wave has been farRow
   uint32_t top = 0;    // the largest value scale seen, which o is kept in
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     shift[qb] = kNoReference;
+    ref[qb] = 0.f;
     ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -794,20 +867,28 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 #pragma unroll
       for (int n = 0; n < 16; ++n) smax = fmaxf(smax, s[qb][n / 4][n % 4]);
       // the reference moves only when a weight would pass 2^(kLift + kSlack)
-      if (__builtin_amdgcn_ballot_w64(fmaf(smax, score_scale, shift[qb]) > kLift + kSlack)) {
-        const float tmax = rowsMax(smax) * score_scale;  // the same in a row's four lanes
-        const bool grow = tmax + shift[qb] > kLift + kSlack;
-        const float next = kLift - tmax;
-        const float alpha = grow ? __builtin_amdgcn_exp2f(next - shift[qb]) : 1.f;  // 0 at first
-        shift[qb] = grow ? next : shift[qb];
+      bool over = fmaf(smax, score_scale, shift[qb]) > kLift + kSlack;
+      if (far) {
+        rarely();
+        over = farExponent(smax, ref[qb], shift[qb], score_scale) > kLift + kSlack;
+      }
+      if (__builtin_amdgcn_ballot_w64(over)) {
+        rarely();
+        const float alpha = moveReference(smax, score_scale, ref[qb], shift[qb]);
+        far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
         ls[qb] *= alpha;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
       }
+      float to_lift = shift[qb];
+      if (far) {
+        rarely();
+        to_lift = fromReference(s[qb], ref[qb], shift[qb]);
+      }
 #pragma unroll
       for (int n = 0; n < 16; ++n)
         s[qb][n / 4][n % 4] =
-            __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], score_scale, shift[qb]));
+            __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], score_scale, to_lift));
       packWeights<Ty::kP>(s[qb], pf[qb]);
     }
 #pragma unroll
@@ -827,35 +908,330 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ls, shift, top);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows over long contexts (bf16, head_dim 128, pages of a multiple of 64): 8 waves and 256 rows a
+// workgroup, in two halves that run a phase apart, a barrier between phases. In its matrix phase a
+// half adds the values of tile kt - 1 and takes the scores of tile kt, and between those products it
+// stages its part of the keys of kt + 1 and the values of kt; in the other phase it asks for the codes of the
+// tile after and turns the scores into weights. So one wave of a SIMD feeds the matrix unit while the other
+// has its softmax, where the kernel above leaves it to chance:
+//   phase     0     1     2     3     4
+//   half 0   M(0)  S(0)  M(1)  S(1)  M(2)
+//   half 1         M(0)  S(0)  M(1)  S(1)
+// A tile's buffers are written by both halves in their M(kt - 1), two phases in a row, and read in their M of
+// the keys' tile, or the one after for values: each has two. Wave priority goes with the matrix phase.
+//
+// 2048 tokens over 8192 (28 / 4 heads x 128) 290 us, 933 TFLOP/s; above 339. A phase takes 1800 cycles
+// either way (products alone: 1455, of which the unit needs 1088). Steps, in us: everything staged in the
+// softmax phase 357, between the products 416, the scales read by their users and page offsets in 32 bits
+// 335, priority 309, loads issued in the softmax phase 295.
+// ---------------------------------------------------------------------------------------------
+constexpr int kPhasedWaves = 8;
+
+template <int D>
+struct PhasedLds {
+  uint16_t k[2][kTileK * D];
+  uint16_t v[2][D * kTileK];
+  uint16_t vf[kPhasedWaves][kTileK];  // each wave's own copy of a tile's value factors
+};
+
+template <bool kBoth>
+struct Products {
+  static constexpr bool kKeys = kBoth;
+};
+
+__device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
+  using T = bf16;
+  constexpr int D = 128, QB = 2, DT = D / 16, DK = D / 32, kRows = 16 * QB * kPhasedWaves;
+  constexpr int kParts = D / 16;  // 16-code chunks of a key; a thread stages one of K and one of V^T
+  static_assert(kTileK * kParts == kPhasedWaves * kWave);
+  __shared__ __attribute__((aligned(16))) PhasedLds<D> lds;
+  const Kv8Pages& pg = a.pages;
+  const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int r = lane % 16, g = lane / 16;
+  const int group = a.q_heads / pg.heads, rows = a.seq_q * group, bs = pg.block_size;
+  // pairs, row tiles and clamped rows as in kv8_chunk
+  const uint32_t lin = blockIdx.x + gridDim.x * blockIdx.y;
+  const int pair = static_cast<int>(lin % gridDim.y), b = pair / pg.heads, kvh = pair - b * pg.heads;
+  const int p0 = static_cast<int>(gridDim.x - 1 - lin / gridDim.y) * kRows;
+  const int pw = p0 + wave * 16 * QB;  // the wave's first row
+  const bool late = wave >= kPhasedWaves / 2;
+  const int64_t past = kv8First(pg, b);
+  auto clamped = [&](int p) { return p < rows ? p : rows - 1; };
+
+  U128 qf[QB][DK][1];
+  int lim[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const float L = __shfl(ls[qb][0], r, kWave);
-    const int p = pw + qb * 16 + r;
-    if (p >= rows) continue;
-    const RowAt at = rowAt(p, group, kvh);
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // no key, or none of any weight: zeros
-    const int e = static_cast<int>(top) - 127 - kValueLift;
-    if (a.splits == 1) {
-      T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + 4 * g;
+    const RowAt at = rowAt(clamped(pw + qb * 16 + r), group, kvh);  // clamped: not stored
+    const T* q = static_cast<const T*>(a.q) + queryAt(a, b, at, D) + g * 8;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          st(out + 16 * dt + i, __builtin_ldexpf(o[qb][dt][i] * inv, e));
-    } else {
-      const int64_t part = queryAt(a, b, at, 1) * a.splits + blockIdx.z;
-      if (g == 0) {
-        a.part_ml[part * 2] = L == 0.f ? -INFINITY : kLift - shift[qb];
-        a.part_ml[part * 2 + 1] = L;
-      }
-      float* out = a.part_o + part * D + 4 * g;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          out[16 * dt + i] = __builtin_ldexpf(o[qb][dt][i] * inv, e);
-    }
+    for (int c = 0; c < DK; ++c) queryFragment<T>(q + c * 32, qf[qb][c]);
+    lim[qb] = visibleKeys(a, past, at.i);
   }
+  const int wg_keys = visibleKeys(a, past, clamped(p0 + kRows - 1) / group);
+  const int wave_full = visibleKeys(a, past, clamped(pw) / group);  // keys every row of the wave sees
+  const int all_tiles = (wg_keys + kTileK - 1) / kTileK;
+  const int per = (all_tiles + a.splits - 1) / a.splits;
+  const int kt0 = static_cast<int>(blockIdx.z) * per;
+  const int kt1 = kt0 + per < all_tiles ? kt0 + per : all_tiles;
+
+  // The page id of tile next_kt is read a tile ahead of the loads that use it. Tiles past the last one
+  // repeat it.
+  const int32_t* table = pg.table + static_cast<int64_t>(b) * pg.max_blocks;
+  const int tiles_per_page = bs / kTileK;
+  int next_kt = kt0, next_page = kt0 / tiles_per_page;
+  int next_slot = (kt0 - next_page * tiles_per_page) * kTileK;
+  int coming_id = 0, coming_slot = 0;
+  auto loadId = [&] {
+    coming_id = gp(table)[next_page];
+    coming_slot = next_slot;
+    if (next_kt < kt1 - 1) {
+      ++next_kt;
+      next_slot += kTileK;
+      if (next_slot >= bs) {
+        next_slot = 0;
+        ++next_page;
+      }
+    }
+  };
+  const uint32_t held = static_cast<uint32_t>(pg.num_blocks < INT32_MAX ? pg.num_blocks : INT32_MAX);
+  const uint32_t head = static_cast<uint32_t>(bs) * D;  // attentionPlan: below 2^31
+  const uint64_t page_codes = static_cast<uint64_t>(pg.heads) * head;
+  const uint64_t page_scales = static_cast<uint64_t>(pg.heads) * 2u * static_cast<uint32_t>(bs);
+  const uint8_t* const keys = pg.key + static_cast<uint64_t>(kvh) * head;
+  const uint8_t* const values = pg.value + static_cast<uint64_t>(kvh) * head;
+  const uint8_t* const scales = pg.scales + static_cast<uint64_t>(kvh) * 2u * static_cast<uint32_t>(bs);
+  // This thread's chunks: part of key t / kParts, and the run of 16 keys t % 4 of dim t / 4.
+  const int key = t / kParts, part = t % kParts, dim = t / 4, run = t % 4;
+  const uint32_t vo = static_cast<uint32_t>(dim) * static_cast<uint32_t>(bs) + 16u * run;
+  const int key_row = 16 * (key % 16 / 4) + 4 * (key / 16) + key % 4;  // as in kv8_chunk
+  // On their way: the keys of a tile and the scales of this thread's key, the value scale of this lane's
+  // key, and the values and value scales of the tile before.
+  U128 kr, vr;
+  uint32_t own_k = 0, own_v = 0, vc = 0, vc_before = 0;
+  bool in = false, in_before = false;  // those tiles' pages hold something
+  uint64_t value_page = 0;
+  auto fetch = [&] {
+    const uint32_t id = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(coming_id));
+    const uint32_t slot = static_cast<uint32_t>(coming_slot);
+    in_before = in;
+    in = id < held;  // else page 0 is read in its place and masked
+    const uint64_t page = in ? id : 0u;
+    loadId();
+    const uint8_t* sb = scales + page * page_scales + slot;
+    own_k = gp(sb)[static_cast<uint32_t>(key)];
+    own_v = gp(sb + bs)[static_cast<uint32_t>(key)];
+    vc_before = vc;
+    vc = gp(sb + bs)[static_cast<uint32_t>(lane)];
+    kr = gload16(keys + page * page_codes + static_cast<uint64_t>(slot) * D + static_cast<uint32_t>(t) * 16);
+    vr = gload16(values + value_page + vo);
+    value_page = page * page_codes + slot;
+  };
+
+  f32x4 o[QB][DT];
+  f32x4 ls[QB];     // element 0 of the lanes g = 0: the sum of row r's weights
+  float shift[QB];  // kLift less the row's reference, times the scale
+  float ref[QB];    // the reference, a score
+  bool far = false;  // a row of the wave has been farRow
+  f32x4 s[QB][4];
+  U128 pf[QB][1][2];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb) {
+    shift[qb] = kNoReference;
+    ref[qb] = 0.f;
+    ls[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    pf[qb][0][0] = pf[qb][0][1] = zero16();
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[qb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
+  const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
+
+  // The largest value scale up to the tile whose factors were written last, up to the one before, and
+  // the one that o is kept in.
+  uint32_t top = 0, top_before = 0, top_o = 0;
+  auto factors = [&](int kt, bool there, uint32_t code) {  // of tile kt
+    code = code == 255u || !there || kt * kTileK + lane >= wg_keys ? 0u : code;
+    top_before = top;
+    if (__builtin_amdgcn_ballot_w64(code > top)) {  // every wave comes to the same
+      rarely();
+      top = waveMaxU(code);
+    }
+    lds.vf[wave][lane] = valueFactorF16(code, top);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' factors are read
+  };
+  uint64_t lives = 0;  // the keys of the tile staged last that are there
+  U128 vf[2] = {zero16(), zero16()};
+  uint32_t nan = 0;
+  float key_scale = 1.f;
+  auto keyScale = [&] {
+    const bool bad = own_k == 255u || own_v == 255u;
+    nan = bad ? 0x7FC07FC0u : 0u;  // the codes of such a row are 0
+    key_scale = mxScaleValue(bad ? 127u : own_k);
+  };
+  auto stageKeys = [&](int buf, int half) {
+    U128 w = scaledKey(kr[2 * half], kr[2 * half + 1], key_scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] |= nan;
+    *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(key_row, 2 * part + half)]) = w;
+  };
+  auto stageValues = [&](int buf, int half) {
+    *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(dim, run, half)]) =
+        valueFragment(vr[2 * half], vr[2 * half + 1], vf[half]);
+  };
+  // The keys of kt + 1 and the values of kt, in pieces that fit between products.
+  constexpr int kPieces = 5, kPieceSteps = 3;
+  auto stage = [&](int kt, int piece) {
+    const int vbuf = kt & 1, kbuf = vbuf ^ 1;
+    if (piece == 0) {
+      vf[0] = load16(&lds.vf[wave][16 * run]);
+      vf[1] = load16(&lds.vf[wave][16 * run + 8]);
+      const int n = wg_keys - kt * kTileK;
+      lives = !in_before || n <= 0 ? uint64_t{0} : n >= kTileK ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
+    } else if (piece == 1) {
+      keyScale();
+      stageKeys(kbuf, 0);
+    } else if (piece == 2) {
+      stageKeys(kbuf, 1);
+    } else if (piece == 3) {
+      if (lives != ~uint64_t{0}) {
+        rarely();
+        keepBytes(vr, static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
+      }
+      stageValues(vbuf, 0);
+    } else {
+      stageValues(vbuf, 1);
+    }
+  };
+  auto products = [&](int kt, auto which) {  // the values of kt - 1, and the scores of kt
+    constexpr bool kKeys = decltype(which)::kKeys;
+    constexpr int kValueSteps = 2 * DT, kSteps = kValueSteps + (kKeys ? 4 * DK : 0);
+    const int kbuf = kt & 1, vbuf = kbuf ^ 1;
+    auto read = [&](int i) {
+      if (i < kValueSteps) return load16(&lds.v[vbuf][valueChunk(16 * (i % DT) + r, g, i / DT)]);
+      const int n = i - kValueSteps;
+      return load16(&lds.k[kbuf][keyChunk<D>(n / DK * 16 + r, 4 * (n % DK) + g)]);
+    };
+    if (top_before != top_o) {
+      rarely();
+      const float down = valueFactor(top_o, top_before);
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= down;
+      top_o = top_before;
+    }
+    U128 frag[kAhead + 1];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) frag[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + kAhead < kSteps) frag[(i + kAhead) % (kAhead + 1)] = read(i + kAhead);
+      if (kKeys && i % kPieceSteps == 0 && i / kPieceSteps < kPieces) stage(kt, i / kPieceSteps);
+      const U128& f = frag[i % (kAhead + 1)];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        if (i < kValueSteps) {
+          if (i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][0][i / DT], ls[qb]);
+          o[qb][i % DT] = F16::mma(f, pf[qb][0][i / DT], o[qb][i % DT]);
+        } else {
+          const int n = i - kValueSteps;
+          if (n % DK == 0) s[qb][n / DK] = f32x4{0.f, 0.f, 0.f, 0.f};
+          s[qb][n / DK] = keyMma<T>(f, qf[qb][n % DK][0], s[qb][n / DK]);
+        }
+      }
+    }
+  };
+
+  if (kt0 < kt1) {
+    // the first tile's keys; zeros in place of the values before it, whose weights are 0
+    loadId();
+    fetch();
+    keyScale();
+    stageKeys(kt0 & 1, 0);
+    stageKeys(kt0 & 1, 1);
+    factors(kt0, in, vc);
+    vr = zero16();
+    stageValues((kt0 & 1) ^ 1, 0);
+    stageValues((kt0 & 1) ^ 1, 1);
+    fetch();
+    __syncthreads();
+    if (late) __syncthreads();
+    for (int kt = kt0; kt < kt1; ++kt) {
+      const int k0 = kt * kTileK;
+      __builtin_amdgcn_s_setprio(1);
+      products(kt, Products<true>{});
+      __builtin_amdgcn_s_setprio(0);
+      __syncthreads();
+      fetch();
+      if (lives != ~uint64_t{0} || k0 + kTileK > wave_full) {
+        rarely();
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const int seen = lim[qb] - k0 - 16 * g;
+          const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu &
+                                (seen >= 16 ? 0xFFFFu : seen > 0 ? (1u << seen) - 1u : 0u);
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            if (!(mine >> n & 1u)) s[qb][n / 4][n % 4] = -INFINITY;
+        }
+      }
+      float most[QB];
+      bool over = false;
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        most[qb] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 16; ++n) most[qb] = fmaxf(most[qb], s[qb][n / 4][n % 4]);
+        over |= fmaf(most[qb], a.scale_log2, shift[qb]) > kLift + kSlack;
+      }
+      if (far) {
+        rarely();
+        over = false;
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+          over |= farExponent(most[qb], ref[qb], shift[qb], a.scale_log2) > kLift + kSlack;
+      }
+      // the references move only when a weight would pass 2^(kLift + kSlack)
+      if (__builtin_amdgcn_ballot_w64(over)) {
+        rarely();
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+          const float alpha = moveReference(most[qb], a.scale_log2, ref[qb], shift[qb]);
+          far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
+          ls[qb] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+        }
+      }
+      float to_lift[QB];
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) to_lift[qb] = shift[qb];
+      if (far) {
+        rarely();
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) to_lift[qb] = fromReference(s[qb], ref[qb], shift[qb]);
+      }
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+          s[qb][n / 4][n % 4] =
+              __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], a.scale_log2, to_lift[qb]));
+        packWeights<1>(s[qb], pf[qb]);
+      }
+      factors(kt + 1, in_before, vc_before);
+      __syncthreads();
+    }
+    products(kt1, Products<false>{});
+    if (!late) __syncthreads();
+  }
+  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ls, shift, top_o);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1041,3 +1417,7 @@ KV8_CHUNK(bf16, bf16, 128, 128)
 KV8_CHUNK(f16, f16, 64, 64)
 KV8_CHUNK(f16, f16, 128, 64)
 KV8_CHUNK(f16, f16, 128, 128)
+extern "C" __global__ void __launch_bounds__(kPhasedWaves* kWave, 1)
+    kv8_phased_d128_bf16(Kv8AttentionArgs a) {
+  kv8_phased(a);
+}

@@ -539,3 +539,123 @@ def test_a_page_past_32_bit_offsets(seq):
     append(pools, k.cuda(), k.cuda(), 50)
     for x, want in zip(read(pools, 128, 0, torch.float32), cache.read([0], 128)):
         assert np.array_equal(x.cpu().double().numpy(), want)
+
+
+# bf16, head_dim 128, many workgroups and contexts past 2500 tokens: two splits of 17 rows a pair, rows of
+# three workgroups a pair, one split
+PHASED = [(16, 8, 8, 17, 64), (16, 32, 2, 40, 128), (32, 8, 8, 33, 64)]
+
+
+@pytest.mark.parametrize("batch,q_heads,heads,seq,block", PHASED)
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows_over_long_contexts(batch, q_heads, heads, seq, block, causal):
+    """Sequences of every length class: none, less than a tile, tile edges, past the pages; pages that hold
+    nothing at the start, in the middle and at the end of a sequence."""
+    tokens = 2560
+    n = tokens // block
+    missing = [(1, n - 1, -1), (2, 0, 1 << 30), (3, n // 2, -7), (4, n // 2, -1), (4, n // 2 + 1, -1)]
+    missing += [(5, i, -1) for i in range(n)]
+    pools = Pools(batch, heads, 128, block, n, seed=seq, missing=missing)
+    lengths = [0, 2530, 2400, 1999, 2100, 900, -seq, -9, 2560, 5000, 30, 31, 47, 48, 63, 64]
+    past = [x - (seq if 20 < x < 70 else 0) for x in lengths] * (batch // 16)
+    q = torch.randn((batch, q_heads, seq, 128), generator=rng(seq + 1)).bfloat16()
+    cache = pools.oracle()
+    pools.cuda()
+    want = cache.attention(q.double().numpy(), past, causal, 128 ** -0.5)
+    whole = attend(pools, q.cuda(), past, causal)
+    check_attention(whole, want, torch.bfloat16, tokens, 128)
+    ws = workspace(pools, q)
+    split = attend(pools, q.cuda(), past, causal, ws=ws, index=torch.int32)
+    check_attention(split, want, torch.bfloat16, tokens, 128)
+    rows = attend(pools, q.cuda(), past, causal, bshd=True, ws=ws)
+    assert torch.equal(rows.transpose(1, 2), split)
+
+
+def test_nan_tokens_and_sizes_over_long_contexts():
+    """Rows behind the last token of any content, NaN tokens that some queries see, values from the least to
+    the largest, scores far below zero: 17 rows a pair, two splits."""
+    pools = Pools(16, 8, 128, 64, 40, seed=3)
+    past = [1000 + 64 * b for b in range(16)]
+    behind = torch.zeros((16, 2560), dtype=torch.bool)
+    for b in range(16):
+        behind[b, past[b] + 17:] = True
+    cache = pools.oracle()
+    for b in range(16):
+        for i in range(40):
+            page, dead = int(pools.table[b, i]), behind[b, 64 * i:64 * i + 64]
+            pools.key[page, :, dead] = 0x7F
+            pools.value[page][:, :, dead] = 0xFF
+            pools.scales[page][:, :, dead] = 255
+            if b == 3:  # one size a tile, from small to large
+                size = torch.full((8, 64), 60 + 4 * i, dtype=torch.uint8)
+                pools.scales[page, :, 1] = torch.where(dead, pools.scales[page, :, 1], size)
+                cache.scales[page, :, 1] = size.numpy()
+        if b % 4 == 1:  # in the middle, and where only the last queries see it
+            for at in (777, past[b] + 9):
+                page = int(pools.table[b, at // 64])
+                for p in (pools, cache):
+                    p.key[page, :2, at % 64] = 0
+                    p.value[page, :2, :, at % 64] = 0
+                    p.scales[page, :2, at // 9 % 2, at % 64] = 255
+    q = torch.randn((16, 8, 17, 128), generator=rng(5))
+    q[7] *= 2.0 ** 100
+    q = q.bfloat16()
+    want = cache.attention(q.double().numpy(), past, True, 128 ** -0.5)
+    ws = workspace(pools, q)
+    pools.cuda()
+    for space in (None, ws):
+        out = attend(pools, q.cuda(), past, ws=space)
+        keep = [b for b in range(16) if b != 7]
+        check_attention(out[keep], tuple(x[keep] for x in want), torch.bfloat16, 2560, 128)
+        # scores of 2^100: the largest takes all the weight
+        assert torch.equal(out[7].cpu(), torch.from_numpy(want[0][7]).bfloat16())
+
+
+def test_long_contexts_captured():
+    """A graph of the kernel replayed with other queries and positions, against eager calls."""
+    pools = Pools(16, 8, 128, 64, 40, seed=4).cuda()
+    q = torch.randn((16, 8, 17, 128), generator=rng(1)).bfloat16().cuda()
+    first = torch.randint(0, 2600, (16,), generator=rng(2)).cuda()
+    ws = workspace(pools, q)
+    attend(pools, q, first, ws=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = attend(pools, q, first, ws=ws)
+    for step in range(4):
+        q.copy_(torch.randn(q.shape, generator=rng(20 + step)))
+        first.copy_(torch.randint(0, 2600, (16,), generator=rng(30 + step)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = static.clone()
+        assert torch.equal(got, attend(pools, q, first, ws=ws))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim,q_heads,seq", [(64, 2, 1), (64, 2, 20), (128, 2, 20), (64, 4, 1200), (128, 4, 1200),
+                                             (80, 2, 3)])
+@pytest.mark.parametrize("size", [26, 60, 100])
+def test_scores_past_whole_numbers(dtype, dim, q_heads, seq, size):
+    """Scores of about 2^size of either sign: the largest takes all the weight. One key of a row's four
+    stands out by a factor of two at least, so sums in fp32 find it."""
+    t = DTYPES[dtype]
+    pools = Pools(4, 1, dim, 64, 24)
+    pools.key[:] = 0
+    g = rng(size)
+    for b in range(4):
+        for i in range(24):
+            page = int(pools.table[b, i])
+            pools.key[page, 0, :, 0] = torch.randint(0x30, 0x38, (64,), generator=g).to(torch.uint8)
+        pools.key[int(pools.table[b, 0]), 0, 3 + b, 0] = 0x48
+        pools.key[int(pools.table[b, 0]), 0, 9, 0] = 0xC8
+    pools.scales[:, :, 0] = 127
+    q = torch.zeros((4, q_heads, seq, dim))
+    q[..., 0] = 2.0 ** size * (1 + torch.rand((4, q_heads, seq), generator=g))
+    q[:, 1::2] *= -1
+    q = q.to(t)
+    cache = pools.oracle()
+    out = attend(pools.cuda(), q.cuda(), 300, scale=dim ** -0.5 * 0.9).cpu()
+    for b in range(4):
+        for h in range(2):
+            want = torch.from_numpy(cache.rows(b, 9 if h else 3 + b)[1][0]).to(t)
+            assert torch.equal(out[b, h::2], want.expand(out[b, h::2].shape))
