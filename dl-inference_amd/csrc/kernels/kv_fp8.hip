@@ -9,7 +9,7 @@
 // a lane; the value pool is dim-major, so a tile's value codes are turned in LDS and leave as runs
 // of 16 tokens. Tiles start at multiples of their size in the cache, so a run never crosses a page.
 //
-// Bound by the bytes they move: with 3.7 us for a launch in a graph taken off, 4 x 2048 tokens (4 heads x 128,
+// Bound by the bytes they move: 3.7 us for a launch in a graph taken off, 4 x 2048 tokens (4 heads x 128,
 // bf16) are written in 5.0 us (25 MB, as fast as a large copy), 2 x 1000 tokens of q|k|v (28 / 4 heads x
 // 128, f16) in 7.8 (36 MB, 4.6 TB/s), 8 x 8192 tokens (4 heads x 128) read back in 41.6 (202 MB, 4.9 TB/s).
 // Short calls are bound by the chain of position, block table and store: 64 x 1 token 4.7 us with the
