@@ -389,11 +389,12 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
       for (int dt = 0; dt < DT; ++dt) o[dt] *= down;
       top = next;
     }
-    const float base = (m == -INFINITY ? 0.f : m) - kLift;
+    // the reference first: from 2^24 on m - kLift is rounded, and a weight passes f16's largest number
+    const float base = m == -INFINITY ? 0.f : m;
     float sum = 0.f;
 #pragma unroll
     for (int n = 0; n < 16; ++n) {
-      s[n / 4][n % 4] = __builtin_amdgcn_exp2f(s[n / 4][n % 4] - base);
+      s[n / 4][n % 4] = __builtin_amdgcn_exp2f(s[n / 4][n % 4] - base + kLift);
       sum += s[n / 4][n % 4];
     }
     l += sum;

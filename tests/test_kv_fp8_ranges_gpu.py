@@ -1,0 +1,75 @@
+"""The 8-bit KV cache's attention at the ends of its numbers' ranges, form by form: large scores, values
+and queries. Expected values are exact or float64; inputs are chosen so that fp32 sums are exact."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from dli import hip
+from test_kv_fp8_gpu import DTYPES, Pools, attend, rng, workspace
+
+pytestmark = pytest.mark.gpu
+
+# (head_dim, query heads, queries): one token, 16 rows at most, chunks of 64 and 128 rows, row by row
+FORMS = [(64, 2, 1), (128, 7, 1), (64, 8, 2), (128, 4, 4), (64, 4, 10), (128, 4, 1200), (64, 4, 1200), (80, 2, 3)]
+
+
+def code(value):
+    """The e4m3 code of an element."""
+    return int(torch.tensor(value).to(torch.float8_e4m3fn).view(torch.uint8))
+
+
+def token(pools, b, pos):
+    """(page, slot) of a position."""
+    return int(pools.table[b, pos // pools.block]), pos % pools.block
+
+
+def value_of(pools, b, pos):
+    """The value row that a position stands for, float64 [D] of KV head 0."""
+    page, slot = token(pools, b, pos)
+    elements = pools.value[page, 0, :, slot].cpu().view(torch.float8_e4m3fn).double()
+    return elements * 2.0 ** (int(pools.scales[page, 0, 1, slot]) - 127)
+
+
+def close(got, want, dtype, steps=16):
+    """Within the output's rounding (half a step, half of the least subnormal) and `steps` fp32 roundings
+    of the largest magnitude among the values."""
+    got, want = got.cpu().double(), want.expand(got.shape)
+    eps = torch.finfo(dtype).eps
+    bound = eps / 2 * want.abs() + steps * 2.0 ** -24 * want.abs().max() + torch.finfo(dtype).smallest_normal * eps
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim,q_heads,seq", FORMS)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("power", [20, 22, 23, 24, 25, 26, 27, 28, 29, 31, 60])
+def test_weights_of_large_scores(dtype, dim, q_heads, seq, sign, power):
+    """Scores (in powers of two) of sign * 1.5 * 2^power at one token and, where fp32 holds it, 4 more at
+    another, eight tiles later: weights 1 and 16. Elsewhere scores are lower by 2^power or more."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 30)
+    pools.key[:] = 0
+    if sign < 0:
+        pools.key[:, :, :, 0] = code(48.0)
+    pools.scales[:, :, 0] = 127 + power - 12
+    pools.scales[:, :, 1] = 127
+    first, second = 70, 70 + 8 * 64
+    apart = 4 if power <= 25 else 0
+    for pos, more in ((first, 0), (second, apart)):
+        page, slot = token(pools, 0, pos)
+        pools.key[page, 0, slot, 0] = code(24.0)
+        pools.key[page, 0, slot, 1] = code(2.0 ** -5 if more else 0.0)
+    q = torch.zeros((1, q_heads, seq, dim))
+    q[..., 0] = sign * 2.0 ** 8
+    q[..., 1] = 2.0 ** (min(power, 25) * -1 + 12 + 2 + 5)  # times 2^-5 2^(power - 12): 4
+    a, b = value_of(pools, 0, first), value_of(pools, 0, second)
+    weight = 2.0 ** apart
+    want = (a + weight * b) / (1 + weight)
+    pools.cuda()
+    for ws in (None, workspace(pools, q)):
+        out = attend(pools, q.to(t).cuda(), 700, scale=math.log(2), ws=ws)
+        # weights are powers of two; the quotient of their sum is rounded, and the output
+        close(out, want, t)
