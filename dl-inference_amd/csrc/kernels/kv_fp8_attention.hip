@@ -1264,13 +1264,15 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
   // no key, or none of any weight: 0; a NaN sum stays one whatever its maximum
   const float f = (m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M)) * l;
   const float L = waveSum(f);
+  // divided before they meet the values: a sum of L times a value may pass the largest number
+  const float share = L == 0.f ? 0.f : f / L;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < a.splits; s0 += kDepth * kAtOnce) {
     if (s0 > 0) load(s0);
 #pragma unroll
     for (int u = 0; u < kDepth; ++u) {
       const int s = s0 + u * kAtOnce + mine;
-      const float w = __shfl(f, s % kWave, kWave);
+      const float w = __shfl(share, s % kWave, kWave);
       if (s < a.splits) acc += x[u] * w;
     }
   }
@@ -1284,7 +1286,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
   const RowAt at = {i, static_cast<int>(bh % a.q_heads)};
   T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + d;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) st(out + u, L == 0.f ? 0.f : acc[u] / L);
+  for (int u = 0; u < 4; ++u) st(out + u, acc[u]);
 }
 
 // ---------------------------------------------------------------------------------------------

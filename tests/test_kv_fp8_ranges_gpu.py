@@ -73,3 +73,26 @@ def test_weights_of_large_scores(dtype, dim, q_heads, seq, sign, power):
         out = attend(pools, q.to(t).cuda(), 700, scale=math.log(2), ws=ws)
         # weights are powers of two; the quotient of their sum is rounded, and the output
         close(out, want, t)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim,q_heads,seq", [(64, 2, 1), (128, 7, 1), (128, 4, 4), (64, 4, 10), (128, 4, 40)])
+@pytest.mark.parametrize("exponent", [247, 246, 235, 0])
+def test_values_near_the_ends_over_splits(dtype, dim, q_heads, seq, exponent):
+    """Every token's values are 448 * 2^(exponent - 127), the weights of a row equal: the join of the splits
+    neither overflows nor loses what the output's type holds."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 30)
+    pools.value[:] = code(448.0)
+    pools.scales[:, :, 1] = exponent
+    q = torch.zeros((1, q_heads, seq, dim), dtype=t)
+    pools.cuda()
+    ws = workspace(pools, q)
+    assert ws.numel() > 0
+    want = torch.tensor(448.0 * 2.0 ** (exponent - 127), dtype=torch.float64)
+    out = attend(pools, q.cuda(), 1700, ws=ws)
+    if exponent == 247:  # 1.75 * 2^128 is past either type
+        assert (out == math.inf).all()
+    else:
+        # some 2000 equal weights: their sum in fp32 is exact, a split's quotient and the join's are rounded
+        close(out, want, t)
