@@ -74,7 +74,8 @@ __device__ __forceinline__ f32x4 keyMma(const U128& a, const U128& b, const f32x
     return Bf16::mma(a, b, c);
 }
 
-// 8 elements of q as terms: q itself, or three bf16 numbers (8 bits each, cut off) that add up to it
+// 8 elements of q as terms: q itself, or three bf16 numbers (8 bits each, cut off) that add up to it;
+// an infinity and two zeros, NaN and two zeros
 template <class T>
 __device__ __forceinline__ void queryFragment(const T* q, U128 (&f)[Kv8Type<T>::kQ]) {
   if constexpr (sizeof(T) == 2) {
@@ -83,13 +84,18 @@ __device__ __forceinline__ void queryFragment(const T* q, U128 (&f)[Kv8Type<T>::
     const U128 lo = gload16(q), hi = gload16(q + 4);
     uint32_t x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
+    for (int i = 0; i < 8; ++i)  // a NaN stays one without its low bits
+      if (__builtin_isnan(__uint_as_float(x[i]))) x[i] = 0x7FC00000u;
+#pragma unroll
     for (int u = 0; u < 3; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         f[u][j] = (x[2 * j] >> 16) | (x[2 * j + 1] & 0xFFFF0000u);
 #pragma unroll
         for (int i = 2 * j; i < 2 * j + 2; ++i)
-          x[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xFFFF0000u));
+          x[i] = u == 0 && !__builtin_isfinite(__uint_as_float(x[i]))
+                     ? 0u
+                     : __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xFFFF0000u));
       }
   }
 }

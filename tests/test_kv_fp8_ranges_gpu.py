@@ -96,3 +96,38 @@ def test_values_near_the_ends_over_splits(dtype, dim, q_heads, seq, exponent):
     else:
         # some 2000 equal weights: their sum in fp32 is exact, a split's quotient and the join's are rounded
         close(out, want, t)
+
+
+def bits(word):
+    return torch.tensor(word, dtype=torch.int32).view(torch.float32).item()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim,q_heads,seq", FORMS)
+def test_queries_that_are_not_finite(dtype, dim, q_heads, seq):
+    """As softmax has it, but zeros where every score is -infinity: an infinite query element whose keys'
+    elements all have the other sign weighs nothing; one key of its sign, or a NaN, makes the row NaN. Rows
+    beside it are those of a call without it, bit for bit."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 22)
+    pools.key[..., 0] = code(1.0)
+    pools.key[..., 1] = code(-1.0)
+    page, slot = token(pools, 0, 90)
+    pools.key[page, 0, slot, 1] = code(0.5)
+    pools.cuda()
+    q = torch.randn((1, q_heads, seq, dim), generator=rng(1)).to(t).cuda()
+    ws = workspace(pools, q)
+    past = 1400 - seq
+    for space in (None, ws):
+        plain = attend(pools, q, past, ws=space)
+        assert plain.isfinite().all()
+        nans = [math.nan] + ([bits(0x7F800001), bits(-0x7FFFFF)] if dtype == "float32" else [])
+        for at, x, want in [(0, -math.inf, 0.0), (1, -math.inf, math.nan), (1, math.inf, math.nan),
+                            (0, math.inf, math.nan)] + [(2, n, math.nan) for n in nans]:
+            odd = q.clone()
+            odd[0, 0, -1, at] = x
+            out = attend(pools, odd, past, ws=space)
+            row = out[0, 0, -1].clone()
+            assert row.isnan().all() if math.isnan(want) else (row == want).all(), (at, x)
+            out[0, 0, -1] = plain[0, 0, -1]
+            assert torch.equal(out, plain)
