@@ -100,6 +100,23 @@ __device__ __forceinline__ void queryFragment(const T* q, U128 (&f)[Kv8Type<T>::
   }
 }
 
+// Queries of 2^100 and more are taken 2^-32 times as large where scores are summed before the key's scale is
+// applied: a sum of 256 products with elements of up to 448 stays finite. Elements that this loses are below
+// 2^-194 of their row's largest.
+constexpr float kLargeQuery = 0x1p100f, kQueryDown = 0x1p-32f, kQueryUp = 0x1p32f;
+
+// Bits 0..14 of the largest magnitude among the halves of w, which are 16-bit floats, or of `most`.
+typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ U16x2 largestHalf(U16x2 most, uint32_t w) {
+  return __builtin_elementwise_max(most, __builtin_bit_cast(U16x2, w & 0x7FFF7FFFu));
+}
+
+// Two bf16 times a power of two, cut to bf16 again.
+__device__ __forceinline__ uint32_t timesBf16(uint32_t w, float f) {
+  return (__float_as_uint(__uint_as_float(w << 16) * f) >> 16) |
+         (__float_as_uint(__uint_as_float(w & 0xFFFF0000u) * f) & 0xFFFF0000u);
+}
+
 // The value of lane 16 g + n in the lanes 16 g .. 16 g + 15; n is a constant once loops are unrolled,
 // and the move becomes an operand of the multiplication it feeds.
 template <int n>
@@ -119,13 +136,13 @@ __device__ __forceinline__ void timesKeys(f32x4 (&s)[4], float factor) {
 
 // The score factor and value scale of the lane's key. nan: neither finite
 struct KeyScales {
-  float k;      // 2^(key scale) * softmax scale * log2(e); NaN where a scale is 255
+  float k;      // 2^(key scale) * the given scale; NaN where a scale is 255
   uint32_t v;   // value scale code, 0 where a scale is 255 or the key is not live
 };
 __device__ __forceinline__ KeyScales keyScales(uint32_t kc, uint32_t vc, bool live,
-                                               float scale_log2) {
+                                               float scale) {
   const bool bad = kc == 255u || vc == 255u;
-  return {mxScaleValue(bad ? 255u : kc) * scale_log2, bad || !live ? 0u : vc};
+  return {mxScaleValue(bad ? 255u : kc) * scale, bad || !live ? 0u : vc};
 }
 
 // 2^(code - top) for code <= top
@@ -327,6 +344,30 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) queryFragment<T>(q + 64 * j + 8 * half, qf[j][half]);
   }
+  // What brings the row's sums back to their size, times the softmax scale: a key's scale alone may then be as
+  // small as it gets. f16 has no queries that large.
+  float q_up = 1.f;
+  bool any_up = false;  // uniform
+  if constexpr (!__is_same(T, f16)) {
+    U16x2 largest = {0, 0};
+#pragma unroll
+    for (int x = 0; x < J * 8; ++x) largest = largestHalf(largest, qf[x / 8][x / 4 % 2][0][x % 4]);
+    const float of_lane = __uint_as_float(
+        static_cast<uint32_t>(largest[0] > largest[1] ? largest[0] : largest[1]) << 16);
+    // one lane of the row is enough; a NaN counts for nothing, its row is NaN in any case
+    const bool up = rowsMax(of_lane) >= kLargeQuery;
+    any_up = __builtin_amdgcn_ballot_w64(up) != 0;
+    if (any_up) {
+      rarely();
+      q_up = (up ? kQueryUp : 1.f) * a.scale_log2;
+      const float down = up ? kQueryDown : 1.f;
+#pragma unroll
+      for (int x = 0; x < J * 8; ++x)
+#pragma unroll
+        for (int u = 0; u < Ty::kQ; ++u)
+          qf[x / 8][x / 4 % 2][u][x % 4] = timesBf16(qf[x / 8][x / 4 % 2][u][x % 4], down);
+    }
+  }
   if constexpr (kSharedQ) {
     if (wave == 0) {
 #pragma unroll
@@ -365,8 +406,13 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
     }
     const bool live = x.live && k0 + lane < most;
     const uint64_t lives = __builtin_amdgcn_ballot_w64(live);
-    const KeyScales sc = keyScales(x.kc, x.vc, live, a.scale_log2);
+    const KeyScales sc = keyScales(x.kc, x.vc, live, any_up ? 1.f : a.scale_log2);
     timesKeys(s, sc.k);
+    if (any_up) {
+      rarely();
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) s[kk] *= q_up;
+    }
     if (lives != ~uint64_t{0} || k0 + kTileK > all_see) {  // uniform
       const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu;
       const int key0 = k0 + 16 * g;
@@ -1311,7 +1357,11 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
     const int64_t bh = row / a.seq_q, b = bh / a.q_heads;
     const int h = static_cast<int>(bh % a.q_heads), kvh = h / (a.q_heads / pg.heads);
     const int lim = visibleKeys(a, kv8First(pg, b), i);
-    for (int d = lane; d < D; d += kWave) q_lds[d] = ld(static_cast<const T*>(a.q) + row * D + d);
+    const T* q = static_cast<const T*>(a.q) + row * D;
+    float largest = 0.f;
+    for (int d = lane; d < D; d += kWave) largest = fmaxf(largest, fabsf(ld(q + d)));
+    const bool up = waveMax(largest) >= kLargeQuery;
+    for (int d = lane; d < D; d += kWave) q_lds[d] = ld(q + d) * (up ? kQueryDown : 1.f);
     __syncthreads();
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     uint32_t top = 0;  // the largest value scale seen, which acc is kept in
@@ -1331,7 +1381,8 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
           float dot = 0.f;
           for (int d = 0; d < D; ++d)
             dot = fmaf(q_lds[d], __builtin_amdgcn_cvt_f32_fp8(k[d], 0), dot);
-          s = dot * (mxScaleValue(kc == 255u || vc == 255u ? 255u : kc) * a.scale_log2);
+          s = dot * mxScaleValue(kc == 255u || vc == 255u ? 255u : kc) *
+              (up ? kQueryUp * a.scale_log2 : a.scale_log2);
           code = vc == 255u ? 0u : vc;
           at = head * D * pg.block_size + slot;
         }

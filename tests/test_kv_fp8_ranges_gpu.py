@@ -131,3 +131,33 @@ def test_queries_that_are_not_finite(dtype, dim, q_heads, seq):
             assert row.isnan().all() if math.isnan(want) else (row == want).all(), (at, x)
             out[0, 0, -1] = plain[0, 0, -1]
             assert torch.equal(out, plain)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim,q_heads,seq", FORMS)
+def test_large_queries_over_small_keys(dtype, dim, q_heads, seq):
+    """Queries of about 2^120 over keys of 2^-126 times their elements: the scores are those of queries and
+    keys that meet in the middle, and so are the results, bit for bit."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 22)
+    pools.key |= 0x48  # elements of 4 and more
+    pools.key[pools.key % 128 == 127] = 0x48
+    pools.scales[:, :, 0] = 121
+    pools.cuda()
+    small = torch.randn((1, q_heads, seq, dim), generator=rng(1)).to(t).cuda()
+    ws = workspace(pools, small)
+    past = 1400 - seq
+    want = [attend(pools, small, past, ws=space) for space in (None, ws)]
+    assert want[0].isfinite().all()
+    pools.scales[:, :, 0] = 1
+    large = small * 2.0 ** 120
+    for space, x in zip((None, ws), want):
+        assert torch.equal(attend(pools, large, past, ws=space), x)
+    # one row of a call, the others as they were
+    pools.scales[:, :, 0] = 121
+    mixed = small.clone()
+    mixed[0, 0, -1] *= 2.0 ** 120
+    for space, x in zip((None, ws), want):
+        out = attend(pools, mixed, past, ws=space)
+        out[0, 0, -1] = x[0, 0, -1]
+        assert torch.equal(out, x)
