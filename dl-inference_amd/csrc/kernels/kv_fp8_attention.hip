@@ -6,10 +6,9 @@
 //   S^T = K Q^T    elements as bf16 (T bf16 and fp32, whose q is the exact sum of three bf16 terms)
 //                  or f16 (T f16); the token's key scale multiplies the score in fp32.
 //   O^T += V^T P^T elements as f16, P as f16: one term (11 bits) where the output is bf16 (8 bits),
-//                  two terms (22 bits) else. A probability is 2^11 at the running reference and at most
-//                  2^15.5, so that f16's normal range reaches down to 2^-25 of the reference. The token's
-//                  value scale, relative to the largest seen, goes into P (few rows) or V (many); the
-//                  running output is kept in units of that largest scale.
+//                  two terms (22 bits) else. The largest is 2^11 to 2^15.5, so that f16's normal range reaches
+//                  down to 2^-25 of it. The token's value scale goes into P (few rows, RowSum), or into V
+//                  relative to the largest seen (many).
 // A token whose row was not finite (scale 255) makes the score NaN, so rows that
 // see it are NaN and rows that do not see it are untouched.
 #include "kv_fp8.h"
@@ -191,6 +190,80 @@ __device__ __forceinline__ void packWeights(const f32x4 (&w)[4], U128 (&f)[kP][2
     }
 }
 
+// A row's softmax and the unit that its output is summed in, as powers of two. Value scales may lie 2^247
+// apart, f16 holds 2^40: weights for the products are taken relative to the largest weight times value scale
+// that the row has seen, so neither a token that it does not see nor one that weighs nothing costs the others
+// a bit.
+struct RowSum {
+  float m = -INFINITY;     // reference of the scores
+  float l = 0.f;           // this lane's part of the sum of 2^(score - m)
+  float unit = 0.f;        // a whole number: the output is sum * 2^(unit - 127)
+  float peak = -INFINITY;  // the largest log2 of a weight in o, at m and unit
+};
+
+// u[n] = s[n] + the scale code of key n - unit
+template <int n = 0>
+__device__ __forceinline__ void inUnit(const f32x4 (&s)[4], float code, float unit, f32x4 (&u)[4]) {
+  if constexpr (n < 16) {
+    u[n / 4][n % 4] = s[n / 4][n % 4] + (rowLane<n>(code) - unit);
+    inUnit<n + 1>(s, code, unit, u);
+  }
+}
+
+__device__ __forceinline__ float largestOf(const f32x4 (&s)[4]) {
+  float most = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < 16; ++n) most = fmaxf(most, s[n / 4][n % 4]);
+  return most;
+}
+
+// Scores of 16 keys (-infinity where masked) -> their weights 2^(score - m + code - unit), between 2^kLift and
+// 2^(kLift + kSlack) at the peak; code: the value scale code of this lane's key. o follows m and unit.
+template <int DT>
+__device__ __forceinline__ void weigh(f32x4 (&s)[4], float code, RowSum& row, f32x4 (&o)[DT]) {
+  FP_EXACT;  // a large score less its reference, in one step with the score's own product, would not be 0
+  const float top = rowsMax(largestOf(s));
+  const bool grow = top > row.m + kSlack;  // false while top is -inf
+  bool changed = __builtin_amdgcn_ballot_w64(grow) != 0;
+  float shift = 0.f;
+  if (changed) {
+    shift = grow ? row.m - top : 0.f;
+    row.m = grow ? top : row.m;
+    row.l *= __builtin_amdgcn_exp2f(shift);  // 0 from -inf
+    row.peak += shift;
+  }
+  // the reference alone first: from 2^24 on its sum with anything is rounded
+  const float base = row.m == -INFINITY ? 0.f : row.m;
+#pragma unroll
+  for (int n = 0; n < 16; ++n) s[n / 4][n % 4] -= base;
+  f32x4 u[4];
+  inUnit(s, code, row.unit, u);
+  row.peak = fmaxf(row.peak, rowsMax(largestOf(u)));
+  // it falls only where the reference moves
+  const bool low = grow && row.peak < kLift && row.peak != -INFINITY;
+  const bool move = row.peak > kLift + kSlack || low;
+  if (__builtin_amdgcn_ballot_w64(move)) {
+    const float by = move ? floorf(row.peak - kLift) : 0.f;
+    row.unit += by;
+    row.peak -= by;
+    shift -= by;
+    changed = true;
+    inUnit(s, code, row.unit, u);
+  }
+  if (changed) {
+    const float alpha = __builtin_amdgcn_exp2f(shift);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int n = 0; n < 16; ++n) {
+    sum += __builtin_amdgcn_exp2f(s[n / 4][n % 4]);
+    s[n / 4][n % 4] = __builtin_amdgcn_exp2f(u[n / 4][n % 4]);
+  }
+  row.l += sum;
+}
+
 // keys that row i of the queries sees, in [0, capacity]
 __device__ __forceinline__ int visibleKeys(const Kv8AttentionArgs& a, int64_t past, int i) {
   const int64_t n = past + (a.causal ? i + 1 : a.seq_q);
@@ -257,9 +330,11 @@ struct DecodeLds {
   // q's terms where there are several: in registers they would push the tiles out (fp32, head_dim 128,
   // 64 sequences of 4096 tokens: 80.7 us with 43 registers spilled, 48.8 so)
   U128 q[Kv8Type<T>::kQ > 1 ? D / 64 * 2 * Kv8Type<T>::kQ : 1][kWave];
+  float row_scale[kWave];
+  int lim[kWave];
   float m[kDecWaves][16];
   float l[kDecWaves][16];
-  uint32_t top[kDecWaves];
+  float unit[kDecWaves][16];
   float o[kDecWaves][D][17];
 };
 
@@ -346,8 +421,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   }
   // What brings the row's sums back to their size, times the softmax scale: a key's scale alone may then be as
   // small as it gets. f16 has no queries that large.
-  float q_up = 1.f;
-  bool any_up = false;  // uniform
+  float row_scale = a.scale_log2;
   if constexpr (!__is_same(T, f16)) {
     U16x2 largest = {0, 0};
 #pragma unroll
@@ -356,10 +430,9 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
         static_cast<uint32_t>(largest[0] > largest[1] ? largest[0] : largest[1]) << 16);
     // one lane of the row is enough; a NaN counts for nothing, its row is NaN in any case
     const bool up = rowsMax(of_lane) >= kLargeQuery;
-    any_up = __builtin_amdgcn_ballot_w64(up) != 0;
-    if (any_up) {
+    if (__builtin_amdgcn_ballot_w64(up)) {
       rarely();
-      q_up = (up ? kQueryUp : 1.f) * a.scale_log2;
+      row_scale *= up ? kQueryUp : 1.f;
       const float down = up ? kQueryDown : 1.f;
 #pragma unroll
       for (int x = 0; x < J * 8; ++x)
@@ -370,6 +443,8 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   }
   if constexpr (kSharedQ) {
     if (wave == 0) {
+      lds.row_scale[lane] = row_scale;
+      lds.lim[lane] = lim;
 #pragma unroll
       for (int x = 0; x < J * 2 * Ty::kQ; ++x)
         lds.q[x][lane] = qf[x / (2 * Ty::kQ)][x / Ty::kQ % 2][x % Ty::kQ];
@@ -381,8 +456,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   };
   const int all_see = visibleKeys(a, past, 0);  // keys that every row sees
 
-  float m = -INFINITY, l = 0.f;
-  uint32_t top = 0;
+  RowSum row;
   f32x4 o[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) o[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -406,51 +480,23 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
     }
     const bool live = x.live && k0 + lane < most;
     const uint64_t lives = __builtin_amdgcn_ballot_w64(live);
-    const KeyScales sc = keyScales(x.kc, x.vc, live, any_up ? 1.f : a.scale_log2);
+    constexpr bool kRowScale = !__is_same(T, f16);
+    const KeyScales sc = keyScales(x.kc, x.vc, live, kRowScale ? 1.f : a.scale_log2);
     timesKeys(s, sc.k);
-    if (any_up) {
-      rarely();
+    if constexpr (kRowScale) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) s[kk] *= q_up;
+      for (int kk = 0; kk < 4; ++kk) s[kk] *= kSharedQ ? lds.row_scale[q_lane] : row_scale;
     }
     if (lives != ~uint64_t{0} || k0 + kTileK > all_see) {  // uniform
       const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu;
-      const int key0 = k0 + 16 * g;
+      const int key0 = k0 + 16 * g, end = kSharedQ ? lds.lim[q_lane] : lim;
 #pragma unroll
       for (int n = 0; n < 16; ++n)
-        if (!(mine >> n & 1u) || key0 + n >= lim) s[n / 4][n % 4] = -INFINITY;
+        if (!(mine >> n & 1u) || key0 + n >= end) s[n / 4][n % 4] = -INFINITY;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) keepBytes(x.v[dt], mine);
     }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < 16; ++n) tmax = fmaxf(tmax, s[n / 4][n % 4]);
-    tmax = rowsMax(tmax);
-    const bool grow = tmax > m + kSlack;  // false while tmax is -inf
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m - tmax) : 1.f;  // 0 from -inf
-      m = grow ? tmax : m;
-      l *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-    }
-    if (__builtin_amdgcn_ballot_w64(sc.v > top)) {
-      const uint32_t next = waveMaxU(sc.v);  // > top
-      const float down = valueFactor(top, next);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[dt] *= down;
-      top = next;
-    }
-    // the reference first: from 2^24 on m - kLift is rounded, and a weight passes f16's largest number
-    const float base = m == -INFINITY ? 0.f : m;
-    float sum = 0.f;
-#pragma unroll
-    for (int n = 0; n < 16; ++n) {
-      s[n / 4][n % 4] = __builtin_amdgcn_exp2f(s[n / 4][n % 4] - base + kLift);
-      sum += s[n / 4][n % 4];
-    }
-    l += sum;
-    timesKeys(s, valueFactor(sc.v, top));
+    weigh(s, static_cast<float>(sc.v), row, o);
     U128 pf[Ty::kP][2];
     packWeights<Ty::kP>(s, pf);
 #pragma unroll
@@ -476,13 +522,13 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
     attend(buf[1], second);
   }
 
-  // join the waves: the row's largest reference and value scale
-  const float l_row = rowsSum(l);
+  // join the waves at the row's largest reference, and the largest unit at it
+  const float l_row = rowsSum(row.l);
   if (g == 0) {
-    lds.m[wave][r] = m;
+    lds.m[wave][r] = row.m;
     lds.l[wave][r] = l_row;
+    lds.unit[wave][r] = row.unit;
   }
-  if (lane == 0) lds.top[wave] = top;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -491,24 +537,24 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
   for (int e = t; e < rows * D; e += kDecWaves * kWave) {
     const int p = e / D, d = e % D;
     float M = -INFINITY;
-    uint32_t high = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWaves; ++w) M = fmaxf(M, lds.m[w][p]);
+    float L = 0.f, unit = -INFINITY, past_m[kDecWaves];
 #pragma unroll
     for (int w = 0; w < kDecWaves; ++w) {
-      M = fmaxf(M, lds.m[w][p]);
-      high = lds.top[w] > high ? lds.top[w] : high;
+      const float m = lds.m[w][p], l = lds.l[w][p];
+      // a wave that saw no key has no part; a NaN sum stays one whatever its reference
+      past_m[w] = m == -INFINITY ? (l == 0.f ? -INFINITY : 0.f) : m - M;
+      L += __builtin_amdgcn_exp2f(past_m[w]) * l;
+      unit = fmaxf(unit, lds.unit[w][p] + rintf(past_m[w]));
     }
-    float L = 0.f, acc = 0.f;
+    float acc = 0.f;
 #pragma unroll
-    for (int w = 0; w < kDecWaves; ++w) {
-      const float f = lds.m[w][p] == -INFINITY ? (lds.l[w][p] == 0.f ? 0.f : 1.f)
-                                               : __builtin_amdgcn_exp2f(lds.m[w][p] - M);
-      L += f * lds.l[w][p];
-      acc += f * valueFactor(lds.top[w], high) * lds.o[w][d][p];
-    }
+    for (int w = 0; w < kDecWaves; ++w)
+      acc += __builtin_amdgcn_exp2f(past_m[w] + (lds.unit[w][p] - unit)) * lds.o[w][d][p];
     const RowAt at = rowAt(p, group, kvh);
-    // 2^(high - 127) * acc / L; the quotient first, so that neither overflows
-    const float result =
-        L == 0.f ? 0.f : __builtin_ldexpf(acc / L, static_cast<int>(high) - 127);
+    // the quotient first, so that neither overflows
+    const float result = L == 0.f ? 0.f : __builtin_ldexpf(acc / L, static_cast<int>(unit) - 127);
     if (a.splits == 1) {
       st(static_cast<T*>(a.out) + outAt(a, b, at, D) + d, result);
     } else {
@@ -1346,6 +1392,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
 // ---------------------------------------------------------------------------------------------
 template <class T>
 __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
+  FP_EXACT;  // as in weigh
   __shared__ float q_lds[256];
   __shared__ float p_lds[kWave];
   __shared__ int64_t at_lds[kWave];
@@ -1364,7 +1411,7 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
     for (int d = lane; d < D; d += kWave) q_lds[d] = ld(q + d) * (up ? kQueryDown : 1.f);
     __syncthreads();
     float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t top = 0;  // the largest value scale seen, which acc is kept in
+    float unit = 0.f, peak = -INFINITY;  // as in RowSum
     for (int j0 = 0; j0 < lim; j0 += kWave) {
       const int j = j0 + lane;
       float s = -INFINITY;
@@ -1389,14 +1436,16 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
       }
       const float next = fmaxf(m, waveMax(s));
       const float base = next == -INFINITY ? 0.f : next;
-      const float p = at >= 0 ? __builtin_amdgcn_exp2f(s - base) : 0.f;
-      const float alpha = __builtin_amdgcn_exp2f(m - base);  // 0 on the first round
-      l = l * alpha + waveSum(p);
+      const float past = s - base, fall = m - base;  // fall: -infinity on the first round
+      l = l * __builtin_amdgcn_exp2f(fall) + waveSum(at >= 0 ? __builtin_amdgcn_exp2f(past) : 0.f);
       m = next;
-      const uint32_t most = waveMaxU(code), high = most > top ? most : top;
-      const float down = alpha * valueFactor(top, high);
-      top = high;
-      p_lds[lane] = p * valueFactor(code, top);
+      const float key_unit = static_cast<float>(code) - unit;
+      peak = fmaxf(peak + fall, waveMax(past + key_unit));  // -infinity where s is
+      const float by = peak == -INFINITY ? 0.f : rintf(peak);
+      unit += by;
+      peak -= by;
+      const float down = __builtin_amdgcn_exp2f(fall - by);
+      p_lds[lane] = at >= 0 ? __builtin_amdgcn_exp2f(past + (key_unit - by)) : 0.f;
       at_lds[lane] = at;
       __syncthreads();
       const int n = lim - j0 < kWave ? lim - j0 : kWave;
@@ -1418,7 +1467,7 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
     for (int u = 0; u < 4; ++u)
       if (lane + u * kWave < D)
         st(out + lane + u * kWave,
-           l == 0.f ? 0.f : __builtin_ldexpf(acc[u] / l, static_cast<int>(top) - 127));
+           l == 0.f ? 0.f : __builtin_ldexpf(acc[u] / l, static_cast<int>(unit) - 127));
   }
 }
 

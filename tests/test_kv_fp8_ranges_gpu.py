@@ -75,6 +75,27 @@ def test_weights_of_large_scores(dtype, dim, q_heads, seq, sign, power):
         close(out, want, t)
 
 
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim,q_heads,seq", FORMS)
+@pytest.mark.parametrize("power", [10, 21, 24, 25, 26, 27, 28, 33, 90])
+def test_equal_large_scores(dtype, dim, q_heads, seq, power):
+    """Two tokens of one score, eight tiles apart, under a softmax scale that rounds it: equal weights."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 30, seed=power)
+    pools.key[:] = 0
+    pools.scales[:, :, 0] = 127 + power - 12
+    pools.scales[:, :, 1] = 127
+    for pos in (70, 582):
+        page, slot = token(pools, 0, pos)
+        pools.key[page, 0, slot, 0] = code(26.0)
+    q = torch.zeros((1, q_heads, seq, dim))
+    q[..., 0] = 2.0 ** 8 * 1.375
+    want = (value_of(pools, 0, 70) + value_of(pools, 0, 582)) / 2
+    pools.cuda()
+    for ws in (None, workspace(pools, q)):
+        close(attend(pools, q.to(t).cuda(), 700, scale=0.2718, ws=ws), want, t)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("dim,q_heads,seq", [(64, 2, 1), (128, 7, 1), (128, 4, 4), (64, 4, 10), (128, 4, 40)])
 @pytest.mark.parametrize("exponent", [247, 246, 235, 0])
@@ -161,3 +182,101 @@ def test_large_queries_over_small_keys(dtype, dim, q_heads, seq):
         out = attend(pools, mixed, past, ws=space)
         out[0, 0, -1] = x[0, 0, -1]
         assert torch.equal(out, x)
+
+
+def dense(pools, tokens):
+    """Keys, value elements and value scales of the one sequence's first tokens, float64: [T, D], [T, D], [T]."""
+    pages = pools.table[0].long().cpu()
+    key, value, scales = (x[pages].cpu() for x in (pools.key, pools.value, pools.scales))
+    k = key[:, 0].view(torch.float8_e4m3fn).double().flatten(0, 1)[:tokens]
+    v = value[:, 0].transpose(1, 2).contiguous().view(torch.float8_e4m3fn).double().flatten(0, 1)[:tokens]
+    unit = torch.exp2(scales[:, 0].double() - 127)  # [pages, 2, block]
+    return k * unit[:, 0].flatten()[:tokens, None], v, unit[:, 1].flatten()[:tokens]
+
+
+def check_far_apart(out, pools, q, past, scale, near=0):
+    """out [1, Hq, S, D] of queries [1, Hq, S, D] (causal), one KV head, against float64. Off by at most: the
+    output's rounding; per weight its rounding (f16 once, or 22 bits) and the shift of its score by fp32's
+    sum of D products, scaling and exponent; the sums' roundings; and f16's half least step, 2^-25 with 2^11
+    or more at the row's largest weight times value scale, for every token's elements. Chunks count
+    from the largest value scale about, which is up to 2^near times that."""
+    t, dim = out.dtype, out.shape[3]
+    k, v, unit = dense(pools, past + q.shape[2])
+    s = q[0].double() @ k.T * scale
+    limit = past + 1 + torch.arange(q.shape[2])
+    s = s.masked_fill(torch.arange(len(k)) >= limit[:, None], -math.inf)
+    w = torch.exp(s - s.amax(-1, keepdim=True))
+    total = w.sum(-1, keepdim=True)
+    want, mag = (w @ (unit[:, None] * x) / total for x in (v, v.abs()))
+    spread = (q[0].double().abs() @ k.abs().T).amax(-1, keepdim=True) * scale
+    floor = (w > 0).double() @ v.abs() * ((w * unit).amax(-1, keepdim=True) / total)
+    eps, tiny = torch.finfo(t).eps, torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    weight = 2.0 ** -12 if t == torch.bfloat16 else 2.0 ** -22
+    shift = 2 * (dim + 8) * 2.0 ** -24 * (spread + 30)
+    sums = (4 * len(k) / 64 + 96) * 2.0 ** -24
+    bound = eps / 2 * want.abs() + (1 + eps) * ((weight + shift + sums) * mag + 2.0 ** (near - 36) * floor) + tiny
+    got = out[0].double().cpu()
+    over = want.abs() > torch.finfo(t).max * (1 + eps / 2)
+    assert (got[over] == want[over].sign() * math.inf).all()
+    edge = (want.abs() + bound > torch.finfo(t).max) & ~over
+    error = (got - want).abs()[~over & ~edge] / bound[~over & ~edge]
+    assert not got[~over].isnan().any()
+    assert (error <= 1).all(), error.max()
+
+
+# value scales against the others': a later token that earlier queries do not see; one seen early on with a
+# weight of 2^-300; one that has the largest weight until the others come; one whose small weight its size
+# makes up for; every token of another size
+APART = ["unseen", "negligible", "at first", "counted", "ladder"]
+
+
+def apart(kind, dtype, dim, q_heads, seq, octaves):
+    """(pools, q): q's element 0 is 1 and k's element 0 chooses a score of a few tokens (in powers of two)."""
+    pools = Pools(1, 1, dim, 64, 30, seed=octaves)
+    pools.key[..., 0] = 0
+    pools.scales[:, :, 0] = 117
+    low = 106 if dtype == "float16" and octaves < 149 else 80  # codes end at 254
+    pools.scales[:, :, 1] = low + torch.randint(0, 3, pools.scales[:, :, 1].shape, generator=rng(3)).to(torch.uint8)
+    q = torch.randn((1, q_heads, seq, dim), generator=rng(seq))
+    q[..., 0] = 1.0
+
+    def place(pos, score, up):
+        page, slot = token(pools, 0, pos)
+        pools.key[page, 0, slot] = 0
+        pools.key[page, 0, slot, 0] = code(math.copysign(1.0, score))
+        pools.scales[page, 0, 0, slot] = 127 + int(math.log2(abs(score)))
+        pools.scales[page, 0, 1, slot] = low + up
+
+    if kind == "unseen":
+        for pos in range(700 + seq - 1, 1920):
+            place(pos, 1.0, octaves)
+    elif kind == "negligible":
+        place(130, -512.0, octaves)
+    elif kind == "at first":
+        place(1, 64.0, octaves)
+        for pos in range(640, 700):
+            place(pos, 256.0, 0)
+    elif kind == "counted":
+        place(300, -float(2 ** int(math.log2(octaves))), octaves)
+    else:
+        size = torch.randint(0, octaves + 1, pools.scales[:, :, 1].shape, generator=rng(9))
+        pools.scales[:, :, 1] = (low + size).to(torch.uint8)
+    return pools, q
+
+
+def far_apart(kind, dtype, dim, q_heads, seq, octaves, near):
+    t = DTYPES[dtype]
+    pools, q = apart(kind, dtype, dim, q_heads, seq, octaves)
+    q = q.to(t)
+    pools.cuda()
+    for space in (None, workspace(pools, q)):
+        out = attend(pools, q.cuda(), 700, scale=math.log(2), ws=space)
+        check_far_apart(out, pools, q, 700, math.log(2), near)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim,q_heads,seq", [f for f in FORMS if f[1] * f[2] <= 16 or f[0] == 80])
+@pytest.mark.parametrize("kind", APART)
+@pytest.mark.parametrize("octaves", [9, 20, 35, 100, 160])
+def test_values_far_apart(dtype, dim, q_heads, seq, kind, octaves):
+    far_apart(kind, dtype, dim, q_heads, seq, octaves, 0)
