@@ -8,7 +8,7 @@
 //   O^T += V^T P^T elements as f16, P as f16: one term (11 bits) where the output is bf16 (8 bits),
 //                  two terms (22 bits) else. The largest is 2^11 to 2^15.5, so that f16's normal range reaches
 //                  down to 2^-25 of it. The token's value scale goes into P (few rows, RowSum), or into V
-//                  relative to the largest seen (many).
+//                  relative to the largest seen (many, if their values are not too far apart: kNear).
 // A token whose row was not finite (scale 255) makes the score NaN, so rows that
 // see it are NaN and rows that do not see it are untouched.
 #include "kv_fp8.h"
@@ -150,13 +150,27 @@ __device__ __forceinline__ float valueFactor(uint32_t code, uint32_t top) {
   return e > 0 ? __uint_as_float(static_cast<uint32_t>(e) << 23) : 0.f;
 }
 
-__device__ __forceinline__ uint32_t waveMaxU(uint32_t v) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) {
-    const uint32_t o = __shfl_xor(v, off, kWave);
-    v = o > v ? o : v;
-  }
-  return v;
+// The largest of the wave's values in each half of a word: over 16 lanes by rotation, then over their rows.
+typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t waveMaxHalves(uint32_t v) {
+  auto larger = [](uint32_t x, uint32_t y) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(U16x2, x),
+                                                                  __builtin_bit_cast(U16x2, y)));
+  };
+  v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, true));
+  v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, true));
+  v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, true));
+  v = larger(v, __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, true));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = larger(a[0], a[1]);
+  const auto c = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(larger(c[0], c[1]));
+}
+
+// t for a second run over the same work: what the first computed from it is not kept in registers.
+__device__ __forceinline__ int againOf(int t) {
+  asm volatile("" : "+v"(t));
+  return t;
 }
 
 // In a branch that is seldom taken: keeps the compiler from computing both sides and selecting.
@@ -660,23 +674,36 @@ __device__ __forceinline__ U128 scaledKey(uint32_t w0, uint32_t w1, float scale)
       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true))};
 }
 
-// Rows first .. first + 16 QB - 1 of a wave, o in units of the value scale top: stored, or left with their
-// maximum and sum for the join.
+// A row's sum of weights 2^(score - m) and its reference m; its output is o / l * 2^e.
+struct RowEnd {
+  float l, m;
+  int e;
+};
+
+// Of rows weighed by their reference and shift, o in units of the value scale top; sum: their lifted sum.
+__device__ __forceinline__ RowEnd endOf(float sum, float ref, float shift, float scale, uint32_t top) {
+  // the shift is what the weights have in them, but for far rows
+  return {__builtin_ldexpf(sum, -static_cast<int>(kLift)), farRow(shift) ? ref * scale : kLift - shift,
+          static_cast<int>(top) - 127 - kValueLift - static_cast<int>(kLift)};
+}
+__device__ __forceinline__ RowEnd endOf(const RowSum& row) {
+  return {rowsSum(row.l), row.m, static_cast<int>(row.unit) - 127};
+}
+
+// Rows first .. first + 16 QB - 1 of a wave: stored, or left with their maximum and sum for the join.
 template <class T, int D, int QB>
 __device__ __forceinline__ void storeRows(const Kv8AttentionArgs& a, int b, int kvh, int group, int rows,
                                           int first, const f32x4 (&o)[QB][D / 16],
-                                          const f32x4 (&ls)[QB], const float (&shift)[QB],
-                                          uint32_t top) {
+                                          const RowEnd (&end)[QB]) {
   constexpr int DT = D / 16;
   const int lane = threadIdx.x % kWave, r = lane % 16, g = lane / 16;
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const float L = __shfl(ls[qb][0], r, kWave);
-    const int p = first + qb * 16 + r;
+    const float L = end[qb].l;
+    const int p = first + qb * 16 + r, e = end[qb].e;
     if (p >= rows) continue;
     const RowAt at = rowAt(p, group, kvh);
     const float inv = L == 0.f ? 0.f : 1.f / L;  // no key, or none of any weight: zeros
-    const int e = static_cast<int>(top) - 127 - kValueLift;
     if (a.splits == 1) {
       T* out = static_cast<T*>(a.out) + outAt(a, b, at, D) + 4 * g;
 #pragma unroll
@@ -687,7 +714,7 @@ __device__ __forceinline__ void storeRows(const Kv8AttentionArgs& a, int b, int 
     } else {
       const int64_t part = queryAt(a, b, at, 1) * a.splits + blockIdx.z;
       if (g == 0) {
-        a.part_ml[part * 2] = L == 0.f ? -INFINITY : fminf(kLift - shift[qb], kNoReference);
+        a.part_ml[part * 2] = L == 0.f ? -INFINITY : fminf(end[qb].m, kNoReference);
         a.part_ml[part * 2 + 1] = L;
       }
       float* out = a.part_o + part * D + 4 * g;
@@ -700,6 +727,31 @@ __device__ __forceinline__ void storeRows(const Kv8AttentionArgs& a, int b, int 
   }
 }
 
+// How far apart the value scales of a workgroup's keys may lie (powers of two) for V to be staged relative to
+// the largest: its elements are exact in f16 down to 2^-22, and a weight is one down to 2^-36 of its row's
+// largest, so what is lost is below 2^-22 of the smallest scale an element. Past that the workgroup starts again
+// with weights in units of their rows (RowSum): 2048 tokens over 8192 take 712 us in place of 294, 4 x 2048
+// prompt tokens (14 / 2 x 64) 107 in place of 53. Scale code 0 is left out, since rows of zeros have it: next
+// to a value scale above 2^-113 such rows, which are below 2^-118, may count for zeros.
+constexpr uint32_t kNear = 14;
+struct ValueScales {  // uniform
+  uint32_t top = 0, bottom = 255;  // of the codes seen so far
+  // Whether the lanes' codes (0 for keys that are not there) lie outside what was seen.
+  __device__ __forceinline__ bool news(uint32_t code) const {
+    return __builtin_amdgcn_ballot_w64(code > top || (code != 0 && code < bottom)) != 0;
+  }
+  // Takes them in; 2^(top before - top).
+  __device__ __forceinline__ float add(uint32_t code) {
+    const uint32_t before = top;
+    const uint32_t most = waveMaxHalves(code | (code != 0 ? 255u - code : 0u) << 16);
+    const uint32_t high = most & 0xFFFFu, low = 255u - (most >> 16);
+    top = high > top ? high : top;
+    bottom = low < bottom ? low : bottom;
+    return valueFactor(before, top);
+  }
+  __device__ __forceinline__ bool apart() const { return top > bottom + kNear; }
+};
+
 template <int D>
 struct ChunkLds {
   uint16_t k[2][kTileK * D];
@@ -708,17 +760,18 @@ struct ChunkLds {
   uint16_t vf[kChunkWaves][kTileK];  // and of the value factors
 };
 
-template <class T, int D, int QB, bool kSmall>
-__device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
+// kInRows: weights in units of their rows. Returns false, the same in every wave and with nothing stored, where
+// the other form finds value scales too far apart. t: the thread.
+template <class T, int D, int QB, bool kSmall, bool kInRows>
+__device__ __forceinline__ bool kv8_chunk_rows(const Kv8AttentionArgs& a, ChunkLds<D>& lds, const int t) {
   using Ty = Kv8Type<T>;
   // f16 keys stay unscaled (their range would not hold a scaled one), the score takes the scale
   constexpr bool kScaleKeys = !__is_same(T, f16);
   constexpr int DT = D / 16, DK = D / 32, kThreads = kChunkWaves * kWave, kRows = 16 * QB * kChunkWaves;
   constexpr int kParts = D / 16;         // 16-code chunks of a key
   constexpr int kPer = 4 * D / kThreads;  // chunks of K, and of V^T, a thread
-  __shared__ __attribute__((aligned(16))) ChunkLds<D> lds;
   const Kv8Pages& pg = a.pages;
-  const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int r = lane % 16, g = lane / 16;
   const int group = a.q_heads / pg.heads, rows = a.seq_q * group, bs = pg.block_size;
   // the pair is the fast index (consecutive workgroups go to different XCDs), the row tile the slow
@@ -836,12 +889,17 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     for (int i = 0; i < kPer; ++i) vr[i] = gload16(vb + vo[i]);
   };
 
+  const float score_scale = kScaleKeys ? a.scale_log2 : 1.f;
+  const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
+  const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
+
   f32x4 o[QB][DT];
-  f32x4 ls[QB];        // element 0 of the lanes g = 0: the sum of row r's weights
-  float shift[QB];     // kLift less the row's reference, times the scale
-  float ref[QB];       // the reference, a score
-  bool far = false;    // a row of the wave has been farRow
-  uint32_t top = 0;    // the largest value scale seen, which o is kept in
+  f32x4 ls[QB];      // element 0 of the lanes g = 0: the sum of row r's weights
+  float shift[QB];   // kLift less the row's reference, times the scale
+  float ref[QB];     // the reference, a score
+  bool far = false;  // a row of the wave has been farRow
+  ValueScales scales;  // o is kept in units of the largest
+  RowSum row[QB];    // in place of these where kInRows
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     shift[qb] = kNoReference;
@@ -850,10 +908,6 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[qb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const float score_scale = kScaleKeys ? a.scale_log2 : 1.f;
-  const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
-  const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
-
   Where at{};
   auto fetch = [&] {
     at = takeIds();
@@ -866,25 +920,27 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
     loadIds();
     fetch();
   }
-  for (int kt = kt0; kt < kt1; ++kt) {
+  int end = kt1;
+  for (int kt = kt0; kt < end; ++kt) {
     const int k0 = kt * kTileK, buf = kt & 1;
     const bool live = in_page && k0 + lane < wg_keys;
     const bool bad = kc == 255u || vc == 255u;
     const uint64_t lives = __builtin_amdgcn_ballot_w64(live);
     const uint64_t bads = __builtin_amdgcn_ballot_w64(live && bad);
     const uint32_t vcode = bad || !live ? 0u : vc;
-    if (__builtin_amdgcn_ballot_w64(vcode > top)) {  // every wave comes to the same
-      const uint32_t next = waveMaxU(vcode);
-      const float down = valueFactor(top, next);
+    if constexpr (!kInRows) {
+      if (scales.news(vcode)) {  // every wave comes to the same
+        const float down = scales.add(vcode);
+        if (scales.apart()) end = kt;  // the last tile
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
+        for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= down;
-      top = next;
+          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= down;
+      }
+      lds.vf[wave][lane] = valueFactorF16(vcode, scales.top);
     }
     const float kf = mxScaleValue(bad ? 255u : kc) * (kScaleKeys ? 1.f : a.scale_log2);
     if constexpr (kScaleKeys) lds.kf[wave][lane] = kf;
-    lds.vf[wave][lane] = valueFactorF16(vcode, top);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' factors are read below
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -908,7 +964,11 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
       *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(row, 2 * part)]) = k0v;
       *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(row, 2 * part + 1)]) = k1v;
     }
-    const U128 vf0 = load16(&lds.vf[wave][16 * (t % 4)]), vf1 = load16(&lds.vf[wave][16 * (t % 4) + 8]);
+    U128 vf[2];
+    if constexpr (!kInRows) {
+      vf[0] = load16(&lds.vf[wave][16 * (t % 4)]);
+      vf[1] = load16(&lds.vf[wave][16 * (t % 4) + 8]);
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int d = chunkOf(i) / 4, run = t % 4;
@@ -916,8 +976,12 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
         rarely();
         keepBytes(vr[i], static_cast<uint32_t>(lives >> (16 * run)) & 0xFFFFu);
       }
-      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, run, 0)]) = valueFragment(vr[i][0], vr[i][1], vf0);
-      *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, run, 1)]) = valueFragment(vr[i][2], vr[i][3], vf1);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t w0 = vr[i][2 * half], w1 = vr[i][2 * half + 1];
+        *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(d, run, half)]) =
+            kInRows ? codesToF16(w0, w1) : valueFragment(w0, w1, vf[half]);
+      }
     }
     fetch();
     // one barrier a tile: the other buffer was last read before the previous one
@@ -954,6 +1018,10 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       if constexpr (!kScaleKeys) timesKeys(s[qb], kf);
+      if constexpr (kInRows && kScaleKeys) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) s[qb][kk] *= score_scale;
+      }
       if (!full) {
         const int seen = lim[qb] - k0 - 16 * g;
         const uint32_t mine = static_cast<uint32_t>(lives >> (16 * g)) & 0xFFFFu &
@@ -962,32 +1030,34 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
         for (int n = 0; n < 16; ++n)
           if (!(mine >> n & 1u)) s[qb][n / 4][n % 4] = -INFINITY;
       }
-      float smax = -INFINITY;
+      if constexpr (kInRows) {
+        weigh(s[qb], static_cast<float>(vcode), row[qb], o[qb]);
+      } else {
+        const float smax = largestOf(s[qb]);
+        // the reference moves only when a weight would pass 2^(kLift + kSlack)
+        bool over = fmaf(smax, score_scale, shift[qb]) > kLift + kSlack;
+        if (far) {
+          rarely();
+          over = farExponent(smax, ref[qb], shift[qb], score_scale) > kLift + kSlack;
+        }
+        if (__builtin_amdgcn_ballot_w64(over)) {
+          rarely();
+          const float alpha = moveReference(smax, score_scale, ref[qb], shift[qb]);
+          far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
+          ls[qb] *= alpha;
 #pragma unroll
-      for (int n = 0; n < 16; ++n) smax = fmaxf(smax, s[qb][n / 4][n % 4]);
-      // the reference moves only when a weight would pass 2^(kLift + kSlack)
-      bool over = fmaf(smax, score_scale, shift[qb]) > kLift + kSlack;
-      if (far) {
-        rarely();
-        over = farExponent(smax, ref[qb], shift[qb], score_scale) > kLift + kSlack;
-      }
-      if (__builtin_amdgcn_ballot_w64(over)) {
-        rarely();
-        const float alpha = moveReference(smax, score_scale, ref[qb], shift[qb]);
-        far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
-        ls[qb] *= alpha;
+          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+        }
+        float to_lift = shift[qb];
+        if (far) {
+          rarely();
+          to_lift = fromReference(s[qb], ref[qb], shift[qb]);
+        }
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+        for (int n = 0; n < 16; ++n)
+          s[qb][n / 4][n % 4] =
+              __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], score_scale, to_lift));
       }
-      float to_lift = shift[qb];
-      if (far) {
-        rarely();
-        to_lift = fromReference(s[qb], ref[qb], shift[qb]);
-      }
-#pragma unroll
-      for (int n = 0; n < 16; ++n)
-        s[qb][n / 4][n % 4] =
-            __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], score_scale, to_lift));
       packWeights<Ty::kP>(s[qb], pf[qb]);
     }
 #pragma unroll
@@ -1000,14 +1070,28 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
       for (int u = Ty::kP - 1; u >= 0; --u)
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-          if (i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][u][i / DT], ls[qb]);
+          if (!kInRows && i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][u][i / DT], ls[qb]);
           o[qb][i % DT] = F16::mma(frag[i % (kAhead + 1)], pf[qb][u][i / DT], o[qb][i % DT]);
         }
     }
     __builtin_amdgcn_sched_barrier(0);
   }
+  if (scales.apart()) return false;
+  RowEnd ends[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+    ends[qb] = kInRows ? endOf(row[qb])
+                       : endOf(__shfl(ls[qb][0], r, kWave), ref[qb], shift[qb], score_scale, scales.top);
+  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ends);
+  return true;
+}
 
-  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ls, shift, top);
+template <class T, int D, int QB, bool kSmall>
+__device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
+  __shared__ __attribute__((aligned(16))) ChunkLds<D> lds;
+  if (kv8_chunk_rows<T, D, QB, kSmall, false>(a, lds, threadIdx.x)) return;
+  __syncthreads();  // waves still read the last tile
+  kv8_chunk_rows<T, D, QB, kSmall, true>(a, lds, againOf(threadIdx.x));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1042,14 +1126,15 @@ struct Products {
   static constexpr bool kKeys = kBoth;
 };
 
-__device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
+// As kv8_chunk_rows.
+template <bool kInRows>
+__device__ __forceinline__ bool kv8_phased_rows(const Kv8AttentionArgs& a, PhasedLds<128>& lds, const int t) {
   using T = bf16;
   constexpr int D = 128, QB = 2, DT = D / 16, DK = D / 32, kRows = 16 * QB * kPhasedWaves;
   constexpr int kParts = D / 16;  // 16-code chunks of a key; a thread stages one of K and one of V^T
   static_assert(kTileK * kParts == kPhasedWaves * kWave);
-  __shared__ __attribute__((aligned(16))) PhasedLds<D> lds;
   const Kv8Pages& pg = a.pages;
-  const int t = threadIdx.x, lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int lane = t % kWave, wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int r = lane % 16, g = lane / 16;
   const int group = a.q_heads / pg.heads, rows = a.seq_q * group, bs = pg.block_size;
   // pairs, row tiles and clamped rows as in kv8_chunk
@@ -1132,6 +1217,7 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
   };
 
   f32x4 o[QB][DT];
+  RowSum row[QB];   // in place of the next four where kInRows
   f32x4 ls[QB];     // element 0 of the lanes g = 0: the sum of row r's weights
   float shift[QB];  // kLift less the row's reference, times the scale
   float ref[QB];    // the reference, a score
@@ -1150,17 +1236,22 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
   const uint32_t one = r == 0 ? 0x3C003C00u : 0u;
   const U128 ones = U128{one, one, one, one};  // A fragment of one row of ones
 
-  // The largest value scale up to the tile whose factors were written last, up to the one before, and
+  // The value scales up to the tile whose factors were written last, the largest up to the one before, and
   // the one that o is kept in.
-  uint32_t top = 0, top_before = 0, top_o = 0;
-  auto factors = [&](int kt, bool there, uint32_t code) {  // of tile kt
-    code = code == 255u || !there || kt * kTileK + lane >= wg_keys ? 0u : code;
-    top_before = top;
-    if (__builtin_amdgcn_ballot_w64(code > top)) {  // every wave comes to the same
+  ValueScales seen_scales;
+  uint32_t top_before = 0, top_o = 0;
+  auto codeIn = [&](int kt, bool there, uint32_t code) {  // this lane's of tile kt, 0 where nothing is
+    return code == 255u || !there || kt * kTileK + lane >= wg_keys ? 0u : code;
+  };
+  auto factors = [&](int kt, bool there, uint32_t raw) {  // of tile kt
+    if constexpr (kInRows) return;
+    const uint32_t code = codeIn(kt, there, raw);
+    top_before = seen_scales.top;
+    if (seen_scales.news(code)) {  // every wave comes to the same
       rarely();
-      top = waveMaxU(code);
+      seen_scales.add(code);
     }
-    lds.vf[wave][lane] = valueFactorF16(code, top);
+    lds.vf[wave][lane] = valueFactorF16(code, seen_scales.top);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // other lanes' factors are read
   };
   uint64_t lives = 0;  // the keys of the tile staged last that are there
@@ -1179,16 +1270,19 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
     *reinterpret_cast<U128*>(&lds.k[buf][keyChunk<D>(key_row, 2 * part + half)]) = w;
   };
   auto stageValues = [&](int buf, int half) {
+    const uint32_t w0 = vr[2 * half], w1 = vr[2 * half + 1];
     *reinterpret_cast<U128*>(&lds.v[buf][valueChunk(dim, run, half)]) =
-        valueFragment(vr[2 * half], vr[2 * half + 1], vf[half]);
+        kInRows ? codesToF16(w0, w1) : valueFragment(w0, w1, vf[half]);
   };
   // The keys of kt + 1 and the values of kt, in pieces that fit between products.
   constexpr int kPieces = 5, kPieceSteps = 3;
   auto stage = [&](int kt, int piece) {
     const int vbuf = kt & 1, kbuf = vbuf ^ 1;
     if (piece == 0) {
-      vf[0] = load16(&lds.vf[wave][16 * run]);
-      vf[1] = load16(&lds.vf[wave][16 * run + 8]);
+      if constexpr (!kInRows) {
+        vf[0] = load16(&lds.vf[wave][16 * run]);
+        vf[1] = load16(&lds.vf[wave][16 * run + 8]);
+      }
       const int n = wg_keys - kt * kTileK;
       lives = !in_before || n <= 0 ? uint64_t{0} : n >= kTileK ? ~uint64_t{0} : (uint64_t{1} << n) - 1;
     } else if (piece == 1) {
@@ -1236,7 +1330,7 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         if (i < kValueSteps) {
-          if (i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][0][i / DT], ls[qb]);
+          if (!kInRows && i % DT == 0) ls[qb] = F16::mma(ones, pf[qb][0][i / DT], ls[qb]);
           o[qb][i % DT] = F16::mma(f, pf[qb][0][i / DT], o[qb][i % DT]);
         } else {
           const int n = i - kValueSteps;
@@ -1267,7 +1361,14 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
       products(kt, Products<true>{});
       __builtin_amdgcn_s_setprio(0);
       __syncthreads();
+      const float code = static_cast<float>(codeIn(kt, in_before, vc_before));
       fetch();
+      if constexpr (kInRows) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) s[qb][kk] *= a.scale_log2;
+      }
       if (lives != ~uint64_t{0} || k0 + kTileK > wave_full) {
         rarely();
 #pragma unroll
@@ -1280,49 +1381,57 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
             if (!(mine >> n & 1u)) s[qb][n / 4][n % 4] = -INFINITY;
         }
       }
-      float most[QB];
-      bool over = false;
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        most[qb] = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < 16; ++n) most[qb] = fmaxf(most[qb], s[qb][n / 4][n % 4]);
-        over |= fmaf(most[qb], a.scale_log2, shift[qb]) > kLift + kSlack;
-      }
-      if (far) {
-        rarely();
-        over = false;
-#pragma unroll
-        for (int qb = 0; qb < QB; ++qb)
-          over |= farExponent(most[qb], ref[qb], shift[qb], a.scale_log2) > kLift + kSlack;
-      }
-      // the references move only when a weight would pass 2^(kLift + kSlack)
-      if (__builtin_amdgcn_ballot_w64(over)) {
-        rarely();
+      if constexpr (kInRows) {
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb) {
-          const float alpha = moveReference(most[qb], a.scale_log2, ref[qb], shift[qb]);
-          far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
-          ls[qb] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+          weigh(s[qb], code, row[qb], o[qb]);
+          packWeights<1>(s[qb], pf[qb]);
         }
-      }
-      float to_lift[QB];
+      } else {
+        float most[QB];
+        bool over = false;
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) to_lift[qb] = shift[qb];
-      if (far) {
-        rarely();
+        for (int qb = 0; qb < QB; ++qb) {
+          most[qb] = -INFINITY;
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) to_lift[qb] = fromReference(s[qb], ref[qb], shift[qb]);
-      }
+          for (int n = 0; n < 16; ++n) most[qb] = fmaxf(most[qb], s[qb][n / 4][n % 4]);
+          over |= fmaf(most[qb], a.scale_log2, shift[qb]) > kLift + kSlack;
+        }
+        if (far) {
+          rarely();
+          over = false;
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
+          for (int qb = 0; qb < QB; ++qb)
+            over |= farExponent(most[qb], ref[qb], shift[qb], a.scale_log2) > kLift + kSlack;
+        }
+        // the references move only when a weight would pass 2^(kLift + kSlack)
+        if (__builtin_amdgcn_ballot_w64(over)) {
+          rarely();
 #pragma unroll
-        for (int n = 0; n < 16; ++n)
-          s[qb][n / 4][n % 4] =
-              __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], a.scale_log2, to_lift[qb]));
-        packWeights<1>(s[qb], pf[qb]);
+          for (int qb = 0; qb < QB; ++qb) {
+            const float alpha = moveReference(most[qb], a.scale_log2, ref[qb], shift[qb]);
+            far = far || __builtin_amdgcn_ballot_w64(farRow(shift[qb])) != 0;
+            ls[qb] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[qb][dt] *= alpha;
+          }
+        }
+        float to_lift[QB];
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) to_lift[qb] = shift[qb];
+        if (far) {
+          rarely();
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) to_lift[qb] = fromReference(s[qb], ref[qb], shift[qb]);
+        }
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            s[qb][n / 4][n % 4] =
+                __builtin_amdgcn_exp2f(fmaf(s[qb][n / 4][n % 4], a.scale_log2, to_lift[qb]));
+          packWeights<1>(s[qb], pf[qb]);
+        }
       }
       factors(kt + 1, in_before, vc_before);
       __syncthreads();
@@ -1330,7 +1439,21 @@ __device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
     products(kt1, Products<false>{});
     if (!late) __syncthreads();
   }
-  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ls, shift, top_o);
+  if (seen_scales.apart()) return false;
+  RowEnd ends[QB];
+#pragma unroll
+  for (int qb = 0; qb < QB; ++qb)
+    ends[qb] = kInRows ? endOf(row[qb])
+                       : endOf(__shfl(ls[qb][0], r, kWave), ref[qb], shift[qb], a.scale_log2, top_o);
+  storeRows<T, D, QB>(a, b, kvh, group, rows, pw, o, ends);
+  return true;
+}
+
+__device__ __forceinline__ void kv8_phased(const Kv8AttentionArgs& a) {
+  __shared__ __attribute__((aligned(16))) PhasedLds<128> lds;
+  if (kv8_phased_rows<false>(a, lds, threadIdx.x)) return;
+  __syncthreads();  // waves still read the last tile
+  kv8_phased_rows<true>(a, lds, againOf(threadIdx.x));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1473,13 +1596,14 @@ __device__ __forceinline__ void kv8_rows(const Kv8AttentionArgs& a) {
 
 }  // namespace
 
-// 64 or 128 rows a workgroup
-#define KV8_CHUNK(suffix, T, D, ROWS)                                                           \
-  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, 2)                           \
+// 64 or 128 rows a workgroup. WAVES of a SIMD at least: what LDS allows with head_dim 128, and with 64 what
+// the registers that the loop needs do.
+#define KV8_CHUNK(suffix, T, D, ROWS, WAVES)                                                     \
+  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, WAVES)                       \
       kv8_chunk_d##D##_r##ROWS##_##suffix(Kv8AttentionArgs a) {                                 \
     kv8_chunk<T, D, ROWS / 64, false>(a);                                                       \
   }                                                                                             \
-  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, 2)                           \
+  extern "C" __global__ void __launch_bounds__(kChunkWaves* kWave, WAVES)                       \
       kv8_chunk_small_d##D##_r##ROWS##_##suffix(Kv8AttentionArgs a) {                           \
     kv8_chunk<T, D, ROWS / 64, true>(a);                                                        \
   }
@@ -1517,15 +1641,15 @@ KV8_ATTENTION(bf16, bf16)
 KV8_ATTENTION(f16, f16)
 
 // attentionPlan (csrc/hip/kv_fp8_ops.cc) chooses the rows
-KV8_CHUNK(f32, float, 64, 64)
-KV8_CHUNK(f32, float, 128, 64)
-KV8_CHUNK(bf16, bf16, 64, 64)
-KV8_CHUNK(bf16, bf16, 64, 128)
-KV8_CHUNK(bf16, bf16, 128, 64)
-KV8_CHUNK(bf16, bf16, 128, 128)
-KV8_CHUNK(f16, f16, 64, 64)
-KV8_CHUNK(f16, f16, 128, 64)
-KV8_CHUNK(f16, f16, 128, 128)
+KV8_CHUNK(f32, float, 64, 64, 3)
+KV8_CHUNK(f32, float, 128, 64, 2)
+KV8_CHUNK(bf16, bf16, 64, 64, 4)
+KV8_CHUNK(bf16, bf16, 64, 128, 3)
+KV8_CHUNK(bf16, bf16, 128, 64, 2)
+KV8_CHUNK(bf16, bf16, 128, 128, 2)
+KV8_CHUNK(f16, f16, 64, 64, 4)
+KV8_CHUNK(f16, f16, 128, 64, 2)
+KV8_CHUNK(f16, f16, 128, 128, 2)
 extern "C" __global__ void __launch_bounds__(kPhasedWaves* kWave, 1)
     kv8_phased_d128_bf16(Kv8AttentionArgs a) {
   kv8_phased(a);

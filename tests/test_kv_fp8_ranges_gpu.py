@@ -186,8 +186,8 @@ def test_large_queries_over_small_keys(dtype, dim, q_heads, seq):
 
 def dense(pools, tokens):
     """Keys, value elements and value scales of the one sequence's first tokens, float64: [T, D], [T, D], [T]."""
-    pages = pools.table[0].long().cpu()
-    key, value, scales = (x[pages].cpu() for x in (pools.key, pools.value, pools.scales))
+    pages = pools.table[0].long().cuda()
+    key, value, scales = (x.cuda()[pages] for x in (pools.key, pools.value, pools.scales))
     k = key[:, 0].view(torch.float8_e4m3fn).double().flatten(0, 1)[:tokens]
     v = value[:, 0].transpose(1, 2).contiguous().view(torch.float8_e4m3fn).double().flatten(0, 1)[:tokens]
     unit = torch.exp2(scales[:, 0].double() - 127)  # [pages, 2, block]
@@ -201,10 +201,11 @@ def check_far_apart(out, pools, q, past, scale, near=0):
     or more at the row's largest weight times value scale, for every token's elements. Chunks count
     from the largest value scale about, which is up to 2^near times that."""
     t, dim = out.dtype, out.shape[3]
+    q = q.cuda()
     k, v, unit = dense(pools, past + q.shape[2])
     s = q[0].double() @ k.T * scale
-    limit = past + 1 + torch.arange(q.shape[2])
-    s = s.masked_fill(torch.arange(len(k)) >= limit[:, None], -math.inf)
+    limit = past + 1 + torch.arange(q.shape[2], device="cuda")
+    s = s.masked_fill(torch.arange(len(k), device="cuda") >= limit[:, None], -math.inf)
     w = torch.exp(s - s.amax(-1, keepdim=True))
     total = w.sum(-1, keepdim=True)
     want, mag = (w @ (unit[:, None] * x) / total for x in (v, v.abs()))
@@ -215,8 +216,10 @@ def check_far_apart(out, pools, q, past, scale, near=0):
     shift = 2 * (dim + 8) * 2.0 ** -24 * (spread + 30)
     sums = (4 * len(k) / 64 + 96) * 2.0 ** -24
     bound = eps / 2 * want.abs() + (1 + eps) * ((weight + shift + sums) * mag + 2.0 ** (near - 36) * floor) + tiny
-    got = out[0].double().cpu()
-    over = want.abs() > torch.finfo(t).max * (1 + eps / 2)
+    got = out[0].double()
+    # infinite where no value within the bound rounds to a finite one; of any such kind where some do (a sum of
+    # large terms that cancel)
+    over = want.abs() - bound > torch.finfo(t).max * (1 + eps / 2)
     assert (got[over] == want[over].sign() * math.inf).all()
     edge = (want.abs() + bound > torch.finfo(t).max) & ~over
     error = (got - want).abs()[~over & ~edge] / bound[~over & ~edge]
@@ -230,13 +233,14 @@ def check_far_apart(out, pools, q, past, scale, near=0):
 APART = ["unseen", "negligible", "at first", "counted", "ladder"]
 
 
-def apart(kind, dtype, dim, q_heads, seq, octaves):
+def apart(kind, dtype, dim, q_heads, seq, octaves, block=64, tokens=1920):
     """(pools, q): q's element 0 is 1 and k's element 0 chooses a score of a few tokens (in powers of two)."""
-    pools = Pools(1, 1, dim, 64, 30, seed=octaves)
+    pools = Pools(1, 1, dim, block, tokens // block, seed=octaves)
     pools.key[..., 0] = 0
     pools.scales[:, :, 0] = 117
     low = 106 if dtype == "float16" and octaves < 149 else 80  # codes end at 254
-    pools.scales[:, :, 1] = low + torch.randint(0, 3, pools.scales[:, :, 1].shape, generator=rng(3)).to(torch.uint8)
+    near = torch.randint(0, 3, pools.scales[:, :, 1].shape, generator=rng(3))
+    pools.scales[:, :, 1] = (low + near).to(torch.uint8)
     q = torch.randn((1, q_heads, seq, dim), generator=rng(seq))
     q[..., 0] = 1.0
 
@@ -248,7 +252,7 @@ def apart(kind, dtype, dim, q_heads, seq, octaves):
         pools.scales[page, 0, 1, slot] = low + up
 
     if kind == "unseen":
-        for pos in range(700 + seq - 1, 1920):
+        for pos in range(700 + seq - 1, tokens):
             place(pos, 1.0, octaves)
     elif kind == "negligible":
         place(130, -512.0, octaves)
@@ -264,13 +268,13 @@ def apart(kind, dtype, dim, q_heads, seq, octaves):
     return pools, q
 
 
-def far_apart(kind, dtype, dim, q_heads, seq, octaves, near):
+def far_apart(kind, dtype, dim, q_heads, seq, octaves, near, **more):
     t = DTYPES[dtype]
-    pools, q = apart(kind, dtype, dim, q_heads, seq, octaves)
+    pools, q = apart(kind, dtype, dim, q_heads, seq, octaves, **more)
     q = q.to(t)
     pools.cuda()
     for space in (None, workspace(pools, q)):
-        out = attend(pools, q.cuda(), 700, scale=math.log(2), ws=space)
+        out = attend(pools, q.cuda(), [700], scale=math.log(2), ws=space)
         check_far_apart(out, pools, q, 700, math.log(2), near)
 
 
@@ -280,3 +284,28 @@ def far_apart(kind, dtype, dim, q_heads, seq, octaves, near):
 @pytest.mark.parametrize("octaves", [9, 20, 35, 100, 160])
 def test_values_far_apart(dtype, dim, q_heads, seq, kind, octaves):
     far_apart(kind, dtype, dim, q_heads, seq, octaves, 0)
+
+
+# (dtype, head_dim, query heads, queries, tokens of a page): chunks of 64 and of 128 rows
+CHUNKS = [("float32", 64, 4, 10, 64), ("float32", 128, 4, 40, 32), ("bfloat16", 64, 4, 40, 64),
+          ("bfloat16", 128, 4, 10, 16), ("float16", 64, 4, 10, 32), ("float16", 128, 4, 40, 64),
+          ("bfloat16", 64, 14, 1200, 64), ("bfloat16", 128, 14, 1200, 64), ("bfloat16", 64, 14, 1200, 32),
+          ("bfloat16", 128, 14, 1200, 16), ("float16", 128, 41, 1200, 64), ("float16", 128, 41, 1200, 32),
+          ("float32", 128, 2, 1200, 64)]
+
+
+@pytest.mark.parametrize("dtype,dim,q_heads,seq,block", CHUNKS)
+@pytest.mark.parametrize("kind", APART)
+@pytest.mark.parametrize("octaves", [9, 13, 20, 35, 100, 160])
+def test_values_far_apart_in_chunks(dtype, dim, q_heads, seq, block, kind, octaves):
+    """Scales of up to 2^14 of each other are taken relative to the largest, others by the row."""
+    # the others lie within 2^2 of each other
+    far_apart(kind, dtype, dim, q_heads, seq, octaves, min(octaves + 2, 14), block=block)
+
+
+@pytest.mark.parametrize("kind", APART)
+@pytest.mark.parametrize("octaves", [9, 13, 20, 35, 100, 160])
+@pytest.mark.parametrize("block", [64, 128])
+def test_values_far_apart_over_long_contexts(kind, octaves, block):
+    """The same where two halves of a workgroup run a phase apart (16800 rows of a pair, up to 2688 tokens)."""
+    far_apart(kind, "bfloat16", 128, 14, 1200, octaves, min(octaves + 2, 14), block=block, tokens=2688)
