@@ -329,23 +329,33 @@ std::pair<Tensor, Tensor> KVCache::read(const std::string& name, std::int64_t st
   // the blocks that hold the positions: [B, blocks, H, ..] -> [B, H, tokens, D]
   const std::int64_t first = length > 0 ? start / e->block_size : 0;
   const std::int64_t blocks = length > 0 ? (start + length - 1) / e->block_size - first + 1 : 0;
-  const at::Tensor rows = e->block_table.torchTensor().narrow(1, first, blocks).reshape({-1}).to(at::kLong);
-  auto tokens = [&](const at::Tensor& pool, bool dim_major) {
-    at::Tensor t = pool.index_select(0, rows);
-    if (dim_major) t = t.transpose(-1, -2);
-    const std::int64_t width = t.size(-1);
-    return t.reshape({e->batch, blocks, e->heads, e->block_size, width})
-        .transpose(1, 2)
-        .reshape({e->batch, e->heads, blocks * e->block_size, width})
-        .narrow(2, blocks > 0 ? start - first * e->block_size : 0, length);
+  std::pair<Tensor, Tensor> out;
+  auto gather = [&] {
+    const at::Tensor rows =
+        e->block_table.torchTensor().narrow(1, first, blocks).reshape({-1}).to(at::kLong);
+    auto tokens = [&](const at::Tensor& pool, bool dim_major) {
+      at::Tensor t = pool.index_select(0, rows);
+      if (dim_major) t = t.transpose(-1, -2);
+      const std::int64_t width = t.size(-1);
+      return t.reshape({e->batch, blocks, e->heads, e->block_size, width})
+          .transpose(1, 2)
+          .reshape({e->batch, e->heads, blocks * e->block_size, width})
+          .narrow(2, blocks > 0 ? start - first * e->block_size : 0, length);
+    };
+    at::Tensor k = tokens(e->key_pool.torchTensor(), false), v = tokens(e->value_pool.torchTensor(), true);
+    if (e->quantized()) {
+      const at::Tensor s = tokens(e->scales.torchTensor(), true);  // [B, H, tokens, 2]
+      k = dequantizeRows(k, s.select(-1, 0));
+      v = dequantizeRows(v, s.select(-1, 1));
+    }
+    out = {Tensor(k.to(toTorchDType(dtype)).contiguous()), Tensor(v.to(toTorchDType(dtype)).contiguous())};
   };
-  at::Tensor k = tokens(e->key_pool.torchTensor(), false), v = tokens(e->value_pool.torchTensor(), true);
-  if (e->quantized()) {
-    const at::Tensor s = tokens(e->scales.torchTensor(), true);  // [B, H, tokens, 2]
-    k = dequantizeRows(k, s.select(-1, 0));
-    v = dequantizeRows(v, s.select(-1, 1));
-  }
-  return {Tensor(k.to(toTorchDType(dtype)).contiguous()), Tensor(v.to(toTorchDType(dtype)).contiguous())};
+  // torch's operators, behind what the cache's stream still writes
+  if (e->key_pool.isCuda())
+    StreamScope::onTorch(stream_, e->key_pool.deviceId(), gather);
+  else
+    gather();
+  return out;
 }
 
 void KVCache::setLength(std::int64_t length) {

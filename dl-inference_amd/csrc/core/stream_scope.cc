@@ -50,4 +50,17 @@ void StreamScope::use(const at::Tensor& tensor, int device_id) {
                                       static_cast<c10::DeviceIndex>(device_id)));
 }
 
+void StreamScope::onTorch(void* stream, int device_id, const std::function<void()>& work) {
+  const auto device = static_cast<c10::DeviceIndex>(device_id);
+  const c10::hip::HIPStream before = c10::hip::getCurrentHIPStream(device);
+  if (static_cast<void*>(before.stream()) == stream) return work();
+  struct Restore {
+    c10::hip::HIPStream stream;
+    ~Restore() { c10::hip::setCurrentHIPStream(stream); }
+  } restore{before};
+  c10::hip::setCurrentHIPStream(
+      c10::hip::getStreamFromExternal(static_cast<hipStream_t>(stream), device));
+  work();
+}
+
 }  // namespace dli

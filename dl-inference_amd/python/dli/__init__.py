@@ -51,7 +51,8 @@ class Engine(_dli_native.Engine):
     def read_kv_cache(self, name, start, length, dtype="", stream=None):
         """Keys and values [B, H, length, D] that entry `name` holds at positions start .. start +
         length - 1 of every sequence, as `dtype` (the entry's own by default); zeros where nothing was
-        written."""
+        written. Device entries are read on `stream` (torch's current one by default), behind the runs
+        given the same one."""
         if stream is None:
             stream = 0
             entry = self.kv_cache_entry(name)

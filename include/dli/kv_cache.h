@@ -88,8 +88,8 @@ class KVCache {
   KVCacheEntry* find(const std::string& name);
 
   // Keys and values [B, H, length, D] that the entry holds at positions start .. start + length - 1 of
-  // every sequence, as `dtype`; zeros where nothing was written. Quantised entries on the device are
-  // read on the cache's stream, others on torch's current one.
+  // every sequence, as `dtype`; zeros where nothing was written. Device entries are read on the cache's
+  // stream.
   std::pair<Tensor, Tensor> read(const std::string& name, std::int64_t start, std::int64_t length,
                                  DType dtype);
 

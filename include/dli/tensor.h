@@ -10,6 +10,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <functional>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -94,6 +95,10 @@ class StreamScope {
   // that belongs to no capture, and an event recorded for the block would end up in the graph.
   static bool allowsScratch(int device_id);
   static void use(const at::Tensor& tensor, int device_id);
+
+  // Runs `work` with `stream` as torch's current one of the device: its operators run there, and what they
+  // allocate belongs to it.
+  static void onTorch(void* stream, int device_id, const std::function<void()>& work);
 
  private:
   void* previous_;
