@@ -125,18 +125,19 @@ struct AttentionPlan {
   int64_t splits;
 };
 
-// reach: tokens that a sequence holds at most, queries included.
+// reach: tokens that a sequence holds at most, queries included, as far as the host knows: all that its pages
+// take where the positions are on the device. phased: whether that kernel may be chosen.
 AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
-                            int64_t head_dim, int64_t block_size, int64_t max_blocks, int64_t reach) {
+                            int64_t head_dim, int64_t block_size, int64_t reach, bool phased = true) {
   const int64_t units = batch * kv_heads, rows = q_heads / kv_heads * seq_q;
   const bool paged = block_size % 64 == 0 || block_size == 16 || block_size == 32;
   // offsets within a page's head are 32 bits
   const bool near = block_size * head_dim < int64_t{1} << 31;
   if (dimIndex(head_dim) < 0 || !paged || !near || units > kMostGrid || units == 0 || rows >= kMostTokens)
     return {0, 0, 1};
-  const int64_t tiles = (block_size * max_blocks + 63) / 64;
+  const int64_t tiles = (reach + 63) / 64;
   if (rows <= 16) {
-    // About one workgroup of 8 waves per CU, each wave with a tile at least. Joining the splits is a
+    // About one workgroup of 8 waves per CU, each wave with a tile at least if the sequences are that long. Joining the splits is a
     // launch of its own, which costs more than two tiles to a wave: 1000 tokens of one sequence (14 / 2
     // heads x 64) 7.6 us undivided and 8.9 in 2 splits; 8 x 2000 (28 / 4 x 128) 18.6, 15.5 and, in 4, 12.2.
     // (Joined by the split that arrives last, in the same launch: 13.1 us for 32 x 4096 where two
@@ -157,7 +158,7 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
                    : dtype == DLI_F16 ? large >= 384 && head_dim == 128
                                       : 0;
   const auto blocksOf = [&](int s) { return units * ((rows + (int64_t{64} << s) - 1) / (int64_t{64} << s)); };
-  // keys split until two workgroups stand on every CU, each with 4 tiles at least; a split's results
+  // keys split until two workgroups stand on every CU, each with 4 tiles at least (as above); a split's results
   // are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4 heads
   // x 128: 37 us, 61 in two splits)
   const auto splitsOf = [&](int64_t blocks, int64_t places) {
@@ -167,7 +168,8 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
     splits = splits < 32 ? splits : 32;
     return splits > 1 ? splits : 1;
   };
-  if (dtype == DLI_BF16 && head_dim == 128 && size == 1 && block_size % 64 == 0 && reach > 2500) {
+  if (phased && dtype == DLI_BF16 && head_dim == 128 && size == 1 && block_size % 64 == 0 &&
+      reach > 2500) {
     // A phased workgroup has a CU to itself, so it pays over long contexts, where its first and last
     // steps count little, and where its rounds fill the card by two thirds. 128 rows and phased, us (28 / 4
     // heads): 2 x 1000 tokens over nothing 37 and 42, over 1000 67 and 72, 2000 101 and 96, 4000 170 and
@@ -278,9 +280,9 @@ size_t dli_hip_paged_attention_fp8_workspace(int64_t batch, int64_t q_heads, int
     return 0;
   int64_t splits = 1;  // the most of any data type and number of tokens held
   for (int dtype : {DLI_F32, DLI_BF16, DLI_F16}) {
-    for (int64_t reach : {int64_t{0}, block_size * max_blocks}) {
-      const AttentionPlan plan =
-          attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks, reach);
+    for (bool phased : {false, true}) {
+      const AttentionPlan plan = attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size,
+                                               block_size * max_blocks, phased);
       splits = splits > plan.splits ? splits : plan.splits;
     }
   }
@@ -311,7 +313,7 @@ int dli_hip_paged_attention_fp8(int dtype, const void* q, const void* key_codes,
   const int64_t reach =
       positions != nullptr || before >= capacity || before + seq_q > capacity ? capacity : before + seq_q;
   AttentionPlan plan =
-      attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, max_blocks, reach);
+      attentionPlan(dtype, batch, q_heads, kv_heads, seq_q, head_dim, block_size, reach);
   // the MFMA forms take 16-byte loads and put masked scores to -inf before the scale's sign could
   // matter, as the other attention kernels do
   if (!(scale > 0.f) || !std::isfinite(scale) || !aligned16(q) || !aligned16(out) ||

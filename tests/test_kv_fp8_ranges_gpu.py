@@ -309,3 +309,17 @@ def test_values_far_apart_in_chunks(dtype, dim, q_heads, seq, block, kind, octav
 def test_values_far_apart_over_long_contexts(kind, octaves, block):
     """The same where two halves of a workgroup run a phase apart (16800 rows of a pair, up to 2688 tokens)."""
     far_apart(kind, "bfloat16", 128, 14, 1200, octaves, min(octaves + 2, 14), block=block, tokens=2688)
+
+
+@pytest.mark.parametrize("dim,q_heads,seq", [(64, 14, 1), (128, 14, 1), (64, 14, 20), (128, 14, 20)])
+def test_short_sequences_in_long_tables(dim, q_heads, seq):
+    """Where the host knows that few tokens are held, keys are not split over workgroups that would find none:
+    the workspace is left as it was, and results are those of a short table."""
+    pools = Pools(1, 2, dim, 64, 300, seed=1).cuda()
+    q = torch.randn((1, q_heads, seq, dim), generator=rng(1)).bfloat16().cuda()
+    ws = workspace(pools, q)
+    assert ws.numel() > 0
+    out = attend(pools, q, 200, ws=ws)
+    assert (ws == 255).all()
+    pools.max_blocks, pools.table = 4, pools.table[:, :4].contiguous()
+    assert torch.equal(attend(pools, q, 200), out)
