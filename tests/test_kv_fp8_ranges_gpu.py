@@ -2,6 +2,7 @@
 and queries. Expected values are exact or float64; inputs are chosen so that fp32 sums are exact."""
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
@@ -194,8 +195,9 @@ def dense(pools, tokens):
     return k * unit[:, 0].flatten()[:tokens, None], v, unit[:, 1].flatten()[:tokens]
 
 
-def check_far_apart(out, pools, q, past, scale, near=0):
-    """out [1, Hq, S, D] of queries [1, Hq, S, D] (causal), one KV head, against float64. Off by at most: the
+def check_far_apart(out, pools, q, past, scale, near=0, missing=()):
+    """out [1, Hq, S, D] of queries [1, Hq, S, D] (causal), one KV head, against float64; missing: pages of the
+    table that hold nothing, though `pools` has them. Off by at most: the
     output's rounding; per weight its rounding (f16 once, or 22 bits) and the shift of its score by fp32's
     sum of D products, scaling and exponent; the sums' roundings; and f16's half least step, 2^-25 with 2^11
     or more at the row's largest weight times value scale, for every token's elements. Chunks count
@@ -205,6 +207,8 @@ def check_far_apart(out, pools, q, past, scale, near=0):
     k, v, unit = dense(pools, past + q.shape[2])
     s = q[0].double() @ k.T * scale
     limit = past + 1 + torch.arange(q.shape[2], device="cuda")
+    for page in missing:
+        s[..., page * pools.block:(page + 1) * pools.block] = -math.inf
     s = s.masked_fill(torch.arange(len(k), device="cuda") >= limit[:, None], -math.inf)
     w = torch.exp(s - s.amax(-1, keepdim=True))
     total = w.sum(-1, keepdim=True)
@@ -323,3 +327,89 @@ def test_short_sequences_in_long_tables(dim, q_heads, seq):
     assert (ws == 255).all()
     pools.max_blocks, pools.table = 4, pools.table[:, :4].contiguous()
     assert torch.equal(attend(pools, q, 200), out)
+
+
+def without(pools, missing):
+    """`pools` with those pages taken out of the table."""
+    bare = copy.copy(pools)
+    bare.table = pools.table.clone()
+    bare.table[0, list(missing)] = -1
+    return bare
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("dim,block,tokens", [(64, 16, 8400), (128, 16, 17000), (64, 32, 17000), (128, 32, 25000),
+                                              (64, 64, 33000), (128, 64, 66000)])
+def test_single_tokens_over_many_pages(dtype, dim, block, tokens):
+    """Keys that are not split: each wave of a workgroup goes through more pages than it has lanes to hold their
+    ids, up to two times over. The weight lies on pages at both sides of where it reads more, and some of them
+    hold nothing."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, block, -(-tokens // block), seed=block).cuda()
+    q = torch.randn((1, 3, 1, dim), generator=rng(1)).to(t)
+    per = 64 // block if block < 64 else 1  # pages a tile
+    runs = 8 * (64 if block == 64 else 16)  # tiles before ids are read anew
+    missing = [p for k in (1, 2) for p in (k * runs * per - 1, k * runs * per + 3, k * runs * per + 9 * per)
+               if p < -(-tokens // block)] + [2, 0]
+    pools.key[..., 0] = 0
+    for page in missing:
+        near = pools.table[0, max(page - 1, 0):page + 2].long()
+        pools.key[near, :, :, 0] = code(448.0)
+        pools.scales[near, :, 0] = 120  # 3.5 in the cache: weights of e^8 and more
+    q[..., 0] = 20.0
+    out = attend(without(pools, missing), q.cuda(), tokens - 1)
+    check_far_apart(out, pools, q, tokens - 1, dim ** -0.5, 0, missing)
+
+
+@pytest.mark.parametrize("dtype,dim,q_heads,seq", [("bfloat16", 128, 14, 1200), ("float16", 128, 4, 100),
+                                                   ("bfloat16", 64, 14, 1200), ("float32", 128, 4, 1),
+                                                   ("bfloat16", 128, 8, 2)])
+def test_pages_past_32_bits(dtype, dim, q_heads, seq):
+    """A sequence whose pages lie behind 2^32 bytes of each pool, in every form that goes by pages."""
+    t = DTYPES[dtype]
+    n = (1 << 32) // (64 * dim) + 60
+    small = Pools(1, 1, dim, 64, 42, seed=5, spare=0)
+    pools = copy.copy(small)
+    shapes = {"key": (n, 1, 64, dim), "value": (n, 1, dim, 64), "scales": (n, 1, 2, 64)}
+    for name, shape in shapes.items():
+        pool = torch.empty(shape, dtype=torch.uint8, device="cuda")
+        pool[n - 42:] = getattr(small, name).cuda()
+        setattr(pools, name, pool)
+    pools.table, pools.count = (small.table + n - 42).cuda(), n
+    q = torch.randn((1, q_heads, seq, dim), generator=rng(seq)).to(t)
+    for ws in (None, workspace(pools, q)):
+        out = attend(pools, q.cuda(), [1400], ws=ws)
+        check_far_apart(out, small, q, 1400, dim ** -0.5, 14)
+
+
+# (dtype, head_dim, query heads, queries, tokens of a page, tokens of the table)
+MIXED = [("bfloat16", 64, 7, 2, 64, 1920), ("float32", 128, 4, 4, 16, 1920), ("float16", 80, 2, 3, 64, 1920)]
+MIXED += [(*c, 1920) for c in CHUNKS if c[3] < 1200 or c[4] == 32]
+MIXED += [("bfloat16", 64, 14, 1200, 64, 1920), ("bfloat16", 128, 14, 1200, 128, 2688)]
+
+
+@pytest.mark.parametrize("dtype,dim,q_heads,seq,block,tokens", MIXED)
+@pytest.mark.parametrize("octaves", [8, 110])
+@pytest.mark.parametrize("side", [0, 1])
+def test_holes_zeros_and_nan_among_values_far_apart(dtype, dim, q_heads, seq, block, tokens, octaves, side):
+    """Pages that hold nothing (with scales of any size), rows of zeros, and a token that is not finite and
+    that only the last query sees."""
+    t = DTYPES[dtype]
+    pools, q = apart("ladder", dtype, dim, q_heads, seq, octaves, block, tokens)
+    missing = [3, 9, 700 // block - 1]
+    for page in missing:
+        pools.scales[int(pools.table[0, page])] = torch.tensor([7, 250], dtype=torch.uint8).view(2, 1)
+    for pos in (0, 77, 699, 700):
+        page, slot = token(pools, 0, pos)
+        pools.value[page, 0, :, slot] = 0
+        pools.scales[page, 0, 1, slot] = 0
+    page, slot = token(pools, 0, 700 + seq - 1)
+    pools.key[page, 0, slot] = pools.value[page, 0, :, slot] = 0
+    pools.scales[page, 0, side, slot] = 255
+    q = q.to(t)
+    pools.cuda()
+    bare = without(pools, missing)
+    for space in (None, workspace(pools, q)):
+        out = attend(bare, q.cuda(), [700], scale=math.log(2), ws=space)
+        assert out[:, :, -1].isnan().all()
+        check_far_apart(out[:, :, :-1], pools, q[:, :, :-1], 700, math.log(2), 14, missing)
