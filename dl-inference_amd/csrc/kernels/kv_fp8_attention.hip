@@ -1486,7 +1486,17 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
   const float f = (m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M)) * l;
   const float L = waveSum(f);
   // divided before they meet the values: a sum of L times a value may pass the largest number
-  const float share = L == 0.f ? 0.f : f / L;
+  float share = L == 0.f ? 0.f : f / L;
+  // a share below what fp32 holds may meet values that make up for it: half of its exponent first
+  const bool small = m - M < -100.f && m != -INFINITY;
+  float half = 1.f;
+  const bool any_small = __builtin_amdgcn_ballot_w64(small) != 0;
+  if (any_small) {
+    rarely();
+    const float h = __builtin_amdgcn_exp2f(0.5f * (m - M));
+    half = small ? h : 1.f;
+    share = small ? h * (l / L) : share;
+  }
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < a.splits; s0 += kDepth * kAtOnce) {
     if (s0 > 0) load(s0);
@@ -1494,6 +1504,10 @@ __device__ __forceinline__ void kv8_merge(const Kv8AttentionArgs& a) {
     for (int u = 0; u < kDepth; ++u) {
       const int s = s0 + u * kAtOnce + mine;
       const float w = __shfl(share, s % kWave, kWave);
+      if (any_small) {
+        rarely();
+        x[u] *= __shfl(half, s % kWave, kWave);
+      }
       if (s < a.splits) acc += x[u] * w;
     }
   }

@@ -413,3 +413,28 @@ def test_holes_zeros_and_nan_among_values_far_apart(dtype, dim, q_heads, seq, bl
         out = attend(bare, q.cuda(), [700], scale=math.log(2), ws=space)
         assert out[:, :, -1].isnan().all()
         check_far_apart(out[:, :, :-1], pools, q[:, :, :-1], 700, math.log(2), 14, missing)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim,q_heads,seq", FORMS[:5] + [(128, 4, 40), (80, 2, 3), (128, 14, 300)])
+@pytest.mark.parametrize("octaves", [90, 140, 200, 230])
+def test_splits_far_apart(dtype, dim, q_heads, seq, octaves):
+    """The first 1024 tokens have weights of 2^-octaves and values 2^octaves as large as the others': the
+    splits that hold only them count as much as the rest."""
+    t = DTYPES[dtype]
+    pools = Pools(1, 1, dim, 64, 30, seed=octaves)
+    pools.key[:] = 0
+    pools.scales[:, :, 0] = 127
+    pools.scales[:, :, 1] = 10
+    for page in pools.table[0, :16].long():
+        pools.key[page, 0, :, 0] = code(-1.0)
+        pools.key[page, 0, :, 1] = code(-0.5)
+        pools.scales[page, 0, 1] = 10 + octaves
+    q = torch.zeros((1, q_heads, seq, dim))
+    q[..., 0] = octaves - octaves % 4 - 2
+    q[..., 1] = 2 * (octaves % 4 + 2)  # octaves in all, exact in 16 bits
+    q = q.to(t)
+    pools.cuda()
+    for space in (None, workspace(pools, q)):
+        out = attend(pools, q.cuda(), [1500], scale=math.log(2), ws=space)
+        check_far_apart(out, pools, q, 1500, math.log(2), 0)
