@@ -313,7 +313,7 @@ __device__ __forceinline__ int64_t outAt(const Kv8AttentionArgs& a, int64_t b, R
 //
 // Long calls are bound by the stream of the cache: 64 sequences of 8192 tokens (28 / 4 heads x 128) 83 us,
 // 511 MB at 6.2 TB/s (part of it from the 256 MB cache). Short ones by latency: 32 of 4096 (14 / 2 x 64)
-// 13.1 us, 32 MB, of which two launches take 7.4; one of 1000 tokens 7.5, three trips to memory (table and
+// 13.0 us, 32 MB, of which two launches take 7.4; one of 1000 tokens 7.6, three trips to memory (table and
 // position, the tile, the store) and a join of 8 waves.
 // ---------------------------------------------------------------------------------------------
 constexpr int kDecWaves = 8;
@@ -342,7 +342,9 @@ struct KeyTile {
 template <class T, int D>
 struct DecodeLds {
   // q's terms where there are several: in registers they would push the tiles out (fp32, head_dim 128,
-  // 64 sequences of 4096 tokens: 80.7 us with 43 registers spilled, 48.8 so)
+  // 64 sequences of 4096 tokens: 80.7 us with 43 registers spilled, 50 so). The same of what a row has
+  // beside them: the wait for a register that comes back from memory is one for the tile on its way (10 of
+  // them: 57).
   U128 q[Kv8Type<T>::kQ > 1 ? D / 64 * 2 * Kv8Type<T>::kQ : 1][kWave];
   float row_scale[kWave];
   int lim[kWave];
@@ -591,7 +593,7 @@ __device__ __forceinline__ void kv8_decode(const Kv8AttentionArgs& a) {
 // chunks permuted by dim so that the 16 rows of a fragment read fall on distinct banks. One barrier a
 // tile: two buffers, and two workgroups on a CU that need not keep step.
 //
-// 2048 tokens over 8192 (28 / 4 heads x 128, bf16) take 339 us, 270 GFLOP at 798 TFLOP/s (290 phased, below).
+// 2048 tokens over 8192 (28 / 4 heads x 128, bf16) take 339 us, 270 GFLOP at 798 TFLOP/s (291 phased, below).
 // No unit is full: MFMA 33% busy, vector instructions 43%, LDS 33% (a quarter of it conflicts); a wave waits
 // for its own chain (scores, weights, products) and for the tile, and two waves a SIMD hide half of
 // that. Left out one at a time, staging saves 100 us, the softmax 60, the loads 42. Tried, in us: 64 rows a
@@ -1107,7 +1109,7 @@ __device__ __forceinline__ void kv8_chunk(const Kv8AttentionArgs& a) {
 // A tile's buffers are written by both halves in their M(kt - 1), two phases in a row, and read in their M of
 // the keys' tile, or the one after for values: each has two. Wave priority goes with the matrix phase.
 //
-// 2048 tokens over 8192 (28 / 4 heads x 128) 290 us, 933 TFLOP/s; above 339. A phase takes 1800 cycles
+// 2048 tokens over 8192 (28 / 4 heads x 128) 291 us, 930 TFLOP/s; above 339. A phase takes 1800 cycles
 // either way (products alone: 1455, of which the unit needs 1088). Steps, in us: everything staged in the
 // softmax phase 357, between the products 416, the scales read by their users and page offsets in 32 bits
 // 335, priority 309, loads issued in the softmax phase 295.

@@ -641,12 +641,15 @@ int dli_hip_kv_read_fp8(int dtype, const void* key_codes, const void* value_code
 /* Attention of q [batch, q_heads, seq_q, head_dim] over the cache, seq_q >= 1, as
  * dli_hip_paged_attention: sequence b holds past + seq_q tokens (positions[b] + seq_q), the query at
  * index i sits at position past + i and, when causal, sees keys at positions <= past + i. A query
- * that sees no token, or whose every score is -infinity, gets zeros. out is [batch, q_heads, seq_q, head_dim], with out_bshd
- * [batch, seq_q, q_heads, head_dim]. A row that sees a NaN token is NaN. Elements must be those that
+ * that sees no token, or whose every score is -infinity, gets zeros. Tokens that a query does not see do not
+ * count, whatever their values; next to values 2^14 larger in the same call, more than 16 rows of a (sequence,
+ * KV head) pair may take tokens whose values are all below 2^-118 for zeros. out is [batch, q_heads, seq_q,
+ * head_dim], with out_bshd [batch, seq_q, q_heads, head_dim]. A row that sees a NaN token is NaN. Elements must be those that
  * the appends write (not e4m3's own NaN, 0x7F and 0xFF), but for tokens that no query sees.
  * A workspace of dli_hip_paged_attention_fp8_workspace bytes, 16-byte aligned and of any content, lets
  * the keys of a row be split over workgroups, their results joined in a fixed order; a smaller one or
- * NULL means fewer splits. Two calls that may run at once need one each. */
+ * NULL means fewer splits. Two calls that may run at once need one each. How a call is split goes by past + seq_q
+ * where positions is NULL, else by what the table's pages take. */
 size_t dli_hip_paged_attention_fp8_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                              int64_t seq_q, int64_t head_dim, int64_t block_size,
                                              int64_t max_blocks);
