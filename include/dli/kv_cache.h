@@ -29,7 +29,7 @@
 //   scales [num_blocks, heads, 2, block_size]   the keys', then the values'
 //
 // Every reader of such an entry sees what it holds: a prompt's own queries attend over the quantised
-// keys and values too, so results do not depend on how a prompt is cut into runs. The quantisation
+// keys and values too, so results depend on how a prompt is cut into runs by roundings only. The quantisation
 // rule is that of dli_hip_kv_append_fp8 (include/dli_hip.h).
 
 #include <cstdint>
