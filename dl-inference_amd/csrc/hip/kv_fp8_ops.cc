@@ -137,11 +137,11 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
     return {0, 0, 1};
   const int64_t tiles = (reach + 63) / 64;
   if (rows <= 16) {
-    // About one workgroup of 8 waves per CU, each wave with a tile at least if the sequences are that long. Joining the splits is a
-    // launch of its own, which costs more than two tiles to a wave: 1000 tokens of one sequence (14 / 2
-    // heads x 64) 7.6 us undivided and 8.9 in 2 splits; 8 x 2000 (28 / 4 x 128) 18.6, 15.5 and, in 4, 12.2.
-    // (Joined by the split that arrives last, in the same launch: 13.1 us for 32 x 4096 where two
-    // launches take 12.6, and 20.6 for 16 splits where they take 11.5.)
+    // About one workgroup of 8 waves per CU, each wave with a tile at least if the sequences are that
+    // long. Joining the splits is a launch of its own, which costs more than two tiles to a wave: 1000
+    // tokens of one sequence (14 / 2 heads x 64) 7.6 us undivided and 8.9 in 2 splits; 8 x 2000 (28 / 4 x
+    // 128) 18.6, 15.5 and, in 4, 12.2. (Joined by the split that arrives last, in the same launch: 13.1 us
+    // for 32 x 4096 where two launches take 12.6, and 20.6 for 16 splits where they take 11.5.)
     if (tiles <= 16) return {1, 0, 1};
     int64_t splits = (256 + units - 1) / units;
     const int64_t most = (tiles + 7) / 8;
@@ -158,9 +158,9 @@ AttentionPlan attentionPlan(int dtype, int64_t batch, int64_t q_heads, int64_t k
                    : dtype == DLI_F16 ? large >= 384 && head_dim == 128
                                       : 0;
   const auto blocksOf = [&](int s) { return units * ((rows + (int64_t{64} << s) - 1) / (int64_t{64} << s)); };
-  // keys split until two workgroups stand on every CU, each with 4 tiles at least (as above); a split's results
-  // are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4 heads
-  // x 128: 37 us, 61 in two splits)
+  // keys split until two workgroups stand on every CU, each with 4 tiles at least (as above); a split's
+  // results are written and read again, so none where the rows fill the card (2 x 1000 prompt tokens, 28 / 4
+  // heads x 128: 37 us, 61 in two splits)
   const auto splitsOf = [&](int64_t blocks, int64_t places) {
     int64_t splits = places / blocks;
     const int64_t most = tiles / 4;

@@ -644,8 +644,8 @@ int dli_hip_kv_read_fp8(int dtype, const void* key_codes, const void* value_code
  * that sees no token, or whose every score is -infinity, gets zeros. Tokens that a query does not see do not
  * count, whatever their values; next to values 2^14 larger in the same call, more than 16 rows of a (sequence,
  * KV head) pair may take tokens whose values are all below 2^-118 for zeros. out is [batch, q_heads, seq_q,
- * head_dim], with out_bshd [batch, seq_q, q_heads, head_dim]. A row that sees a NaN token is NaN. Elements must be those that
- * the appends write (not e4m3's own NaN, 0x7F and 0xFF), but for tokens that no query sees.
+ * head_dim], with out_bshd [batch, seq_q, q_heads, head_dim]. A row that sees a NaN token is NaN. Elements must
+ * be those that the appends write (not e4m3's own NaN, 0x7F and 0xFF), but for tokens that no query sees.
  * A workspace of dli_hip_paged_attention_fp8_workspace bytes, 16-byte aligned and of any content, lets
  * the keys of a row be split over workgroups, their results joined in a fixed order; a smaller one or
  * NULL means fewer splits. Two calls that may run at once need one each. How a call is split goes by past + seq_q
